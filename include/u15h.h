@@ -538,6 +538,85 @@ u15h_status u15h_mot_gemm_i8(u15h_ctx* ctx, u15h_stream stream,
                              int nproj);
 
 /* ------------------------------------------------------------------ */
+/* fp8 tier: e4m3 with a scale for each block of 128                    */
+/* ------------------------------------------------------------------ */
+
+/* Codes are OCP e4m3 (one byte; largest value 448).  K is cut in blocks of
+ * 128 columns, KB = ceil(K / 128) of them, the last one shorter where 128
+ * does not divide K.  Activations have one f32 scale per row and block,
+ * stored BLOCK-MAJOR, s[KB][rows]; weights one per 128 x 128 block,
+ * s[ceil(N / 128)][KB] (the layout of fp8 checkpoints' inverse scales).
+ * For the values v of a block, in f32:
+ *   a = max |v|,   s = max(a / 448, 2^-126),   code = e4m3_rne(v * (1 / s))
+ * A block with a NaN has the scale NaN, one with an infinity the scale
+ * infinity: what is restored from either is NaN.  A block of zeros has the
+ * least scale and codes 0.  No reference counterpart (its quantised tiers
+ * are affine packs and int8).  Widths (K, dim, inter) are multiples of 16,
+ * so that every row of codes starts 16-byte aligned; no call allocates. */
+
+/* Codes q [rows][K] and scales s [KB][rows] of bf16 activations x
+ * [rows][K].  K <= 131072, rows <= 2^24. */
+u15h_status u15h_quant_rows_fp8(u15h_ctx* ctx, u15h_stream stream,
+                                const u15h_bf16* x, int rows, int K,
+                                uint8_t* q, float* s);
+
+/* Codes q [N][K] and scales s [ceil(N / 128)][KB] of a bf16 weight w
+ * [N][K].  K <= 131072, N <= 2^20. */
+u15h_status u15h_quant_blocks_fp8(u15h_ctx* ctx, u15h_stream stream,
+                                  const u15h_bf16* w, int N, int K,
+                                  uint8_t* q, float* s);
+
+/* u15h_mot_rms_norm with the fp8 tier's output: for rows [0, M_und) with
+ * w_und and the next M_gen rows with w_gen,
+ *   r = bf16(x + delta) when delta is given, stored to x_out; else r = x
+ *   n = (r * inv) * w,  inv = 1/sqrt(mean(r^2) + eps)           in f32
+ *   q [rows][dim], s [KB][rows] = the codes and scales of n
+ *   y [rows][dim] = bf16(n)                       (when y is not NULL)
+ * The codes are those of the f32 values, rounded once (not of y).  x_out
+ * may be x (the residual stream updated in place); delta and x_out are
+ * given together or not at all; y must not be x_out.  dim <= 16384,
+ * eps >= 0. */
+u15h_status u15h_mot_rms_norm_fp8(u15h_ctx* ctx, u15h_stream stream,
+                                  const u15h_bf16* x, const u15h_bf16* delta,
+                                  u15h_bf16* x_out, int M_und, int M_gen,
+                                  int dim, const u15h_bf16* w_und,
+                                  const u15h_bf16* w_gen, float eps,
+                                  u15h_bf16* y, uint8_t* q, float* s);
+
+/* The down projection's fp8 input in one pass: h = silu(gate) * up in f32,
+ * its codes q [rows][inter] and scales s [ceil(inter / 128)][rows] (of the
+ * f32 values, rounded once), and bf16(h) where h is not NULL.
+ * inter <= 131072, rows <= 2^24. */
+u15h_status u15h_swiglu_quant_fp8(u15h_ctx* ctx, u15h_stream stream,
+                                  const u15h_bf16* gate, const u15h_bf16* up,
+                                  int rows, int inter, u15h_bf16* h,
+                                  uint8_t* q, float* s);
+
+/* One fp8 projection: the codes and block scales of both weight sets, and
+ * the output. */
+typedef struct {
+  const uint8_t* wq_und;  /* [N][K]                */
+  const float*   sw_und;  /* [ceil(N / 128)][KB]   */
+  const uint8_t* wq_gen;  /* [N][K]                */
+  const float*   sw_gen;  /* [ceil(N / 128)][KB]   */
+  u15h_bf16*     y;       /* [M_und + M_gen][N]    */
+  int            N;
+} u15h_mot_proj_fp8;
+
+/* The two-group grouped GEMM over fp8 codes, u15h_mot_gemm_i8's twin: rows
+ * [0, M_und) take the und weights, the next M_gen rows the gen weights, and
+ * with b the blocks of K
+ *   y[m][n] = bf16( sum_b (sx[b][m] * sw[n / 128][b]) *
+ *                         sum_{k in b} xq[m][k] * wq[n][k] )
+ * with f32 sums.  xq [M][K], sx [KB][M] over the rows of both groups.
+ * Limits: 1 <= nproj <= U15H_MAX_PROJ, K % 16 == 0, K <= 131072,
+ * N % 8 == 0, N <= 2^20, M_und + M_gen <= 2^24. */
+u15h_status u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream,
+                              const uint8_t* xq, const float* sx, int M_und,
+                              int M_gen, int K, const u15h_mot_proj_fp8* proj,
+                              int nproj);
+
+/* ------------------------------------------------------------------ */
 /* The resident MoT layer stack                                        */
 /* ------------------------------------------------------------------ */
 

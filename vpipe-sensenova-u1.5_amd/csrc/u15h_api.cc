@@ -747,6 +747,24 @@ u15h::set_error(u15h_ctx* ctx, u15h_status st, const char* msg)
   return fail(ctx, st, "%s", msg);
 }
 
+u15h_status
+u15h::begin_call(u15h_ctx* ctx)
+{
+  return bind_device(ctx);
+}
+
+u15h_status
+u15h::end_call(u15h_ctx* ctx, hipError_t e, const char* what)
+{
+  return launched(ctx, e, what);
+}
+
+int
+u15h::num_cus(const u15h_ctx* ctx)
+{
+  return ctx->num_cu;
+}
+
 extern "C" {
 
 int

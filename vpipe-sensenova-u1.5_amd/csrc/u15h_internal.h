@@ -262,6 +262,59 @@ hipError_t launch_f32_to_bf16(const float* src, int64_t n, uint16_t* dst,
 hipError_t launch_gather_rows(const uint16_t* src, const int32_t* perm,
                               int M, int cols, uint16_t* dst, bool scatter,
                               hipStream_t s);
+// ---- fp8 (e4m3) with a scale for each block of 128 (u15h_fp8.hip) ----------
+constexpr int kFp8Block = 128;
+// One GEMM of an fp8 batch: y[rows][n] = a[rows][K] . w[n][K]^T, the codes
+// scaled per activation row and per 128 weight rows for each 128 of K.
+struct Fp8Problem {
+  const uint8_t* a;       // activation codes [rows][K]
+  const float*   sa;      // their scales: block b's row r at sa[b * sa_pitch + r]
+  const uint8_t* w;       // weight codes [n][K]
+  const float*   sw;      // their scales [ceil(n / 128)][blocks of K]
+  uint16_t*      y;       // [rows][n]
+  int rows;
+  int n;
+  int tiles_m;
+  int tiles_n;
+  int tile_begin;         // first linear tile index of this problem
+};
+struct Fp8Batch {
+  Fp8Problem p[kMaxProb];
+  int nprob;
+  int K;                  // % 16 == 0
+  int sa_pitch;           // rows of the whole call
+  int total_tiles;
+};
+hipError_t launch_fp8_gemm(const Fp8Batch& b, hipStream_t s);
+// Codes [rows][K] and scales [ceil(K / 128)][rows] of bf16 rows, or with `up`
+// of silu(x) * up, whose bf16 values go to h where that is not null.
+hipError_t launch_fp8_quant_rows(const uint16_t* x, const uint16_t* up, int rows, int K,
+                                 uint16_t* h, uint8_t* q, float* sc, hipStream_t s);
+// Codes [N][K] and scales [ceil(N / 128)][ceil(K / 128)] of a bf16 weight.
+hipError_t launch_fp8_quant_blocks(const uint16_t* w, int N, int K, uint8_t* q, float* sc,
+                                   hipStream_t s);
+// The residual add (d and x_out both or neither), RMSNorm and codes of rows.
+struct Fp8NormArgs {
+  const uint16_t* x;
+  const uint16_t* d;
+  uint16_t* x_out;
+  const uint16_t* w_und;
+  const uint16_t* w_gen;
+  uint16_t* y;            // or null
+  uint8_t* q;
+  float* sc;
+  int m_und, rows, dim;
+  float eps;
+};
+hipError_t launch_fp8_norm(const Fp8NormArgs& a, hipStream_t s);
+bool fp8_kernels_loadable();
+
+// What entry points outside u15h_api.cc need of the context: the device made
+// current; a launch's result as the call's status; the number of CUs.
+u15h_status begin_call(u15h_ctx* ctx);
+u15h_status end_call(u15h_ctx* ctx, hipError_t e, const char* what);
+int num_cus(const u15h_ctx* ctx);
+
 // Forces every kernel's code object to load; false if any cannot.
 bool kernels_loadable();
 

@@ -52,6 +52,12 @@ class _MotProjI8(ctypes.Structure):
                 ("y", ctypes.c_void_p), ("N", ctypes.c_int)]
 
 
+class _MotProjFp8(ctypes.Structure):
+    _fields_ = [("wq_und", ctypes.c_void_p), ("sw_und", ctypes.c_void_p),
+                ("wq_gen", ctypes.c_void_p), ("sw_gen", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("N", ctypes.c_int)]
+
+
 class _LayerIO(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in
                 ("x", "q", "k", "v", "attn", "o", "x2", "gate", "up", "h",
@@ -120,6 +126,13 @@ def load_library() -> ctypes.CDLL:
                                      ctypes.POINTER(_MotProjI8), i]),
         "u15h_mot_gemm_i8": (i, [vp, vp, vp, vp, i, i, i,
                                  ctypes.POINTER(_MotProjI8), i]),
+        "u15h_quant_rows_fp8": (i, [vp, vp, vp, i, i, vp, vp]),
+        "u15h_quant_blocks_fp8": (i, [vp, vp, vp, i, i, vp, vp]),
+        "u15h_mot_rms_norm_fp8": (i, [vp, vp, vp, vp, vp, i, i, i, vp, vp,
+                                      ctypes.c_float, vp, vp, vp]),
+        "u15h_swiglu_quant_fp8": (i, [vp, vp, vp, vp, i, i, vp, vp, vp]),
+        "u15h_mot_gemm_fp8": (i, [vp, vp, vp, vp, i, i, i,
+                                  ctypes.POINTER(_MotProjFp8), i]),
         "u15h_route_rows": (i, [vp, i, vp, ctypes.POINTER(i),
                                 ctypes.POINTER(i)]),
         "u15h_dequant_affine": (i, [vp, vp, ctypes.POINTER(_QWeight), i, i,
@@ -545,6 +558,11 @@ def _need(t, dtype, shape, name):
         raise ValueError(f"{name} must be on the GPU")
 
 
+def _blocks(n):
+    """Blocks of 128 (the last one maybe shorter) in n."""
+    return (n + 127) // 128
+
+
 def layer_scratch(stack, M, tier=TIER_BF16, device="cuda"):
     """The scratch buffers of u15h_stack_layer_full for M rows."""
     def bf(n):
@@ -815,6 +833,136 @@ class Ops:
         self._check(st, "u15h_mot_gemm_i8")
 
     # ---- profiling -------------------------------------------------------
+    # ---- fp8 tier ------------------------------------------------------
+    def _stream_here(self, stream):
+        """The call's stream: the current one of this context's device."""
+        if stream is not None:
+            return stream.cuda_stream
+        if _raw_stream is not None and torch.cuda.is_initialized():
+            return _raw_stream(self.device)
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _need_here(self, t, dtype, shape, name):
+        """_need, and that the tensor is on this context's device."""
+        _need(t, dtype, shape, name)
+        if t.get_device() != self.device:
+            raise ValueError(f"{name} is on cuda:{t.get_device()}, this context on "
+                             f"cuda:{self.device}")
+
+    def quant_rows_fp8(self, x, q, s, stream=None):
+        """e4m3 codes q [rows][K] of x and their scales s [blocks of
+        K][rows], one per row and 128 columns."""
+        if x.dim() != 2:
+            raise ValueError("x must be [rows][K]")
+        rows, K = x.shape
+        self._need_here(x, torch.bfloat16, (rows, K), "x")
+        self._need_here(q, torch.float8_e4m3fn, (rows, K), "q")
+        self._need_here(s, torch.float32, (_blocks(K), rows), "s")
+        st = self._lib.u15h_quant_rows_fp8(self._ctx, self._stream_here(stream), x.data_ptr(),
+                                           rows, K, q.data_ptr(), s.data_ptr())
+        if st:
+            self._check(st, "u15h_quant_rows_fp8")
+
+    def quant_blocks_fp8(self, w, q, s, stream=None):
+        """e4m3 codes q [N][K] of a weight and their scales s [blocks of
+        N][blocks of K], one per 128 x 128."""
+        if w.dim() != 2:
+            raise ValueError("w must be [N][K]")
+        N, K = w.shape
+        self._need_here(w, torch.bfloat16, (N, K), "w")
+        self._need_here(q, torch.float8_e4m3fn, (N, K), "q")
+        self._need_here(s, torch.float32, (_blocks(N), _blocks(K)), "s")
+        st = self._lib.u15h_quant_blocks_fp8(self._ctx, self._stream_here(stream),
+                                             w.data_ptr(), N, K, q.data_ptr(), s.data_ptr())
+        if st:
+            self._check(st, "u15h_quant_blocks_fp8")
+
+    def mot_rms_norm_fp8(self, x, M_und, M_gen, w_und, w_gen, q, s, delta=None, x_out=None,
+                         y=None, eps=1e-6, stream=None):
+        """u15h_mot_rms_norm_fp8: with `delta`, r = x + delta first, stored
+        to x_out (x itself where none is given); then q, s = the codes and
+        scales of the norm of r's rows (w_und for the first M_und, w_gen for
+        the rest), and y = the norm in bf16 when given."""
+        rows = M_und + M_gen
+        if x.dim() != 2 or x.shape[0] != rows:
+            raise ValueError(f"x must be [{rows}][dim]")
+        dim = x.shape[1]
+        self._need_here(x, torch.bfloat16, (rows, dim), "x")
+        if M_und:
+            self._need_here(w_und, torch.bfloat16, (dim,), "w_und")
+        if M_gen:
+            self._need_here(w_gen, torch.bfloat16, (dim,), "w_gen")
+        self._need_here(q, torch.float8_e4m3fn, (rows, dim), "q")
+        self._need_here(s, torch.float32, (_blocks(dim), rows), "s")
+        if delta is not None:
+            self._need_here(delta, torch.bfloat16, (rows, dim), "delta")
+            if x_out is None:
+                x_out = x
+        elif x_out is not None:
+            raise ValueError("x_out is written only with delta")
+        if x_out is not None:
+            self._need_here(x_out, torch.bfloat16, (rows, dim), "x_out")
+        if y is not None:
+            self._need_here(y, torch.bfloat16, (rows, dim), "y")
+        st = self._lib.u15h_mot_rms_norm_fp8(
+            self._ctx, self._stream_here(stream), x.data_ptr(), _ptr(delta), _ptr(x_out), M_und,
+            M_gen, dim, _ptr(w_und), _ptr(w_gen), eps, _ptr(y), q.data_ptr(), s.data_ptr())
+        if st:
+            self._check(st, "u15h_mot_rms_norm_fp8")
+
+    def swiglu_quant_fp8(self, gate, up, q, s, h=None, stream=None):
+        """e4m3 codes q [rows][inter] of silu(gate) * up and their scales s
+        [blocks of inter][rows] (and h in bf16 when given)."""
+        if gate.dim() != 2:
+            raise ValueError("gate must be [rows][inter]")
+        rows, inter = gate.shape
+        self._need_here(gate, torch.bfloat16, (rows, inter), "gate")
+        self._need_here(up, torch.bfloat16, (rows, inter), "up")
+        self._need_here(q, torch.float8_e4m3fn, (rows, inter), "q")
+        self._need_here(s, torch.float32, (_blocks(inter), rows), "s")
+        if h is not None:
+            self._need_here(h, torch.bfloat16, (rows, inter), "h")
+        st = self._lib.u15h_swiglu_quant_fp8(self._ctx, self._stream_here(stream),
+                                             gate.data_ptr(), up.data_ptr(), rows, inter,
+                                             _ptr(h), q.data_ptr(), s.data_ptr())
+        if st:
+            self._check(st, "u15h_swiglu_quant_fp8")
+
+    def mot_gemm_fp8(self, xq, sx, M_und, M_gen, K, projs, stream=None):
+        """u15h_mot_gemm_fp8: y = x . w^T for every projection (dicts of
+        wq_und, sw_und, wq_gen, sw_gen, y), rows [0, M_und) with the und
+        weights and the next M_gen with the gen weights; xq, sx and the
+        weights as quant_rows_fp8 and quant_blocks_fp8 make them."""
+        M = M_und + M_gen
+        kb = _blocks(K)
+        self._need_here(xq, torch.float8_e4m3fn, (M, K), "xq")
+        self._need_here(sx, torch.float32, (kb, M), "sx")
+        n = len(projs)
+        if not 1 <= n <= MAX_PROJ:
+            raise ValueError(f"1..{MAX_PROJ} projections per launch")
+        arr = (_MotProjFp8 * n)()
+        for p, a in zip(projs, arr):
+            y = p["y"]
+            if y.dim() != 2:
+                raise ValueError("y must be [M][N]")
+            N = y.shape[1]
+            self._need_here(y, torch.bfloat16, (M, N), "y")
+            a.y, a.N = y.data_ptr(), N
+            if M_und:
+                w, sw = p["wq_und"], p["sw_und"]
+                self._need_here(w, torch.float8_e4m3fn, (N, K), "wq_und")
+                self._need_here(sw, torch.float32, (_blocks(N), kb), "sw_und")
+                a.wq_und, a.sw_und = w.data_ptr(), sw.data_ptr()
+            if M_gen:
+                w, sw = p["wq_gen"], p["sw_gen"]
+                self._need_here(w, torch.float8_e4m3fn, (N, K), "wq_gen")
+                self._need_here(sw, torch.float32, (_blocks(N), kb), "sw_gen")
+                a.wq_gen, a.sw_gen = w.data_ptr(), sw.data_ptr()
+        st = self._lib.u15h_mot_gemm_fp8(self._ctx, self._stream_here(stream), xq.data_ptr(),
+                                         sx.data_ptr(), M_und, M_gen, K, arr, n)
+        if st:
+            self._check(st, "u15h_mot_gemm_fp8")
+
     def profile_next_gemm(self, event):
         """Record the raw hipEvent_t `event` (a ctypes.c_void_p or int
         handle) right after the next GEMM kernel, before any split-K
