@@ -765,6 +765,20 @@ u15h::num_cus(const u15h_ctx* ctx)
   return ctx->num_cu;
 }
 
+u15h_status
+u15h::split_workspace(u15h_ctx* ctx, void** ws)
+{
+  const u15h_status st = ensure_split_ws(ctx);
+  *ws = ctx->split_ws;
+  return st;
+}
+
+size_t
+u15h::split_workspace_bytes(const u15h_ctx* ctx)
+{
+  return split_ws_capacity(ctx);
+}
+
 extern "C" {
 
 int

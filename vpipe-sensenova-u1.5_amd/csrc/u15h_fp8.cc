@@ -2,6 +2,7 @@
 // (nothing is launched on a refusal) and the batch tables of u15h_fp8.hip.
 #include "u15h.h"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -87,6 +88,97 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
   p.y = y;
   p.rows = rows;
   p.n = n;
+}
+
+// A launch of the product: `narrow` bm rows and bn columns per workgroup with K
+// split over its waves, else tiles of bm x bn, the last partial round in
+// `split` shares of K.
+struct Plan {
+  bool narrow;
+  int bm, bn, waves, split;
+};
+
+// Counts the tiles of a batch; false if they are too many.
+bool
+set_tiles(Fp8Batch& b, const Plan& p)
+{
+  b.narrow = p.narrow;
+  b.bm = p.bm;
+  b.bn = p.bn;
+  b.waves = p.waves;
+  long long tiles = 0;
+  for (int i = 0; i < b.nprob; ++i) {
+    Fp8Problem& q = b.p[i];
+    q.tiles_m = (q.rows + p.bm - 1) / p.bm;
+    q.tiles_n = (q.n + p.bn - 1) / p.bn;
+    q.tile_begin = (int)tiles;
+    tiles += (long long)q.tiles_m * q.tiles_n;
+    if (tiles > (1 << 28)) { return false; }
+  }
+  b.total_tiles = b.split_begin = (int)tiles;
+  b.split = 1;
+  return true;
+}
+
+// Cuts the last partial round of a batch's tiles into up to `shares` shares of
+// K each, as many as the workspace holds.
+void
+set_split(Fp8Batch& b, const Plan& p, int slots, size_t workspace)
+{
+  const int nb = (b.K + u15h::kFp8Block - 1) / u15h::kFp8Block;
+  const int tail = b.total_tiles % slots;
+  if (tail == 0) { return; }
+  int S = std::min(p.split, nb);
+  S = std::min(S, (int)std::min<size_t>(1 << 16, workspace / ((size_t)tail * p.bm * p.bn * 4)));
+  if (S < 2) { return; }
+  b.split = S;
+  b.split_begin = b.total_tiles - tail;
+}
+
+// Workgroups of a plan that run at once.
+int
+slots_of(const Plan& p, int cus)
+{
+  return p.waves == 4 ? 2 * cus : cus;
+}
+
+Plan
+choose(const Fp8Batch& b, int cus)
+{
+  int rows = 0, cols = 0;
+  for (int i = 0; i < b.nprob; ++i) {
+    rows = std::max(rows, b.p[i].rows);
+    cols += (b.p[i].n + 15) / 16;
+  }
+  if (rows <= 64) {
+    const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int fi = cols > 4 * cus && mt > 1 ? 2 : 1;
+    return Plan{true, 16 * mt, 16 * fi, 4, 1};
+  }
+  const int nb = (b.K + u15h::kFp8Block - 1) / u15h::kFp8Block;
+  // us per stage with every slot busy, and per round beside its stages
+  const struct { int bm, bn, waves; double stage, round; } kinds[] = {
+      {256, 256, 8, 1.60, 6.0}, {192, 256, 8, 1.25, 5.0}, {128, 256, 8, 0.90, 5.0},
+      {128, 128, 4, 0.95, 5.0}, {64, 128, 4, 0.65, 5.0}};
+  Plan best = {};
+  double least = 0;
+  for (const auto& k : kinds) {
+    int tiles = 0;
+    for (int i = 0; i < b.nprob; ++i) {
+      tiles += ((b.p[i].rows + k.bm - 1) / k.bm) * ((b.p[i].n + k.bn - 1) / k.bn);
+    }
+    const int slots = k.waves == 4 ? 2 * cus : cus;
+    const int full = tiles / slots, rem = tiles % slots;
+    const int S = rem == 0 ? 1 : std::max(1, std::min(slots / rem, nb / 4));
+    double us = full * (nb * k.stage + k.round);
+    if (rem > 0) { us += (nb + S - 1) / S * k.stage + k.round; }
+    if (S > 1) { us += 3.0 + 0.3e-6 * rem * S * k.bm * k.bn * 4; }
+    if (least == 0 || us < least) {
+      least = us;
+      best = Plan{false, k.bm, k.bn, k.waves, S};
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -231,6 +323,15 @@ u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream, const uint8_t* xq, const fl
   for (int i = 0; i < nproj; ++i) {
     const u15h_mot_proj_fp8& p = proj[i];
     add_problem(b, xq, sx, p.wq_und, p.sw_und, p.y, M_und, p.N);
+  }
+  b.cus = u15h::num_cus(ctx);
+  const Plan plan = choose(b, b.cus);
+  if (!set_tiles(b, plan)) { return refuse(ctx, "%s: too many tiles", what); }
+  if (!plan.narrow) { set_split(b, plan, slots_of(plan, b.cus), u15h::split_workspace_bytes(ctx)); }
+  if (b.split > 1) {
+    void* ws = nullptr;
+    if ((st = u15h::split_workspace(ctx, &ws)) != U15H_OK) { return st; }
+    b.ws = static_cast<float*>(ws);
   }
   return u15h::end_call(ctx, u15h::launch_fp8_gemm(b, reinterpret_cast<hipStream_t>(stream)),
                         what);

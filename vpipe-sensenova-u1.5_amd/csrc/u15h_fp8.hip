@@ -19,6 +19,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "u15h_internal.h"
 
@@ -346,61 +347,631 @@ find_problem(const Fp8Batch& B, int tile)
   return p;
 }
 
-constexpr int kTile = 64;
+// One work item: a tile, and with K shares which blocks of K.
+struct Fp8Work {
+  int tile, share, prob;
+  bool is_split;
+  int row0, col0;
+  int kbeg, nst;
+};
 
-// 64 x 64 outputs per workgroup, 16 columns x 64 rows per wave, fragments
-// straight from memory.
-__global__ __launch_bounds__(256) void
-fp8_gemm_kernel(const Fp8Batch B)
+// Work item w: whole tiles first, then the split tiles, `split` consecutive
+// items each.  Tiles of a problem go in bands of 4 row tiles, walked column by
+// column, so that items that run together share rows of both operands in L2.
+template <int BM, int BN>
+__device__ __forceinline__ Fp8Work
+fp8_work(const Fp8Batch& B, int nb, int w)
 {
-  const int tile = blockIdx.x;
-  const Fp8Problem& P = B.p[find_problem(B, tile)];
-  const int t = tile - P.tile_begin;
-  const int row0 = t % P.tiles_m * kTile, col0 = t / P.tiles_m * kTile;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int lr = lane & 15, lh = lane >> 4, K = B.K;
-  const int nb = (K + kFp8Block - 1) / kFp8Block;
-  const int n = col0 + wave * 16;
-  if (n >= P.n) { return; }
-  auto load = [&](const uint8_t* row, int b) {
-    const int k = b * kFp8Block + lh * 16;
-    i32x4_t lo = {}, hi = {};
-    if (k < K) { lo = *reinterpret_cast<const i32x4_t*>(row + k); }
-    if (k + 64 < K) { hi = *reinterpret_cast<const i32x4_t*>(row + k + 64); }
+  Fp8Work t;
+  t.is_split = w >= B.split_begin;
+  t.tile = w;
+  t.share = 0;
+  t.kbeg = 0;
+  t.nst = nb;
+  if (t.is_split) {
+    const unsigned v = w - B.split_begin, q = v / (unsigned)B.split;
+    t.tile = B.split_begin + q;
+    t.share = v - q * B.split;
+    t.kbeg = (unsigned)t.share * nb / (unsigned)B.split;
+    t.nst = (unsigned)(t.share + 1) * nb / (unsigned)B.split - t.kbeg;
+  }
+  t.prob = find_problem(B, t.tile);
+  const Fp8Problem& P = B.p[t.prob];
+  const unsigned at = t.tile - P.tile_begin, per = 4 * P.tiles_n;
+  const unsigned band = at / per, in = at - band * per;
+  const unsigned gm = min(P.tiles_m - (int)band * 4, 4);
+  const unsigned col = gm == 4 ? in / 4 : in / gm;
+  t.row0 = (band * 4 + (in - col * gm)) * BM;
+  t.col0 = col * BN;
+  return t;
+}
+
+// LDS of a workgroup: R stages of scales (the tile's rows', then its columns'),
+// R stages of activations, WS = R - 2 of weights.
+template <int BM, int FI, int NW, int R>
+struct Fp8Lds {
+  static constexpr int WS = R - 2;
+  static constexpr int kRowScales = (BM + 63) / 64 * 64;
+  static constexpr int kScales = kRowScales + 64;                // floats per stage
+  static constexpr int kAct = (R * kScales * 4 + 1023) / 1024 * 1024;
+  static constexpr int kWeight = kAct + R * BM * 128;
+  static constexpr int kBytes = kWeight + NW * WS * FI * 2048;
+};
+
+// NW waves, each all BM activation rows x 16 FI weight rows; one stage is one
+// block of K.  Both operands come through LDS by direct loads of 1 KiB (8 rows x
+// 128 bytes: 12 cycles each; loaded to registers in a fragment's layout, 16 rows
+// x 64 bytes, the same bytes take 64).
+// The activation rows are shared: R stages of them, handed over by one barrier
+// a stage.  A wave's weights are its own: it reads a stage's fragments into
+// registers during the stage before and refills their place at once, waiting
+// for no other wave.
+// Row r's 16-byte chunk c sits at position c ^ ((r >> 1) & 7), which spreads
+// the 16 rows of a fragment read over the bank groups; the loads put it there
+// by fetching the chunk that belongs at their landing position.  Fragment j
+// takes activation rows j, FJ + j, 2 FJ + j, ..: a lane's FJ rows are
+// neighbours, and their scales one run.
+//
+// A stage walks the activation fragments j.  The results of the step before
+// join the sums (one multiply-add each) while the matrix unit works.
+//
+// Persistent: the loads run R - 1 stages ahead of the products, over the end of
+// a tile into the next one, whose first stages land while this one's results
+// are stored.
+template <int BM, int FI, int NW, int R, int FB>
+__device__ __forceinline__ void
+fp8_tiles(const Fp8Batch& B, char* lds)
+{
+  using L = Fp8Lds<BM, FI, NW, R>;
+  constexpr int BN = 16 * FI * NW, FJ = BM / 16, WS = L::WS;
+  constexpr int kStage = BM * 128;
+  constexpr int kBlocks = BM / 8;                    // 1 KiB loads per stage
+  constexpr int LB = (kBlocks + NW - 1) / NW;        // per wave
+  constexpr int kA = LB + 1, kW = 2 * FI;            // a wave's loads per stage
+  static_assert(R >= 3 && L::kRowScales / 64 < NW, "a wave for the columns' scales");
+  float* const scales = reinterpret_cast<float*>(lds);
+
+  const int K = B.K, nb = (K + 127) / 128, sa_pitch = B.sa_pitch;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lh = lane >> 4;
+  const int wcol = wave * 16 * FI;                   // the wave's columns of a tile
+
+  // Items go in rounds of gridDim.x; workgroups b, b + 8, .. run on XCD b % 8,
+  // and of each round every XCD takes a contiguous run.
+  const int items = B.split_begin + (B.total_tiles - B.split_begin) * B.split;
+  const int G = gridDim.x, rounds = (items + G - 1) / G;
+  auto item_of = [&](int round) {
+    const int base = round * G, n = min(G, items - base), b = blockIdx.x;
+    if (round >= rounds) { return -1; }
+    if (G % 8 != 0) { return b < n ? base + b : -1; }
+    const int x = b & 7, i = b >> 3;
+    return i < (n >> 3) + (x < (n & 7) ? 1 : 0) ? base + x * (n >> 3) + min(x, n & 7) + i : -1;
+  };
+
+  // ---- loads ---------------------------------------------------------------
+  // What the loads of the stage R - 1 ahead need; past the last item they
+  // fetch zeros.
+  struct {
+    __amdgpu_buffer_rsrc_t a, w;
+    const float* sc;      // this wave's scales at the item's first block
+    int pitch, count;     // floats between blocks, floats per block
+    int kbeg, nst, k, round;
+  } ld;
+  const bool row_wave = wave < L::kRowScales / 64;
+  auto load_item = [&](int round) {
+    const int it = item_of(round);
+    const Fp8Work t = fp8_work<BM, BN>(B, nb, max(it, 0));
+    const Fp8Problem& P = B.p[t.prob];
+    const int rows = min(BM, P.rows - t.row0), cols = min(BN, P.n - t.col0);
+    ld.a = make_rsrc(P.a + (size_t)t.row0 * K, rows * K);
+    ld.w = make_rsrc(P.w + (size_t)t.col0 * K, cols * K);
+    if (row_wave) {
+      ld.sc = P.sa + (size_t)t.kbeg * sa_pitch + t.row0 + wave * 64;
+      ld.pitch = sa_pitch;
+      ld.count = max(0, min(64, rows - wave * 64));
+    } else {
+      ld.sc = P.sw + (size_t)(t.col0 / 128) * nb + t.kbeg;
+      ld.pitch = 1;
+      ld.count = ((cols + 127) / 128 - 1) * nb + 1;
+    }
+    ld.kbeg = t.kbeg;
+    ld.nst = it < 0 ? 0 : t.nst;
+    ld.k = 0;
+    ld.round = round;
+  };
+  // a load's lane l fills chunk position l % 8 of row l / 8 of its 8 rows
+  // activations: wave w fills blocks w, w + NW, .. of the stage (the same one
+  // twice where there are fewer blocks than waves); LDS row 16 j + i is row i FJ + j
+  const int blk = wave % kBlocks;
+  int aoff[LB];
+  const int prow = 8 * blk + (lane >> 3);
+  const int chunk = (lane & 7) ^ ((prow >> 1) & 7);
+#pragma unroll
+  for (int b = 0; b < LB; ++b) {
+    const int p = prow + 8 * NW * b;
+    aoff[b] = (p % 16 * FJ + p / 16) * K + (chunk << 4);
+  }
+  const int atail = (nb - 1) * 128 + (chunk << 4) < K ? 0 : kOobOffset;
+  // weights: blocks of 8 rows; the chunk depends on the block's parity
+  const int wrow = lane >> 3;
+  const int wchunk[2] = {(lane & 7) ^ (wrow >> 1), (lane & 7) ^ (4 + (wrow >> 1))};
+  int woff[2], wtail[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    woff[h] = (wcol + 8 * h + wrow) * K + (wchunk[h] << 4);
+    wtail[h] = (nb - 1) * 128 + (wchunk[h] << 4) < K ? 0 : kOobOffset;
+  }
+  // scales: a lane each; the columns' are nb apart
+  constexpr int kColBlocks = (BN + 127) / 128;
+  const int soff = row_wave ? lane * 4 : lane < kColBlocks ? lane * nb * 4 : kOobOffset;
+  char* const mine = lds + L::kWeight + wave * (WS * FI * 2048);
+  auto dma16 = [](const __amdgpu_buffer_rsrc_t& r, char* to, int v, int s) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (__attribute__((address_space(3))) void*)to, 16, v, s, 0, 0);
+  };
+  // Instruction op of the kA of a stage's activations (the last its scales),
+  // and of the kW of its weights.
+  auto load_a = [&](int slot, int op) {
+    const bool past = ld.k >= ld.nst;
+    if (op < LB) {
+      const int oob = (ld.kbeg + ld.k == nb - 1 ? atail : 0) | (past ? kOobOffset : 0);
+      dma16(ld.a, lds + L::kAct + slot * kStage + (blk + NW * op) * 1024, aoff[op] + oob,
+            (ld.kbeg + ld.k) * 128);
+    } else {
+      const int g = row_wave ? wave * 64 : L::kRowScales;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          make_rsrc(ld.sc + (size_t)ld.k * ld.pitch, past ? 0 : ld.count * 4),
+          (__attribute__((address_space(3))) void*)(scales + slot * L::kScales + g), 4, soff, 0,
+          0, 0);
+    }
+  };
+  auto load_w = [&](int slot, int op) {
+    const int oob = (ld.kbeg + ld.k == nb - 1 ? wtail[op & 1] : 0) |
+                    (ld.k >= ld.nst ? kOobOffset : 0);
+    dma16(ld.w, mine + slot * (FI * 2048) + op * 1024, woff[op & 1] + (op >> 1) * 16 * K + oob,
+          (ld.kbeg + ld.k) * 128);
+  };
+  // (a tile takes an even number of stages: one past the range adds 0 * 0)
+  auto advance = [&] {
+    if (++ld.k >= ((ld.nst + 1) & ~1) && ld.nst > 0) { load_item(ld.round + 1); }
+  };
+
+  // ---- fragments -------------------------------------------------------------
+  const int key = (lr >> 1) & 7;
+  const int rd0 = lr * 128 + ((lh ^ key) << 4), rd1 = lr * 128 + (((4 + lh) ^ key) << 4);
+  auto read_frag = [&](const char* base) {
+    const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(base + rd0);
+    const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(base + rd1);
     return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
-  // rows past the problem repeat its last one; their results are not stored
-  const uint8_t* const wr = P.w + (size_t)min(n + lr, P.n - 1) * K;
-  const uint8_t* ar[4];
-  int m[4];
-  f32x4_t acc[4];
+  auto read_a = [&](int slot, int j) {
+    return read_frag(lds + L::kAct + slot * kStage + j * 2048);
+  };
+  constexpr int SV = FJ < 4 ? FJ : 4;                // row scales read at a time
+  typedef float sv_t __attribute__((ext_vector_type(SV)));
+  auto read_s = [&](int slot, int j) {
+    return *reinterpret_cast<const sv_t*>(scales + slot * L::kScales + lr * FJ + j);
+  };
+
+  constexpr int FH = FI < 2 ? 1 : 2, HS = FI / FH;   // products per step, steps per fragment
+  f32x4_t acc[FI][FJ], d[2][FH];
+  i32x8_t fa[2][FI], fb[FB];
+  sv_t sv[2];
+  float w, wprev;
+  auto clear = [&] {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    m[j] = min(row0 + 16 * j + lr, P.rows - 1);
-    ar[j] = P.a + (size_t)m[j] * K;
-    acc[j] = f32x4_t{};
+    for (int i = 0; i < FI; ++i) {
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) { acc[i][j] = f32x4_t{}; }
+    }
+#pragma unroll
+    for (int i = 0; i < FH; ++i) { d[0][i] = d[1][i] = f32x4_t{}; }
+    sv[0] = sv[1] = sv_t{};
+    w = 0.0f;
+  };
+  auto add = [&](int jp, int hp, int par, float sc) {
+#pragma unroll
+    for (int i = 0; i < FH; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[hp * FH + i][jp][e] = fmaf(d[par][i][e], sc, acc[hp * FH + i][jp][e]);
+      }
+    }
+  };
+  constexpr int kSvs = FJ / SV;                      // scale reads per stage
+  // Where in a stage: its activation loads before fragment JR, there the next
+  // stage's weights are read, and from JW on their place is refilled.
+  constexpr int JR = FJ >= 12 ? 6 : FJ >= 8 ? 3 : FJ >= 4 ? 1 : 0;
+  constexpr int JW = FJ >= 12 ? 9 : FJ >= 8 ? 6 : FJ - 1;
+  constexpr int kAPerJ = JR > 0 ? (kA + JR - 1) / JR : kA;
+  constexpr int kWPerJ = (kW + FJ - JW - 1) / (FJ - JW);
+  // Loads that may be in flight behind the awaited ones (a stage issues its
+  // kA, then its kW, and so do the first stages' loads below), and a tile's
+  // stores between.
+  constexpr int kStores = FI * FJ;
+  constexpr int kWaitA = (R - 3) * (kA + kW) + kW, kWaitW = (WS - 1) * (kA + kW) + kA;
+  static_assert(kWaitW + kStores < 64 && kWaitA + kStores < 64, "the counter has 6 bits");
+  // The sums so far stay where they are computed: nothing of a stage moves past
+  // a branch, where it would hold its operands' registers.
+  auto settle = [&] {
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) { asm volatile("" : "+v"(acc[i][j])); }
+    }
+  };
+  // One stage: par its parity, slot its activations' place, next the next
+  // stage's, ahead the last one's, ws where the next stage's weights are;
+  // stored: a tile's results were stored just before.
+  auto stage = [&](auto par_c, bool stored, int slot, int next, int ahead, int ws) {
+    constexpr int par = decltype(par_c)::value;
+    constexpr int f = par * FJ, g = par * kSvs;
+    // the next stage's activations have landed in every wave, and every wave
+    // has read the last stage's
+    if (par == 0 && stored) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitA + kStores) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitA) : "memory");
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    wprev = w;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      // the scale of fragment j - 1
+      const float before = j == 0 ? sv[(g + 1) & 1][SV - 1] * wprev
+                                  : sv[(g + (j - 1) / SV) & 1][(j - 1) % SV] * w;
+#pragma unroll
+      for (int o = j * kAPerJ; o < (j + 1) * kAPerJ && o < kA; ++o) { load_a(ahead, o); }
+      if (j == JR) {
+        if (par == 0) {
+          settle();
+          if (stored) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW + kStores) : "memory");
+          } else {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW) : "memory");
+          }
+        } else {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          fa[par ^ 1][i] = read_frag(mine + ws * (FI * 2048) + i * 2048);
+        }
+      }
+      if (j == 0) { w = scales[slot * L::kScales + L::kRowScales + wcol / 128]; }
+      if (j % SV == 0) { sv[(g + j / SV) & 1] = read_s(slot, j); }
+      constexpr int A = FB - 1;                      // fragments read ahead
+      fb[(f + j + A) % FB] = j + A < FJ ? read_a(slot, j + A) : read_a(next, j + A - FJ);
+#pragma unroll
+      for (int h = 0; h < HS; ++h) {
+        const int now = ((f + j) * HS + h) & 1, other = now ^ 1;
+#pragma unroll
+        for (int i = 0; i < FH; ++i) {
+          d[now][i] = mfma_block(fa[par][h * FH + i], fb[(f + j) % FB]);
+        }
+        if (h == 0) {
+          add((j + FJ - 1) % FJ, HS - 1, other, before);
+        } else {
+          add(j, h - 1, other, sv[(g + j / SV) & 1][j % SV] * w);
+        }
+#pragma unroll
+        for (int i = 0; i < FH; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
+          if (i == 0 && h == 0) { __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); }  // reads
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);        // the sums
+        }
+        if (h + 1 < HS) { __builtin_amdgcn_sched_barrier(0); }
+      }
+      if (j >= JW) {
+        if (j == JW) {
+          __builtin_amdgcn_sched_barrier(0);
+          // the next weights are in registers: their place is free
+#pragma unroll
+          for (int i = 0; i < FI; ++i) { asm volatile("" : "+v"(fa[par ^ 1][i])); }
+        }
+#pragma unroll
+        for (int o = (j - JW) * kWPerJ; o < (j - JW + 1) * kWPerJ && o < kW; ++o) {
+          load_w(ws, o);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    settle();
+    // tiles take an even number of stages, so the loads' items end in one of
+    // the two parities only
+    if constexpr ((par + R) % 2 == 0) { advance(); } else { ++ld.k; }
+  };
+
+  // ---- the first item's first stages -------------------------------------------
+  int it = item_of(0);
+  if (it < 0) { return; }
+  load_item(0);
+  // the loads' order is a stage's: activations, then the next stage's weights,
+  // the first stage's before all
+#pragma unroll
+  for (int o = 0; o < kW; ++o) { load_w(0, o); }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int r = 0; r < R - 1; ++r) {
+#pragma unroll
+    for (int o = 0; o < kA; ++o) { load_a(r, o); }
+    __builtin_amdgcn_sched_barrier(0);
+    if (r > 0 && r < WS) {
+#pragma unroll
+      for (int o = 0; o < kW; ++o) { load_w(r, o); }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (r < R - 2) { advance(); }
   }
-  for (int b = 0; b < nb; ++b) {
-    const i32x8_t w = load(wr, b);
-    const float sw = P.sw[(size_t)(n / kFp8Block) * nb + b];
+  // stage 0 has landed
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R - 2) * kA + (WS - 1) * kW) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4_t d = mfma_block(w, load(ar[j], b));
-      const float s = P.sa[(size_t)b * B.sa_pitch + m[j]] * sw;
+  for (int i = 0; i < FI; ++i) { fa[0][i] = read_frag(mine + i * 2048); }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) { acc[j][e] = fmaf(d[e], s, acc[j][e]); }
+  for (int a = 0; a < FB - 1; ++a) { fb[a] = read_a(0, a); }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < FI; ++i) { asm volatile("" : "+v"(fa[0][i])); }
+#pragma unroll
+  for (int o = 0; o < kW; ++o) { load_w(0, o); }
+  __builtin_amdgcn_sched_barrier(0);
+  advance();
+  static_assert(2 * FJ % FB == 0 && FB - 1 <= FJ, "the fragment buffers come round with two stages");
+
+  int cur = 0, ws = WS > 1 ? 1 : 0, round = 0;
+  using std::integral_constant;
+  clear();
+  for (;;) {
+    const Fp8Work t = fp8_work<BM, BN>(B, nb, it);
+    const Fp8Problem& P = B.p[t.prob];
+    for (int k = 0; k < t.nst; k += 2) {
+      const int s1 = cur + 1 == R ? 0 : cur + 1, s2 = s1 + 1 == R ? 0 : s1 + 1;
+      stage(integral_constant<int, 0>{}, k == 0 && round > 0, cur, s1,
+            cur == 0 ? R - 1 : cur - 1, ws);
+      ws = ws + 1 == WS ? 0 : ws + 1;
+      stage(integral_constant<int, 1>{}, false, s1, s2, cur, ws);
+      ws = ws + 1 == WS ? 0 : ws + 1;
+      cur = s2;
+    }
+    add(FJ - 1, HS - 1, 1, sv[1][SV - 1] * w);
+
+    // ---- results: kStores stores whatever the tile's edges, which drop some ------
+    const int rows = min(BM, P.rows - t.row0);
+    const int n0 = t.col0 + wcol + lh * 4;
+    if (t.is_split) {
+      const __amdgpu_buffer_rsrc_t to = make_rsrc(
+          B.ws + (size_t)((t.tile - B.split_begin) * B.split + t.share) * (BM * BN), rows * BN * 4);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(u32x4_t, acc[i][j]), to,
+              ((lr * FJ + j) * BN + wcol + i * 16 + lh * 4) * 4, 0, 0);
+        }
+      }
+    } else {
+      const __amdgpu_buffer_rsrc_t to =
+          make_rsrc(P.y + (size_t)t.row0 * P.n, rows * P.n * 2);
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          const int n = n0 + i * 16;
+          __builtin_amdgcn_raw_buffer_store_b64(
+              u32x2_t{pack_bf16x2(acc[i][j][0], acc[i][j][1]),
+                      pack_bf16x2(acc[i][j][2], acc[i][j][3])},
+              to, n < P.n ? ((lr * FJ + j) * P.n + n) * 2 : kOobOffset, 0, 0);
+        }
+      }
+    }
+    it = item_of(++round);
+    if (it < 0) { break; }
+    clear();
+  }
+  // no load may still be writing LDS when the workgroup ends
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <int BM, int FI, int NW, int R, int FB>
+__global__ __launch_bounds__(64 * NW, 2) void
+fp8_tile_kernel(const Fp8Batch B)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[Fp8Lds<BM, FI, NW, R>::kBytes];
+  fp8_tiles<BM, FI, NW, R, FB>(B, lds);
+}
+
+// ---- few rows: the weights' stream ---------------------------------------------
+// At most 16 MT rows.  A workgroup takes 16 FI columns and its NW waves the
+// blocks of K, a contiguous share each, with nothing between them until their
+// sums join through LDS, in wave order.  A wave streams its blocks (weights,
+// rows, row scales) through D places of its own in LDS by direct loads, so all
+// of D stages are in flight from the start; the weight scales are a register
+// each of 64 blocks, read by lane.
+template <int MT, int FI, int NW, int D>
+struct Fp8NarrowLds {
+  static constexpr int kSlot = FI * 2048 + MT * 2048 + (MT + 3) / 4 * 256;
+  static constexpr int kBytes = NW * std::max(D * kSlot, MT * FI * 1024);
+};
+
+template <int MT, int FI, int NW, int D>
+__global__ __launch_bounds__(64 * NW) void
+fp8_narrow_kernel(const Fp8Batch B)
+{
+  using L = Fp8NarrowLds<MT, FI, NW, D>;
+  __shared__ __attribute__((aligned(1024))) char lds[L::kBytes];
+  constexpr int kOps = 2 * FI + 2 * MT + (MT + 3) / 4;
+  static_assert(D * kOps < 64, "the counter has 6 bits");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lh = lane >> 4;
+  const int prob = find_problem(B, blockIdx.x);
+  const Fp8Problem& P = B.p[prob];
+  const int n0 = (blockIdx.x - P.tile_begin) * (16 * FI);
+  const int K = B.K, nb = (K + 127) / 128, sa_pitch = B.sa_pitch;
+  const int b0 = wave * nb / NW, b1 = (wave + 1) * nb / NW;
+
+  const __amdgpu_buffer_rsrc_t rw =
+      make_rsrc(P.w + (size_t)n0 * K, min(16 * FI, P.n - n0) * K);
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(P.a, P.rows * K);
+  const float* const sa = P.sa;
+  const int scale_bytes = P.rows * 4;
+  char* const mine = lds + wave * (D * L::kSlot);
+  // a load's lane l fills chunk position l % 8 of row l / 8 of its 8 rows; the
+  // chunk depends on the 8 rows' parity
+  const int row = lane >> 3;
+  int off[2], tail[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int chunk = (lane & 7) ^ (4 * h + (row >> 1));
+    off[h] = (8 * h + row) * K + (chunk << 4);
+    tail[h] = (nb - 1) * 128 + (chunk << 4) < K ? 0 : kOobOffset;
+  }
+  auto load = [&](int slot, int b) {
+    char* const to = mine + slot * L::kSlot;
+    const int kt = min(b, nb - 1), past = b < b1 ? 0 : kOobOffset;
+    const int ko = __builtin_amdgcn_readfirstlane(kt * 128);
+#pragma unroll
+    for (int r = 0; r < 2 * (FI + MT); ++r) {
+      const int h = r & 1, v = off[h] + ((kt == nb - 1 ? tail[h] : 0) | past);
+      const bool weights = r < 2 * FI;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          weights ? rw : ra, (__attribute__((address_space(3))) void*)(to + r * 1024), 16,
+          v + (weights ? r : r - 2 * FI) / 2 * 16 * K, ko, 0, 0);
+    }
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sa + (size_t)kt * sa_pitch, scale_bytes);
+#pragma unroll
+    for (int g = 0; g < (MT + 3) / 4; ++g) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(to + (FI + MT) * 2048 + g * 256), 4,
+          g * 256 + lane * 4, 0, 0, 0);
+    }
+  };
+  const float* const sw = P.sw + (size_t)(n0 / 128) * nb;
+  float wv = b0 + lane < b1 ? sw[b0 + lane] : 0.0f;
+
+  const int key = (lr >> 1) & 7;
+  const int rd0 = lr * 128 + ((lh ^ key) << 4), rd1 = lr * 128 + (((4 + lh) ^ key) << 4);
+  f32x4_t acc[FI][MT];
+#pragma unroll
+  for (int i = 0; i < FI; ++i) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) { acc[i][j] = f32x4_t{}; }
+  }
+#pragma unroll
+  for (int r = 0; r < D; ++r) {
+    load(r, b0 + r);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  int slot = 0;
+  for (int b = b0; b < b1; ++b) {
+    if (((b - b0) & 63) == 0 && b != b0) {
+      wv = b + lane < b1 ? sw[b + lane] : 0.0f;
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(wv)::"memory");
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * kOps) : "memory");
+    const char* const at = mine + slot * L::kSlot;
+    i32x8_t f[FI + MT];
+    float s[MT];
+#pragma unroll
+    for (int r = 0; r < FI + MT; ++r) {
+      const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(at + r * 2048 + rd0);
+      const i32x4_t hi = *reinterpret_cast<const i32x4_t*>(at + r * 2048 + rd1);
+      f[r] = i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      s[j] = *reinterpret_cast<const float*>(at + (FI + MT) * 2048 + (16 * j + lr) * 4);
+    }
+    // in registers: the place is free
+#pragma unroll
+    for (int r = 0; r < FI + MT; ++r) { asm volatile("" : "+v"(f[r])); }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) { asm volatile("" : "+v"(s[j])); }
+    load(slot, b + D);
+    const float w = __uint_as_float(
+        __builtin_amdgcn_readlane(__float_as_uint(wv), (b - b0) & 63));
+    f32x4_t d[FI][MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+#pragma unroll
+      for (int i = 0; i < FI; ++i) { d[i][j] = mfma_block(f[i], f[FI + j]); }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { acc[i][j][e] = fmaf(d[i][j][e], s[j] * w, acc[i][j][e]); }
+      }
+    }
+    slot = slot + 1 == D ? 0 : slot + 1;
+  }
+  // every load has landed before its place takes the sums
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < FI; ++i) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      *reinterpret_cast<f32x4_t*>(lds + ((wave * FI + i) * MT + j) * 1024 + lane * 16) = acc[i][j];
     }
   }
-  const int c = n + lh * 4;
-  if (c >= P.n) { return; }
+  __syncthreads();
+  for (int c = wave; c < FI * MT; c += NW) {
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(lds + c * 1024 + lane * 16);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int r = row0 + 16 * j + lr;
-    if (r < P.rows) {
-      *reinterpret_cast<u32x2_t*>(P.y + (size_t)r * P.n + c) =
-          u32x2_t{pack_bf16x2(acc[j][0], acc[j][1]), pack_bf16x2(acc[j][2], acc[j][3])};
+    for (int q = 1; q < NW; ++q) {
+      v += *reinterpret_cast<const f32x4_t*>(lds + (q * FI * MT + c) * 1024 + lane * 16);
+    }
+    const int m = c % MT * 16 + lr, n = n0 + c / MT * 16 + lh * 4;
+    if (m < P.rows && n < P.n) {
+      *reinterpret_cast<u32x2_t*>(P.y + (size_t)m * P.n + n) =
+          u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     }
   }
+}
+
+// The shares of split tiles: one workgroup per 8 rows of a tile.
+template <int BM, int BN>
+__global__ __launch_bounds__(256) void
+fp8_reduce_kernel(const Fp8Batch B)
+{
+  const int tile = B.split_begin + blockIdx.x / (BM / 8);
+  const int nb = (B.K + 127) / 128;
+  const Fp8Work t = fp8_work<BM, BN>(B, nb, B.split_begin + (tile - B.split_begin) * B.split);
+  const Fp8Problem& P = B.p[t.prob];
+  const float* const ws = B.ws + (size_t)(tile - B.split_begin) * B.split * (BM * BN);
+  for (int c = threadIdx.x; c < 8 * BN / 4; c += 256) {
+    const int m = blockIdx.x % (BM / 8) * 8 + c / (BN / 4), n = c % (BN / 4) * 4;
+    if (t.row0 + m >= P.rows || t.col0 + n >= P.n) { continue; }
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(ws + m * BN + n);
+    for (int q = 1; q < B.split; ++q) {
+      v += *reinterpret_cast<const f32x4_t*>(ws + (size_t)q * (BM * BN) + m * BN + n);
+    }
+    *reinterpret_cast<u32x2_t*>(P.y + (size_t)(t.row0 + m) * P.n + t.col0 + n) =
+        u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  }
+}
+
+template <int BM, int FI, int NW, int R, int FB>
+hipError_t
+tile_launch(const Fp8Batch& b, hipStream_t s)
+{
+  const int tail = b.total_tiles - b.split_begin;
+  const int items = b.split_begin + tail * b.split;
+  // as many workgroups as run at once
+  constexpr int kPerCu = std::min(160 * 1024 / Fp8Lds<BM, FI, NW, R>::kBytes, 8 / NW * 2);
+  fp8_tile_kernel<BM, FI, NW, R, FB>
+      <<<std::min(items, b.cus * std::max(kPerCu, 1)), 64 * NW, 0, s>>>(b);
+  if (b.split > 1 && tail > 0) {
+    fp8_reduce_kernel<BM, 16 * FI * NW><<<tail * (BM / 8), 256, 0, s>>>(b);
+  }
+  return hipGetLastError();
 }
 
 template <int WPR, int CPL>
@@ -426,22 +997,39 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 
 }  // namespace
 
+// The tile builds: X(BM, FI, NW, R, FB).
+#define U15H_FP8_TILES(X) \
+  X(256, 2, 8, 3, 4)      \
+  X(192, 2, 8, 3, 4)      \
+  X(128, 2, 8, 4, 4)      \
+  X(128, 2, 4, 3, 4)      \
+  X(64, 2, 4, 4, 4)
+
+#define U15H_FP8_NARROW(X) \
+  X(1, 1, 4, 4)            \
+  X(1, 2, 4, 4)            \
+  X(2, 1, 4, 4)            \
+  X(2, 2, 4, 4)            \
+  X(4, 1, 4, 3)            \
+  X(4, 2, 4, 3)            \
+  X(6, 1, 4, 2)            \
+  X(8, 1, 4, 2)
+
 hipError_t
-launch_fp8_gemm(const Fp8Batch& b0, hipStream_t s)
+launch_fp8_gemm(const Fp8Batch& b, hipStream_t s)
 {
-  Fp8Batch b = b0;
-  long long tiles = 0;
-  for (int i = 0; i < b.nprob; ++i) {
-    Fp8Problem& p = b.p[i];
-    p.tiles_m = (p.rows + kTile - 1) / kTile;
-    p.tiles_n = (p.n + kTile - 1) / kTile;
-    p.tile_begin = (int)tiles;
-    tiles += (long long)p.tiles_m * p.tiles_n;
-    if (tiles > (1 << 30)) { return hipErrorInvalidValue; }
+#define U15H_CASE(MT, FI, NW, D)                                                          \
+  if (b.narrow && b.bm == 16 * MT && b.bn == 16 * FI && b.waves == NW) {              \
+    fp8_narrow_kernel<MT, FI, NW, D><<<b.total_tiles, 64 * NW, 0, s>>>(b);               \
+    return hipGetLastError();                                                            \
   }
-  b.total_tiles = (int)tiles;
-  fp8_gemm_kernel<<<dim3((unsigned)tiles), 256, 0, s>>>(b);
-  return hipGetLastError();
+  U15H_FP8_NARROW(U15H_CASE)
+#undef U15H_CASE
+#define U15H_CASE(BM, FI, NW, R, FB)                                  \
+  if (!b.narrow && b.bm == BM && b.bn == 16 * FI * NW && b.waves == NW) { return tile_launch<BM, FI, NW, R, FB>(b, s); }
+  U15H_FP8_TILES(U15H_CASE)
+#undef U15H_CASE
+  return hipErrorInvalidValue;
 }
 
 hipError_t
@@ -502,7 +1090,14 @@ fp8_kernels_loadable()
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 2, true>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 4, false>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 4, true>),
-      reinterpret_cast<const void*>(&fp8_gemm_kernel),
+#define U15H_FN(MT, FI, NW, D) reinterpret_cast<const void*>(&fp8_narrow_kernel<MT, FI, NW, D>),
+      U15H_FP8_NARROW(U15H_FN)
+#undef U15H_FN
+#define U15H_FN(BM, FI, NW, R, FB)                                                    \
+  reinterpret_cast<const void*>(&fp8_tile_kernel<BM, FI, NW, R, FB>),                 \
+      reinterpret_cast<const void*>(&fp8_reduce_kernel<BM, 16 * FI * NW>),
+      U15H_FP8_TILES(U15H_FN)
+#undef U15H_FN
   };
   for (const void* f : fns) {
     hipFuncAttributes a;

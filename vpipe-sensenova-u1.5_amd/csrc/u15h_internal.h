@@ -283,8 +283,23 @@ struct Fp8Batch {
   int nprob;
   int K;                  // % 16 == 0
   int sa_pitch;           // rows of the whole call
+  int bm, bn;             // tile: activation rows x weight rows
+  int waves;              // per workgroup
+  bool narrow;
+  int cus;                // compute units
   int total_tiles;
+  // Tiles [split_begin, total_tiles) run as `split` workgroups each, every
+  // one a contiguous share of the blocks of K whose f32 sums go to ws
+  // ([(tile - split_begin) * split + share][bm][bn]); a second kernel adds
+  // the shares in order.
+  int split_begin;
+  int split;
+  float* ws;
 };
+inline size_t fp8_split_bytes(const Fp8Batch& b)
+{
+  return (size_t)(b.total_tiles - b.split_begin) * b.split * b.bm * b.bn * 4;
+}
 hipError_t launch_fp8_gemm(const Fp8Batch& b, hipStream_t s);
 // Codes [rows][K] and scales [ceil(K / 128)][rows] of bf16 rows, or with `up`
 // of silu(x) * up, whose bf16 values go to h where that is not null.
@@ -314,6 +329,10 @@ bool fp8_kernels_loadable();
 u15h_status begin_call(u15h_ctx* ctx);
 u15h_status end_call(u15h_ctx* ctx, hipError_t e, const char* what);
 int num_cus(const u15h_ctx* ctx);
+// The context's split-K workspace (allocated on first use, also under stream
+// capture) and its size.
+u15h_status split_workspace(u15h_ctx* ctx, void** ws);
+size_t split_workspace_bytes(const u15h_ctx* ctx);
 
 // Forces every kernel's code object to load; false if any cannot.
 bool kernels_loadable();
