@@ -3,6 +3,7 @@
 #include "u15h.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -90,95 +91,128 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
   p.n = n;
 }
 
-// A launch of the product: `narrow` bm rows and bn columns per workgroup with K
-// split over its waves, else tiles of bm x bn, the last partial round in
-// `split` shares of K.
-struct Plan {
+// The kinds of launch, and what a call takes on each, in us: `fixed`, then
+//   narrow: `round` per workgroup of the busiest CU, `stage` per block of K of
+//           those, `stream` per block of all of them over the CUs;
+//   tiles:  `round` and `stage` per round of workgroups (a CU that runs two
+//           takes two stages), `split` for the second launch with K shares and
+//           `part` per MB of their sums;
+//   and `weight` per MB of weights.
+// Fitted to 7250 timings (a graph, weights rotated; M 1-2800, K 256-12288, N
+// 512-24576, every kind and 1 to 16 shares), each to 5-9% on the mean; the kind
+// and shares with the least estimate take 1.4% longer than the fastest of all,
+// on the mean over the 325 sizes, and 31% at worst (65 rows, K 8192, N 1024:
+// 15.8 against 12.1 us).
+struct Kind {
   bool narrow;
-  int bm, bn, waves, split;
+  int bm, bn, waves;
+  double fixed, round, stage, stream, split, part, weight;
+};
+constexpr Kind kKinds[] = {
+    {true, 16, 16, 4, 2.57, 0.61, 0.0407, 0.0622, 0, 0, 0},
+    {true, 16, 32, 4, 2.10, 1.33, 0.0516, 0.1525, 0, 0, 0},
+    {true, 32, 16, 4, 1.82, 1.59, 0.0613, 0.0587, 0, 0, 0},
+    {true, 32, 32, 4, 2.43, 1.26, 0.0674, 0.1547, 0, 0, 0},
+    {true, 64, 16, 4, 1.55, 2.08, 0.0836, 0.0818, 0, 0, 0},
+    {true, 64, 32, 4, 3.74, 0.44, 0.0894, 0.2003, 0, 0, 0},
+    {true, 96, 16, 4, 1.48, 2.32, 0.1122, 0.0918, 0, 0, 0},
+    {true, 128, 16, 4, 1.39, 2.83, 0.1437, 0.0984, 0, 0, 0},
+    {false, 64, 128, 4, 5.09, 0.03, 0.350, 0, 3.15, 0.397, 0.109},
+    {false, 128, 128, 4, 5.50, 0, 0.521, 0, 3.19, 0.341, 0.123},
+    {false, 128, 256, 8, 4.28, 2.94, 0.738, 0, 4.06, 0.370, 0.100},
+    {false, 192, 256, 8, 4.91, 5.51, 0.952, 0, 5.73, 0.179, 0.118},
+    {false, 256, 256, 8, 11.74, 0, 1.2235, 0, 6.12, 0.135, 0.094},
 };
 
-// Counts the tiles of a batch; false if they are too many.
-bool
-set_tiles(Fp8Batch& b, const Plan& p)
+// Workgroups of a kind of tile that run at once.
+int
+slots_of(const Kind& k, int cus)
 {
-  b.narrow = p.narrow;
-  b.bm = p.bm;
-  b.bn = p.bn;
-  b.waves = p.waves;
+  return k.waves == 4 ? 2 * cus : cus;
+}
+
+// Counts a batch's tiles on a kind and cuts its last partial round in `shares`
+// shares of K; false if the tiles are too many.
+bool
+set_tiles(Fp8Batch& b, const Kind& k, int shares)
+{
+  b.narrow = k.narrow;
+  b.bm = k.bm;
+  b.bn = k.bn;
+  b.waves = k.waves;
   long long tiles = 0;
   for (int i = 0; i < b.nprob; ++i) {
     Fp8Problem& q = b.p[i];
-    q.tiles_m = (q.rows + p.bm - 1) / p.bm;
-    q.tiles_n = (q.n + p.bn - 1) / p.bn;
+    q.tiles_m = (q.rows + k.bm - 1) / k.bm;
+    q.tiles_n = (q.n + k.bn - 1) / k.bn;
     q.tile_begin = (int)tiles;
     tiles += (long long)q.tiles_m * q.tiles_n;
     if (tiles > (1 << 28)) { return false; }
   }
   b.total_tiles = b.split_begin = (int)tiles;
-  b.split = 1;
+  b.split = shares;
+  if (shares > 1) { b.split_begin -= b.total_tiles % slots_of(k, b.cus); }
   return true;
 }
 
-// Cuts the last partial round of a batch's tiles into up to `shares` shares of
-// K each, as many as the workspace holds.
-void
-set_split(Fp8Batch& b, const Plan& p, int slots, size_t workspace)
+// Chooses a batch's kind and shares by their estimates; false if the tiles are
+// too many.
+bool
+plan(Fp8Batch& b, size_t workspace)
 {
-  const int nb = (b.K + u15h::kFp8Block - 1) / u15h::kFp8Block;
-  const int tail = b.total_tiles % slots;
-  if (tail == 0) { return; }
-  int S = std::min(p.split, nb);
-  S = std::min(S, (int)std::min<size_t>(1 << 16, workspace / ((size_t)tail * p.bm * p.bn * 4)));
-  if (S < 2) { return; }
-  b.split = S;
-  b.split_begin = b.total_tiles - tail;
-}
-
-// Workgroups of a plan that run at once.
-int
-slots_of(const Plan& p, int cus)
-{
-  return p.waves == 4 ? 2 * cus : cus;
-}
-
-Plan
-choose(const Fp8Batch& b, int cus)
-{
-  int rows = 0, cols = 0;
+  const int C = b.cus, nb = (b.K + u15h::kFp8Block - 1) / u15h::kFp8Block;
+  int rows = 0;
+  double mb = 0;                                   // the weights'
   for (int i = 0; i < b.nprob; ++i) {
     rows = std::max(rows, b.p[i].rows);
-    cols += (b.p[i].n + 15) / 16;
+    mb += 1e-6 * b.p[i].n * b.K;
   }
-  if (rows <= 64) {
-    const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int fi = cols > 4 * cus && mt > 1 ? 2 : 1;
-    return Plan{true, 16 * mt, 16 * fi, 4, 1};
-  }
-  const int nb = (b.K + u15h::kFp8Block - 1) / u15h::kFp8Block;
-  // us per stage with every slot busy, and per round beside its stages
-  const struct { int bm, bn, waves; double stage, round; } kinds[] = {
-      {256, 256, 8, 1.60, 6.0}, {192, 256, 8, 1.25, 5.0}, {128, 256, 8, 0.90, 5.0},
-      {128, 128, 4, 0.95, 5.0}, {64, 128, 4, 0.65, 5.0}};
-  Plan best = {};
+  const Kind* best = nullptr;
+  int best_shares = 1;
   double least = 0;
-  for (const auto& k : kinds) {
-    int tiles = 0;
-    for (int i = 0; i < b.nprob; ++i) {
-      tiles += ((b.p[i].rows + k.bm - 1) / k.bm) * ((b.p[i].n + k.bn - 1) / k.bn);
-    }
-    const int slots = k.waves == 4 ? 2 * cus : cus;
-    const int full = tiles / slots, rem = tiles % slots;
-    const int S = rem == 0 ? 1 : std::max(1, std::min(slots / rem, nb / 4));
-    double us = full * (nb * k.stage + k.round);
-    if (rem > 0) { us += (nb + S - 1) / S * k.stage + k.round; }
-    if (S > 1) { us += 3.0 + 0.3e-6 * rem * S * k.bm * k.bn * 4; }
-    if (least == 0 || us < least) {
+  auto consider = [&](const Kind& k, int shares, double us) {
+    if (best == nullptr || us < least) {
+      best = &k;
+      best_shares = shares;
       least = us;
-      best = Plan{false, k.bm, k.bn, k.waves, S};
+    }
+  };
+  for (const Kind& k : kKinds) {
+    double tiles = 0, valid = 0, padded = 0;
+    for (int i = 0; i < b.nprob; ++i) {
+      const double tn = (b.p[i].n + k.bn - 1) / k.bn, tm = (b.p[i].rows + k.bm - 1) / k.bm;
+      tiles += tm * tn;
+      valid += b.p[i].rows * tn;
+      padded += tm * k.bm * tn;
+    }
+    if (k.narrow) {
+      if (rows > k.bm) { continue; }
+      const double load = std::ceil(tiles / C);
+      consider(k, 1, k.fixed + load * (k.round + nb * k.stage) + tiles * nb / C * k.stream);
+      continue;
+    }
+    const int slots = slots_of(k, C), two = slots / C;
+    const double full = std::floor(tiles / slots), rem = tiles - full * slots;
+    const double fixed = k.fixed + mb * k.weight + full * (k.round + nb * two * k.stage);
+    const double tile_mb = 4e-6 * k.bm * k.bn;
+    for (int S = 1; S <= 16; S += S < 4 ? 1 : S < 8 ? 2 : 4) {
+      if (S > 1 && (rem == 0 || S > nb / 2 || rem * S > 2.0 * slots ||
+                    rem * S * tile_mb * 1e6 > workspace)) {
+        break;
+      }
+      double us = fixed;
+      if (rem > 0) {
+        const int nst = (nb + S - 1) / S;
+        const double rounds = std::ceil(rem * S / slots);
+        // the last of them may have a CU to each workgroup
+        const double last = rem * S - (rounds - 1) * slots > C ? two : 1;
+        us += rounds * k.round + ((rounds - 1) * two + last) * nst * k.stage;
+      }
+      if (S > 1) { us += k.split + rem * S * tile_mb * (valid / padded) * k.part; }
+      consider(k, S, us);
     }
   }
-  return best;
+  return set_tiles(b, *best, best_shares);
 }
 
 }  // namespace
@@ -325,9 +359,7 @@ u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream, const uint8_t* xq, const fl
     add_problem(b, xq, sx, p.wq_und, p.sw_und, p.y, M_und, p.N);
   }
   b.cus = u15h::num_cus(ctx);
-  const Plan plan = choose(b, b.cus);
-  if (!set_tiles(b, plan)) { return refuse(ctx, "%s: too many tiles", what); }
-  if (!plan.narrow) { set_split(b, plan, slots_of(plan, b.cus), u15h::split_workspace_bytes(ctx)); }
+  if (!plan(b, u15h::split_workspace_bytes(ctx))) { return refuse(ctx, "%s: too many tiles", what); }
   if (b.split > 1) {
     void* ws = nullptr;
     if ((st = u15h::split_workspace(ctx, &ws)) != U15H_OK) { return st; }

@@ -51,6 +51,18 @@ make_rsrc(const void* base, int bytes)
       reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), 0, n, kRsrcWord3);
 }
 
+// A wave-uniform value made explicitly so: it stays in SGPRs.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <class T>
+__device__ __forceinline__ T*
+uniform(T* p)
+{
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return reinterpret_cast<T*>(((uint64_t)hi << 32) | lo);
+}
+
 // Two floats as packed bf16 (lo in the low half), round to nearest even.
 __device__ __forceinline__ uint32_t
 pack_bf16x2(float lo, float hi)
@@ -450,18 +462,18 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   };
 
   // ---- loads ---------------------------------------------------------------
-  // What the loads of the stage R - 1 ahead need; past the last item they
-  // fetch zeros.
+  // What the loads of the stage R - 1 ahead need, stepped along with the stages;
+  // past the last item they fetch its last block again, for nobody.
   struct {
     __amdgpu_buffer_rsrc_t a, w;
-    const float* sc;      // this wave's scales at the item's first block
-    int pitch, count;     // floats between blocks, floats per block
-    int kbeg, nst, k, round;
+    const float* sc;      // this wave's scales of the block
+    int pitch, count;     // floats between blocks, bytes per block
+    int ko, left, last;   // the block's bytes into a row, blocks left, -1 in the last of K
+    int round;
   } ld;
   const bool row_wave = wave < L::kRowScales / 64;
-  auto load_item = [&](int round) {
-    const int it = item_of(round);
-    const Fp8Work t = fp8_work<BM, BN>(B, nb, max(it, 0));
+  auto load_item = [&](int it) {
+    const Fp8Work t = fp8_work<BM, BN>(B, nb, it);
     const Fp8Problem& P = B.p[t.prob];
     const int rows = min(BM, P.rows - t.row0), cols = min(BN, P.n - t.col0);
     ld.a = make_rsrc(P.a + (size_t)t.row0 * K, rows * K);
@@ -469,16 +481,18 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     if (row_wave) {
       ld.sc = P.sa + (size_t)t.kbeg * sa_pitch + t.row0 + wave * 64;
       ld.pitch = sa_pitch;
-      ld.count = max(0, min(64, rows - wave * 64));
+      ld.count = max(0, min(64, rows - wave * 64)) * 4;
     } else {
       ld.sc = P.sw + (size_t)(t.col0 / 128) * nb + t.kbeg;
       ld.pitch = 1;
-      ld.count = ((cols + 127) / 128 - 1) * nb + 1;
+      ld.count = (((cols + 127) / 128 - 1) * nb + 1) * 4;
     }
-    ld.kbeg = t.kbeg;
-    ld.nst = it < 0 ? 0 : t.nst;
-    ld.k = 0;
-    ld.round = round;
+    ld.sc = uniform(ld.sc);
+    ld.pitch = uniform(ld.pitch);
+    ld.count = uniform(ld.count);
+    ld.ko = uniform(t.kbeg * 128);
+    ld.left = uniform(t.nst);
+    ld.last = uniform(t.kbeg == nb - 1 ? -1 : 0);
   };
   // a load's lane l fills chunk position l % 8 of row l / 8 of its 8 rows
   // activations: wave w fills blocks w, w + NW, .. of the stage (the same one
@@ -513,28 +527,34 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   // Instruction op of the kA of a stage's activations (the last its scales),
   // and of the kW of its weights.
   auto load_a = [&](int slot, int op) {
-    const bool past = ld.k >= ld.nst;
     if (op < LB) {
-      const int oob = (ld.kbeg + ld.k == nb - 1 ? atail : 0) | (past ? kOobOffset : 0);
-      dma16(ld.a, lds + L::kAct + slot * kStage + (blk + NW * op) * 1024, aoff[op] + oob,
-            (ld.kbeg + ld.k) * 128);
+      dma16(ld.a, lds + L::kAct + slot * kStage + (blk + NW * op) * 1024,
+            aoff[op] | (atail & ld.last), ld.ko);
     } else {
       const int g = row_wave ? wave * 64 : L::kRowScales;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          make_rsrc(ld.sc + (size_t)ld.k * ld.pitch, past ? 0 : ld.count * 4),
+          make_rsrc(ld.sc, ld.count),
           (__attribute__((address_space(3))) void*)(scales + slot * L::kScales + g), 4, soff, 0,
           0, 0);
     }
   };
   auto load_w = [&](int slot, int op) {
-    const int oob = (ld.kbeg + ld.k == nb - 1 ? wtail[op & 1] : 0) |
-                    (ld.k >= ld.nst ? kOobOffset : 0);
-    dma16(ld.w, mine + slot * (FI * 2048) + op * 1024, woff[op & 1] + (op >> 1) * 16 * K + oob,
-          (ld.kbeg + ld.k) * 128);
+    dma16(ld.w, mine + slot * (FI * 2048) + op * 1024,
+          (woff[op & 1] + (op >> 1) * 16 * K) | (wtail[op & 1] & ld.last), ld.ko);
   };
-  // (a tile takes an even number of stages: one past the range adds 0 * 0)
   auto advance = [&] {
-    if (++ld.k >= ((ld.nst + 1) & ~1) && ld.nst > 0) { load_item(ld.round + 1); }
+    if (ld.left > 1) {
+      --ld.left;
+      ld.ko += 128;
+      ld.sc += ld.pitch;
+      ld.last = ld.ko == (nb - 1) * 128 ? -1 : 0;
+    } else {
+      const int it = item_of(ld.round + 1);
+      if (it >= 0) {
+        ++ld.round;
+        load_item(it);
+      }
+    }
   };
 
   // ---- fragments -------------------------------------------------------------
@@ -553,12 +573,15 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   auto read_s = [&](int slot, int j) {
     return *reinterpret_cast<const sv_t*>(scales + slot * L::kScales + lr * FJ + j);
   };
+  auto read_w = [&](int slot) { return scales[slot * L::kScales + L::kRowScales + wcol / 128]; };
 
   constexpr int FH = FI < 2 ? 1 : 2, HS = FI / FH;   // products per step, steps per fragment
   f32x4_t acc[FI][FJ], d[2][FH];
   i32x8_t fa[2][FI], fb[FB];
+  // row scales of two groups of SV fragments, the columns' scale of this stage
+  // and the next, and the scale that the last step's results wait for
   sv_t sv[2];
-  float w, wprev;
+  float w, wnext, pending;
   auto clear = [&] {
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
@@ -567,8 +590,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     }
 #pragma unroll
     for (int i = 0; i < FH; ++i) { d[0][i] = d[1][i] = f32x4_t{}; }
-    sv[0] = sv[1] = sv_t{};
-    w = 0.0f;
+    pending = 0.0f;
   };
   auto add = [&](int jp, int hp, int par, float sc) {
 #pragma unroll
@@ -606,7 +628,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   // stored: a tile's results were stored just before.
   auto stage = [&](auto par_c, bool stored, int slot, int next, int ahead, int ws) {
     constexpr int par = decltype(par_c)::value;
-    constexpr int f = par * FJ, g = par * kSvs;
+    constexpr int f = 0, g = par * kSvs;               // (a stage's fragments come round)
     // the next stage's activations have landed in every wave, and every wave
     // has read the last stage's
     if (par == 0 && stored) {
@@ -616,12 +638,11 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     }
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    wprev = w;
+    w = wnext;
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
       // the scale of fragment j - 1
-      const float before = j == 0 ? sv[(g + 1) & 1][SV - 1] * wprev
-                                  : sv[(g + (j - 1) / SV) & 1][(j - 1) % SV] * w;
+      const float before = j == 0 ? pending : sv[(g + (j - 1) / SV) & 1][(j - 1) % SV] * w;
 #pragma unroll
       for (int o = j * kAPerJ; o < (j + 1) * kAPerJ && o < kA; ++o) { load_a(ahead, o); }
       if (j == JR) {
@@ -640,8 +661,12 @@ fp8_tiles(const Fp8Batch& B, char* lds)
           fa[par ^ 1][i] = read_frag(mine + ws * (FI * 2048) + i * 2048);
         }
       }
-      if (j == 0) { w = scales[slot * L::kScales + L::kRowScales + wcol / 128]; }
-      if (j % SV == 0) { sv[(g + j / SV) & 1] = read_s(slot, j); }
+      // the next group's scales, and the next stage's columns', two steps ahead
+      if (j % SV == (SV > 2 ? SV - 2 : 0)) {
+        const int to = j / SV + 1;
+        sv[(g + to) & 1] = to < kSvs ? read_s(slot, to * SV) : read_s(next, 0);
+      }
+      if (j == (FJ > 2 ? FJ - 2 : 0)) { wnext = read_w(next); }
       constexpr int A = FB - 1;                      // fragments read ahead
       fb[(f + j + A) % FB] = j + A < FJ ? read_a(slot, j + A) : read_a(next, j + A - FJ);
 #pragma unroll
@@ -678,16 +703,16 @@ fp8_tiles(const Fp8Batch& B, char* lds)
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    pending = sv[(g + kSvs - 1) & 1][SV - 1] * w;
     settle();
-    // tiles take an even number of stages, so the loads' items end in one of
-    // the two parities only
-    if constexpr ((par + R) % 2 == 0) { advance(); } else { ++ld.k; }
+    advance();
   };
 
   // ---- the first item's first stages -------------------------------------------
   int it = item_of(0);
   if (it < 0) { return; }
-  load_item(0);
+  ld.round = 0;
+  load_item(it);
   // the loads' order is a stage's: activations, then the next stage's weights,
   // the first stage's before all
 #pragma unroll
@@ -713,6 +738,8 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   for (int i = 0; i < FI; ++i) { fa[0][i] = read_frag(mine + i * 2048); }
 #pragma unroll
   for (int a = 0; a < FB - 1; ++a) { fb[a] = read_a(0, a); }
+  sv[0] = read_s(0, 0);
+  wnext = read_w(0);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < FI; ++i) { asm volatile("" : "+v"(fa[0][i])); }
@@ -720,24 +747,33 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   for (int o = 0; o < kW; ++o) { load_w(0, o); }
   __builtin_amdgcn_sched_barrier(0);
   advance();
-  static_assert(2 * FJ % FB == 0 && FB - 1 <= FJ, "the fragment buffers come round with two stages");
+  static_assert(FJ % FB == 0 && FJ * HS % 2 == 0, "the fragment buffers come round with a stage");
 
-  int cur = 0, ws = WS > 1 ? 1 : 0, round = 0;
+  int cur = 0, next = 1, behind = R - 1, ws = WS > 1 ? 1 : 0, round = 0;
   using std::integral_constant;
+  auto step = [&](auto par_c, bool stored) {
+    stage(par_c, stored, cur, next, behind, ws);
+    behind = cur;
+    cur = next;
+    next = next + 1 == R ? 0 : next + 1;
+    ws = ws + 1 == WS ? 0 : ws + 1;
+  };
   clear();
   for (;;) {
     const Fp8Work t = fp8_work<BM, BN>(B, nb, it);
     const Fp8Problem& P = B.p[t.prob];
-    for (int k = 0; k < t.nst; k += 2) {
-      const int s1 = cur + 1 == R ? 0 : cur + 1, s2 = s1 + 1 == R ? 0 : s1 + 1;
-      stage(integral_constant<int, 0>{}, k == 0 && round > 0, cur, s1,
-            cur == 0 ? R - 1 : cur - 1, ws);
-      ws = ws + 1 == WS ? 0 : ws + 1;
-      stage(integral_constant<int, 1>{}, false, s1, s2, cur, ws);
-      ws = ws + 1 == WS ? 0 : ws + 1;
-      cur = s2;
+    for (int k = 0; k + 1 < t.nst; k += 2) {
+      step(integral_constant<int, 0>{}, k == 0 && round > 0);
+      step(integral_constant<int, 1>{}, false);
     }
-    add(FJ - 1, HS - 1, 1, sv[1][SV - 1] * w);
+    if (t.nst & 1) {
+      step(integral_constant<int, 0>{}, t.nst == 1 && round > 0);
+      // the next stage is an even one again
+#pragma unroll
+      for (int i = 0; i < FI; ++i) { fa[0][i] = fa[1][i]; }
+      if constexpr (kSvs % 2 == 1) { sv[0] = sv[1]; }
+    }
+    add(FJ - 1, HS - 1, 1, pending);
 
     // ---- results: kStores stores whatever the tile's edges, which drop some ------
     const int rows = min(BM, P.rows - t.row0);
@@ -1018,6 +1054,13 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 hipError_t
 launch_fp8_gemm(const Fp8Batch& b, hipStream_t s)
 {
+  // whole tiles, or a tail in two shares or more that has a workspace
+  const bool split = b.split_begin != b.total_tiles;
+  if (b.total_tiles <= 0 || b.split_begin < 0 || b.split_begin > b.total_tiles ||
+      (split ? b.narrow || b.split < 2 || b.split > (b.K + 127) / 128 || b.ws == nullptr
+             : b.split != 1)) {
+    return hipErrorInvalidValue;
+  }
 #define U15H_CASE(MT, FI, NW, D)                                                          \
   if (b.narrow && b.bm == 16 * MT && b.bn == 16 * FI && b.waves == NW) {              \
     fp8_narrow_kernel<MT, FI, NW, D><<<b.total_tiles, 64 * NW, 0, s>>>(b);               \
