@@ -20,6 +20,7 @@ import ctypes
 import os
 import pathlib
 import re
+import struct
 
 import torch
 
@@ -52,10 +53,10 @@ class _MotProjI8(ctypes.Structure):
                 ("y", ctypes.c_void_p), ("N", ctypes.c_int)]
 
 
-class _MotProjFp8(ctypes.Structure):
-    _fields_ = [("wq_und", ctypes.c_void_p), ("sw_und", ctypes.c_void_p),
-                ("wq_gen", ctypes.c_void_p), ("sw_gen", ctypes.c_void_p),
-                ("y", ctypes.c_void_p), ("N", ctypes.c_int)]
+# n u15h_mot_proj_fp8 in a row: five pointers and an int each, padded to a
+# pointer's alignment
+_PROJ_FP8 = [struct.Struct("@" + "PPPPPi0P" * n) for n in range(1, MAX_PROJ + 1)]
+_BF16, _F8, _F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32
 
 
 class _LayerIO(ctypes.Structure):
@@ -131,8 +132,7 @@ def load_library() -> ctypes.CDLL:
         "u15h_mot_rms_norm_fp8": (i, [vp, vp, vp, vp, vp, i, i, i, vp, vp,
                                       ctypes.c_float, vp, vp, vp]),
         "u15h_swiglu_quant_fp8": (i, [vp, vp, vp, vp, i, i, vp, vp, vp]),
-        "u15h_mot_gemm_fp8": (i, [vp, vp, vp, vp, i, i, i,
-                                  ctypes.POINTER(_MotProjFp8), i]),
+        "u15h_mot_gemm_fp8": (i, [vp, vp, vp, vp, i, i, i, vp, i]),
         "u15h_route_rows": (i, [vp, i, vp, ctypes.POINTER(i),
                                 ctypes.POINTER(i)]),
         "u15h_dequant_affine": (i, [vp, vp, ctypes.POINTER(_QWeight), i, i,
@@ -558,11 +558,6 @@ def _need(t, dtype, shape, name):
         raise ValueError(f"{name} must be on the GPU")
 
 
-def _blocks(n):
-    """Blocks of 128 (the last one maybe shorter) in n."""
-    return (n + 127) // 128
-
-
 def layer_scratch(stack, M, tier=TIER_BF16, device="cuda"):
     """The scratch buffers of u15h_stack_layer_full for M rows."""
     def bf(n):
@@ -834,32 +829,37 @@ class Ops:
 
     # ---- profiling -------------------------------------------------------
     # ---- fp8 tier ------------------------------------------------------
+    # The smallest of these calls take less on the GPU than on the host, so a
+    # tensor's checks and its address are one pass, and the stream is looked up
+    # without asking whether CUDA is up (a checked tensor lives on it).
     def _stream_here(self, stream):
         """The call's stream: the current one of this context's device."""
         if stream is not None:
             return stream.cuda_stream
-        if _raw_stream is not None and torch.cuda.is_initialized():
+        if _raw_stream is not None:
             return _raw_stream(self.device)
         return torch.cuda.current_stream(self.device).cuda_stream
 
-    def _need_here(self, t, dtype, shape, name):
-        """_need, and that the tensor is on this context's device."""
+    def _at(self, t, dtype, shape, name):
+        """The address of a tensor of this type and shape, contiguous and on
+        this context's device; raises otherwise."""
+        if t is not None and t.dtype is dtype and t.shape == shape and t.is_contiguous() \
+                and t.get_device() == self.device:
+            return t.data_ptr()
         _need(t, dtype, shape, name)
-        if t.get_device() != self.device:
-            raise ValueError(f"{name} is on cuda:{t.get_device()}, this context on "
-                             f"cuda:{self.device}")
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, this context on "
+                         f"cuda:{self.device}")
 
     def quant_rows_fp8(self, x, q, s, stream=None):
         """e4m3 codes q [rows][K] of x and their scales s [blocks of
         K][rows], one per row and 128 columns."""
         if x.dim() != 2:
             raise ValueError("x must be [rows][K]")
-        rows, K = x.shape
-        self._need_here(x, torch.bfloat16, (rows, K), "x")
-        self._need_here(q, torch.float8_e4m3fn, (rows, K), "q")
-        self._need_here(s, torch.float32, (_blocks(K), rows), "s")
-        st = self._lib.u15h_quant_rows_fp8(self._ctx, self._stream_here(stream), x.data_ptr(),
-                                           rows, K, q.data_ptr(), s.data_ptr())
+        rows, K = shape = x.shape
+        at = self._at
+        st = self._lib.u15h_quant_rows_fp8(
+            self._ctx, self._stream_here(stream), at(x, _BF16, shape, "x"), rows, K,
+            at(q, _F8, shape, "q"), at(s, _F32, ((K + 127) // 128, rows), "s"))
         if st:
             self._check(st, "u15h_quant_rows_fp8")
 
@@ -868,12 +868,12 @@ class Ops:
         N][blocks of K], one per 128 x 128."""
         if w.dim() != 2:
             raise ValueError("w must be [N][K]")
-        N, K = w.shape
-        self._need_here(w, torch.bfloat16, (N, K), "w")
-        self._need_here(q, torch.float8_e4m3fn, (N, K), "q")
-        self._need_here(s, torch.float32, (_blocks(N), _blocks(K)), "s")
-        st = self._lib.u15h_quant_blocks_fp8(self._ctx, self._stream_here(stream),
-                                             w.data_ptr(), N, K, q.data_ptr(), s.data_ptr())
+        N, K = shape = w.shape
+        at = self._at
+        st = self._lib.u15h_quant_blocks_fp8(
+            self._ctx, self._stream_here(stream), at(w, _BF16, shape, "w"), N, K,
+            at(q, _F8, shape, "q"),
+            at(s, _F32, ((N + 127) // 128, (K + 127) // 128), "s"))
         if st:
             self._check(st, "u15h_quant_blocks_fp8")
 
@@ -886,27 +886,22 @@ class Ops:
         rows = M_und + M_gen
         if x.dim() != 2 or x.shape[0] != rows:
             raise ValueError(f"x must be [{rows}][dim]")
-        dim = x.shape[1]
-        self._need_here(x, torch.bfloat16, (rows, dim), "x")
-        if M_und:
-            self._need_here(w_und, torch.bfloat16, (dim,), "w_und")
-        if M_gen:
-            self._need_here(w_gen, torch.bfloat16, (dim,), "w_gen")
-        self._need_here(q, torch.float8_e4m3fn, (rows, dim), "q")
-        self._need_here(s, torch.float32, (_blocks(dim), rows), "s")
-        if delta is not None:
-            self._need_here(delta, torch.bfloat16, (rows, dim), "delta")
-            if x_out is None:
-                x_out = x
-        elif x_out is not None:
+        shape = x.shape
+        dim = shape[1]
+        at = self._at
+        if delta is None and x_out is not None:
             raise ValueError("x_out is written only with delta")
-        if x_out is not None:
-            self._need_here(x_out, torch.bfloat16, (rows, dim), "x_out")
-        if y is not None:
-            self._need_here(y, torch.bfloat16, (rows, dim), "y")
+        xp = at(x, _BF16, shape, "x")
+        dp = op = None
+        if delta is not None:
+            dp = at(delta, _BF16, shape, "delta")
+            op = xp if x_out is None else at(x_out, _BF16, shape, "x_out")
         st = self._lib.u15h_mot_rms_norm_fp8(
-            self._ctx, self._stream_here(stream), x.data_ptr(), _ptr(delta), _ptr(x_out), M_und,
-            M_gen, dim, _ptr(w_und), _ptr(w_gen), eps, _ptr(y), q.data_ptr(), s.data_ptr())
+            self._ctx, self._stream_here(stream), xp, dp, op, M_und, M_gen, dim,
+            at(w_und, _BF16, (dim,), "w_und") if M_und else None,
+            at(w_gen, _BF16, (dim,), "w_gen") if M_gen else None, eps,
+            None if y is None else at(y, _BF16, shape, "y"), at(q, _F8, shape, "q"),
+            at(s, _F32, ((dim + 127) // 128, rows), "s"))
         if st:
             self._check(st, "u15h_mot_rms_norm_fp8")
 
@@ -915,16 +910,13 @@ class Ops:
         [blocks of inter][rows] (and h in bf16 when given)."""
         if gate.dim() != 2:
             raise ValueError("gate must be [rows][inter]")
-        rows, inter = gate.shape
-        self._need_here(gate, torch.bfloat16, (rows, inter), "gate")
-        self._need_here(up, torch.bfloat16, (rows, inter), "up")
-        self._need_here(q, torch.float8_e4m3fn, (rows, inter), "q")
-        self._need_here(s, torch.float32, (_blocks(inter), rows), "s")
-        if h is not None:
-            self._need_here(h, torch.bfloat16, (rows, inter), "h")
-        st = self._lib.u15h_swiglu_quant_fp8(self._ctx, self._stream_here(stream),
-                                             gate.data_ptr(), up.data_ptr(), rows, inter,
-                                             _ptr(h), q.data_ptr(), s.data_ptr())
+        rows, inter = shape = gate.shape
+        at = self._at
+        st = self._lib.u15h_swiglu_quant_fp8(
+            self._ctx, self._stream_here(stream), at(gate, _BF16, shape, "gate"),
+            at(up, _BF16, shape, "up"), rows, inter,
+            None if h is None else at(h, _BF16, shape, "h"), at(q, _F8, shape, "q"),
+            at(s, _F32, ((inter + 127) // 128, rows), "s"))
         if st:
             self._check(st, "u15h_swiglu_quant_fp8")
 
@@ -934,32 +926,30 @@ class Ops:
         weights and the next M_gen with the gen weights; xq, sx and the
         weights as quant_rows_fp8 and quant_blocks_fp8 make them."""
         M = M_und + M_gen
-        kb = _blocks(K)
-        self._need_here(xq, torch.float8_e4m3fn, (M, K), "xq")
-        self._need_here(sx, torch.float32, (kb, M), "sx")
+        kb = (K + 127) // 128
         n = len(projs)
         if not 1 <= n <= MAX_PROJ:
             raise ValueError(f"1..{MAX_PROJ} projections per launch")
-        arr = (_MotProjFp8 * n)()
-        for p, a in zip(projs, arr):
+        at = self._at
+        xp, sp = at(xq, _F8, (M, K), "xq"), at(sx, _F32, (kb, M), "sx")
+        table = []
+        for p in projs:
             y = p["y"]
             if y.dim() != 2:
                 raise ValueError("y must be [M][N]")
             N = y.shape[1]
-            self._need_here(y, torch.bfloat16, (M, N), "y")
-            a.y, a.N = y.data_ptr(), N
+            ws, ss = (N, K), ((N + 127) // 128, kb)
             if M_und:
-                w, sw = p["wq_und"], p["sw_und"]
-                self._need_here(w, torch.float8_e4m3fn, (N, K), "wq_und")
-                self._need_here(sw, torch.float32, (_blocks(N), kb), "sw_und")
-                a.wq_und, a.sw_und = w.data_ptr(), sw.data_ptr()
+                table += (at(p["wq_und"], _F8, ws, "wq_und"), at(p["sw_und"], _F32, ss, "sw_und"))
+            else:
+                table += (0, 0)
             if M_gen:
-                w, sw = p["wq_gen"], p["sw_gen"]
-                self._need_here(w, torch.float8_e4m3fn, (N, K), "wq_gen")
-                self._need_here(sw, torch.float32, (_blocks(N), kb), "sw_gen")
-                a.wq_gen, a.sw_gen = w.data_ptr(), sw.data_ptr()
-        st = self._lib.u15h_mot_gemm_fp8(self._ctx, self._stream_here(stream), xq.data_ptr(),
-                                         sx.data_ptr(), M_und, M_gen, K, arr, n)
+                table += (at(p["wq_gen"], _F8, ws, "wq_gen"), at(p["sw_gen"], _F32, ss, "sw_gen"))
+            else:
+                table += (0, 0)
+            table += (at(y, _BF16, (M, N), "y"), N)
+        st = self._lib.u15h_mot_gemm_fp8(self._ctx, self._stream_here(stream), xp, sp, M_und,
+                                         M_gen, K, _PROJ_FP8[n - 1].pack(*table), n)
         if st:
             self._check(st, "u15h_mot_gemm_fp8")
 
