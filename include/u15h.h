@@ -555,7 +555,7 @@ u15h_status u15h_mot_gemm_i8(u15h_ctx* ctx, u15h_stream stream,
  * so that every row of codes starts 16-byte aligned. */
 
 /* Codes q [rows][K] and scales s [KB][rows] of bf16 activations x
- * [rows][K].  K <= 131072, rows <= 2^24. */
+ * [rows][K].  K <= 131072, rows <= 2^22. */
 u15h_status u15h_quant_rows_fp8(u15h_ctx* ctx, u15h_stream stream,
                                 const u15h_bf16* x, int rows, int K,
                                 uint8_t* q, float* s);
@@ -586,7 +586,7 @@ u15h_status u15h_mot_rms_norm_fp8(u15h_ctx* ctx, u15h_stream stream,
 /* The down projection's fp8 input in one pass: h = silu(gate) * up in f32,
  * its codes q [rows][inter] and scales s [ceil(inter / 128)][rows] (of the
  * f32 values, rounded once), and bf16(h) where h is not NULL.
- * inter <= 131072, rows <= 2^24. */
+ * inter <= 131072, rows <= 2^22. */
 u15h_status u15h_swiglu_quant_fp8(u15h_ctx* ctx, u15h_stream stream,
                                   const u15h_bf16* gate, const u15h_bf16* up,
                                   int rows, int inter, u15h_bf16* h,
@@ -615,7 +615,7 @@ typedef struct {
  * bf16 is larger).  Tiles that leave a partial round split K over
  * workgroups, whose f32 sums go to the context's split-K workspace.
  * Limits: 1 <= nproj <= U15H_MAX_PROJ, K % 16 == 0, K <= 131072,
- * N % 8 == 0, N <= 2^20, M_und + M_gen <= 2^24. */
+ * N % 8 == 0, N <= 2^20, M_und + M_gen <= 2^22. */
 u15h_status u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream,
                               const uint8_t* xq, const float* sx, int M_und,
                               int M_gen, int K, const u15h_mot_proj_fp8* proj,

@@ -16,7 +16,7 @@ using u15h::Fp8Batch;
 using u15h::Fp8Problem;
 
 constexpr int kMaxK = 131072;
-constexpr int kMaxRows = 1 << 24;
+constexpr int kMaxRows = 1 << 22;    // a norm's workgroups of 512 threads: 2^31 threads
 constexpr int kMaxN = 1 << 20;
 
 u15h_status

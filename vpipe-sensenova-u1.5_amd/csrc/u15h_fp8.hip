@@ -35,6 +35,8 @@ typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRsrcWord3 = 0x00020000;      // raw buffer, 32-bit data format
 constexpr int kOobOffset = 0x40000000;      // any offset past every resource
+constexpr int kNonTemporal = 2;             // a load's or store's cache policy
+constexpr int kRowGroups = 16384;           // of a launch's y dimension
 constexpr float kFp8Top = 448.0f;
 constexpr float kFp8Least = 0x1p-126f;
 
@@ -142,8 +144,17 @@ swiglu_f32(float g, float u)
 // ---- rows: codes and block-major scales --------------------------------------
 // One workgroup of four waves per 4 RPW rows x 512 columns.  A wave reads 512
 // columns of a row at a time, lane l columns 8 l..8 l + 7, so a block of 128 is
-// 16 neighbouring lanes; all of its RPW rows' loads issue first.  The scales
-// of the workgroup's rows are gathered in LDS and written as runs of 4 RPW.
+// 16 neighbouring lanes; all of its loads issue first (two: RPW rows of one
+// operand, or a row of two).  The scales of the workgroup's rows are gathered
+// in LDS and written as runs of 4 RPW.
+// Bound by memory: 2 bytes read (4 for SwiGLU) and 1 + 1/32 written per value.
+// Workgroups walk a row's columns first, so those that run together read whole
+// rows: 4224 rows of 12288 take 27.5 us (5.7 TB/s; SwiGLU 47 us, 5.6 TB/s)
+// against 33.5 (53) walking the rows first.  The operands are read once and
+// for the last time, so past the caches' other lines (non-temporal): 1.0 (1.2)
+// us of it.  The codes are stored plainly: stored past the caches these take 2
+// us less and the product that reads them 2 more.  Four rows of 4096: 2.0 us,
+// a launch.
 template <bool SWIGLU, int RPW>
 __global__ __launch_bounds__(256) void
 fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ up, int rows,
@@ -154,7 +165,9 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
   __shared__ float scales[4][R];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  const int row0 = blockIdx.x * R, col = blockIdx.y * 512 + lane * 8;
+  const int group = blockIdx.z * kRowGroups + blockIdx.y;
+  const int row0 = group * R, col = blockIdx.x * 512 + lane * 8;
+  if (row0 >= rows) { return; }
   const int valid = min(R, rows - row0);
   const int oob = col < K ? 0 : kOobOffset;
   const size_t base = (size_t)row0 * K;
@@ -165,8 +178,10 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
 #pragma unroll
   for (int i = 0; i < RPW; ++i) {
     const int at = (wave * RPW + i) * K + col;
-    xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xs, at * 2 + oob, 0, 0);
-    if constexpr (SWIGLU) { uv[i] = __builtin_amdgcn_raw_buffer_load_b128(us, at * 2 + oob, 0, 0); }
+    xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xs, at * 2 + oob, 0, kNonTemporal);
+    if constexpr (SWIGLU) {
+      uv[i] = __builtin_amdgcn_raw_buffer_load_b128(us, at * 2 + oob, 0, kNonTemporal);
+    }
   }
 #pragma unroll
   for (int i = 0; i < RPW; ++i) {
@@ -193,7 +208,7 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
   __syncthreads();
   const int nb = (K + kFp8Block - 1) / kFp8Block;
   for (int t = threadIdx.x; t < 4 * R; t += 256) {
-    const int b = blockIdx.y * 4 + t / R, r = t % R;
+    const int b = blockIdx.x * 4 + t / R, r = t % R;
     if (b < nb && r < valid) { sc[(size_t)b * rows + row0 + r] = scales[t / R][r]; }
   }
 }
@@ -201,6 +216,9 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
 // ---- weights: a scale per 128 x 128 ------------------------------------------
 // One workgroup of four waves per block; a wave reads four rows' 256 bytes at a
 // time (lane l: row l / 16, columns 8 (l % 16)..), eight such reads in flight.
+// Bound by memory: 3 bytes per value, 12288 x 4096 in 27.7 us (5.5 TB/s).  A
+// weight is read once and its codes wait for a later use, so both go past the
+// caches' other lines (non-temporal); plainly it is 30.4 us.
 __global__ __launch_bounds__(256) void
 fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* __restrict__ q,
                         float* __restrict__ sc)
@@ -218,7 +236,7 @@ fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* _
   u32x4_t v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    v[i] = __builtin_amdgcn_raw_buffer_load_b128(ws, (at + i * 16 * K) * 2 + oob, 0, 0);
+    v[i] = __builtin_amdgcn_raw_buffer_load_b128(ws, (at + i * 16 * K) * 2 + oob, 0, kNonTemporal);
   }
   uint32_t m = 0;
 #pragma unroll
@@ -239,7 +257,8 @@ fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* _
   for (int i = 0; i < 8; ++i) {
     float f[8];
     unpack8(v[i], f);
-    __builtin_amdgcn_raw_buffer_store_b64(codes8(f, inv), qs, at + i * 16 * K + oob, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b64(codes8(f, inv), qs, at + i * 16 * K + oob, 0,
+                                         kNonTemporal);
   }
 }
 
@@ -252,6 +271,13 @@ fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* _
 //   by xor shuffles, the row through LDS.
 // The codes are those of n itself, rounded once; y, where wanted, is bf16(n).
 // Every store of a row follows all of its loads, so x_out may be x.
+// Bound by memory: with the add 7 bytes per value (5 in, out 2 and the codes),
+// 4224 rows of 4096 in 23.7 us (5.1 TB/s); without it 3 bytes, 13.8 us (3.8
+// TB/s).  x, d and r go past the caches' other lines (non-temporal): d is read
+// for the last time and x's or r's next reader is half a layer away; plainly 25.4
+// and 15.1 us.  A row of 4096 has eight waves with the add, two loads each as
+// it has with four waves without it: eight against four take 2.3 against 2.4 us
+// for one row and 23 to 24 both for 4224 with the add, 15.1 against 13.8 without.
 template <int WPR, int CPL, bool ADD>
 __global__ __launch_bounds__(64 * WPR) void
 fp8_norm_kernel(const Fp8NormArgs A)
@@ -266,7 +292,7 @@ fp8_norm_kernel(const Fp8NormArgs A)
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
     const int c = (i * WPR + part) * 64 + lane;
-    v[i] = __builtin_amdgcn_raw_buffer_load_b128(xs, c * 16, 0, 0);
+    v[i] = __builtin_amdgcn_raw_buffer_load_b128(xs, c * 16, 0, kNonTemporal);
     g[i] = __builtin_amdgcn_raw_buffer_load_b128(ws, c * 16, 0, 0);
   }
   if constexpr (ADD) {
@@ -275,7 +301,8 @@ fp8_norm_kernel(const Fp8NormArgs A)
     u32x4_t d[CPL];
 #pragma unroll
     for (int i = 0; i < CPL; ++i) {
-      d[i] = __builtin_amdgcn_raw_buffer_load_b128(ds, ((i * WPR + part) * 64 + lane) * 16, 0, 0);
+      d[i] = __builtin_amdgcn_raw_buffer_load_b128(ds, ((i * WPR + part) * 64 + lane) * 16, 0,
+                                                   kNonTemporal);
     }
 #pragma unroll
     for (int i = 0; i < CPL; ++i) {
@@ -284,7 +311,8 @@ fp8_norm_kernel(const Fp8NormArgs A)
         v[i][e] = pack_bf16x2(bf16_lo(v[i][e]) + bf16_lo(d[i][e]),
                               bf16_hi(v[i][e]) + bf16_hi(d[i][e]));
       }
-      __builtin_amdgcn_raw_buffer_store_b128(v[i], os, ((i * WPR + part) * 64 + lane) * 16, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b128(v[i], os, ((i * WPR + part) * 64 + lane) * 16, 0,
+                                             kNonTemporal);
     }
   }
   float ss = 0.0f;
@@ -1010,16 +1038,11 @@ tile_launch(const Fp8Batch& b, hipStream_t s)
   return hipGetLastError();
 }
 
-template <int WPR, int CPL>
+template <int WPR, int CPL, bool ADD>
 void
 norm_launch(const Fp8NormArgs& a, hipStream_t s)
 {
-  const dim3 grid(a.rows), block(64 * WPR);
-  if (a.d != nullptr) {
-    fp8_norm_kernel<WPR, CPL, true><<<grid, block, 0, s>>>(a);
-  } else {
-    fp8_norm_kernel<WPR, CPL, false><<<grid, block, 0, s>>>(a);
-  }
+  fp8_norm_kernel<WPR, CPL, ADD><<<a.rows, 64 * WPR, 0, s>>>(a);
 }
 
 template <bool SWIGLU, int RPW>
@@ -1027,7 +1050,9 @@ void
 rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h, uint8_t* q,
             float* sc, hipStream_t s)
 {
-  const dim3 grid((rows + 4 * RPW - 1) / (4 * RPW), (K + 511) / 512);
+  const int groups = (rows + 4 * RPW - 1) / (4 * RPW);
+  const dim3 grid((K + 511) / 512, std::min(groups, kRowGroups),
+                  (groups + kRowGroups - 1) / kRowGroups);
   fp8_quant_rows_kernel<SWIGLU, RPW><<<grid, 256, 0, s>>>(x, up, rows, K, h, q, sc);
 }
 
@@ -1080,15 +1105,9 @@ launch_fp8_quant_rows(const uint16_t* x, const uint16_t* up, int rows, int K, ui
                       uint8_t* q, float* sc, hipStream_t s)
 {
   if (up != nullptr) {
-    if (rows >= 1024) {
-      rows_launch<true, 4>(x, up, rows, K, h, q, sc, s);
-    } else {
-      rows_launch<true, 1>(x, up, rows, K, h, q, sc, s);
-    }
-  } else if (rows >= 1024) {
-    rows_launch<false, 8>(x, up, rows, K, h, q, sc, s);
+    rows_launch<true, 1>(x, up, rows, K, h, q, sc, s);
   } else {
-    rows_launch<false, 1>(x, up, rows, K, h, q, sc, s);
+    rows_launch<false, 2>(x, up, rows, K, h, q, sc, s);
   }
   return hipGetLastError();
 }
@@ -1104,14 +1123,15 @@ launch_fp8_quant_blocks(const uint16_t* w, int N, int K, uint8_t* q, float* sc, 
 hipError_t
 launch_fp8_norm(const Fp8NormArgs& a, hipStream_t s)
 {
+  const bool add = a.d != nullptr;
   if (a.dim <= 2048) {
-    norm_launch<4, 1>(a, s);
+    add ? norm_launch<4, 1, true>(a, s) : norm_launch<4, 1, false>(a, s);
   } else if (a.dim <= 4096) {
-    norm_launch<4, 2>(a, s);
+    add ? norm_launch<8, 1, true>(a, s) : norm_launch<4, 2, false>(a, s);
   } else if (a.dim <= 8192) {
-    norm_launch<8, 2>(a, s);
+    add ? norm_launch<8, 2, true>(a, s) : norm_launch<8, 2, false>(a, s);
   } else {
-    norm_launch<8, 4>(a, s);
+    add ? norm_launch<8, 4, true>(a, s) : norm_launch<8, 4, false>(a, s);
   }
   return hipGetLastError();
 }
@@ -1120,15 +1140,13 @@ bool
 fp8_kernels_loadable()
 {
   const void* fns[] = {
-      reinterpret_cast<const void*>(&fp8_quant_rows_kernel<false, 1>),
-      reinterpret_cast<const void*>(&fp8_quant_rows_kernel<false, 8>),
+      reinterpret_cast<const void*>(&fp8_quant_rows_kernel<false, 2>),
       reinterpret_cast<const void*>(&fp8_quant_rows_kernel<true, 1>),
-      reinterpret_cast<const void*>(&fp8_quant_rows_kernel<true, 4>),
       reinterpret_cast<const void*>(&fp8_quant_blocks_kernel),
       reinterpret_cast<const void*>(&fp8_norm_kernel<4, 1, false>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<4, 1, true>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<4, 2, false>),
-      reinterpret_cast<const void*>(&fp8_norm_kernel<4, 2, true>),
+      reinterpret_cast<const void*>(&fp8_norm_kernel<8, 1, true>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 2, false>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 2, true>),
       reinterpret_cast<const void*>(&fp8_norm_kernel<8, 4, false>),
