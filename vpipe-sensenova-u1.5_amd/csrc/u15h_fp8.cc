@@ -98,30 +98,31 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
 //           takes two stages), `split` for the second launch with K shares and
 //           `part` per MB of their sums;
 //   and `weight` per MB of weights.
-// Fitted to 7250 timings (a graph, weights rotated; M 1-2800, K 256-12288, N
-// 512-24576, every kind and 1 to 16 shares), each to 5-9% on the mean; the kind
-// and shares with the least estimate take 1.4% longer than the fastest of all,
-// on the mean over the 325 sizes, and 31% at worst (65 rows, K 8192, N 1024:
-// 15.8 against 12.1 us).
+// Fitted to 8858 timings (a graph, weights rotated; M 1-4224, K 256-12288, N
+// 512-24576, every kind and 1 to 16 shares), each to 4-9% on the mean; the kind
+// and shares with the least estimate take 1.2% longer than the fastest of all,
+// on the mean over the 338 sizes, and 36% at worst (65 rows, K 8192, N 1024:
+// 16.3 against 12.0 us).
 struct Kind {
   bool narrow;
   int bm, bn, waves;
   double fixed, round, stage, stream, split, part, weight;
 };
 constexpr Kind kKinds[] = {
-    {true, 16, 16, 4, 2.57, 0.61, 0.0407, 0.0622, 0, 0, 0},
-    {true, 16, 32, 4, 2.10, 1.33, 0.0516, 0.1525, 0, 0, 0},
-    {true, 32, 16, 4, 1.82, 1.59, 0.0613, 0.0587, 0, 0, 0},
-    {true, 32, 32, 4, 2.43, 1.26, 0.0674, 0.1547, 0, 0, 0},
-    {true, 64, 16, 4, 1.55, 2.08, 0.0836, 0.0818, 0, 0, 0},
-    {true, 64, 32, 4, 3.74, 0.44, 0.0894, 0.2003, 0, 0, 0},
-    {true, 96, 16, 4, 1.48, 2.32, 0.1122, 0.0918, 0, 0, 0},
-    {true, 128, 16, 4, 1.39, 2.83, 0.1437, 0.0984, 0, 0, 0},
-    {false, 64, 128, 4, 5.09, 0.03, 0.350, 0, 3.15, 0.397, 0.109},
-    {false, 128, 128, 4, 5.50, 0, 0.521, 0, 3.19, 0.341, 0.123},
-    {false, 128, 256, 8, 4.28, 2.94, 0.738, 0, 4.06, 0.370, 0.100},
-    {false, 192, 256, 8, 4.91, 5.51, 0.952, 0, 5.73, 0.179, 0.118},
-    {false, 256, 256, 8, 11.74, 0, 1.2235, 0, 6.12, 0.135, 0.094},
+    {true, 16, 16, 4, 2.56, 0.61, 0.0410, 0.0615, 0, 0, 0},
+    {true, 16, 32, 4, 2.27, 1.13, 0.0513, 0.1562, 0, 0, 0},
+    {true, 32, 16, 4, 1.78, 1.65, 0.0618, 0.0570, 0, 0, 0},
+    {true, 32, 32, 4, 2.41, 1.28, 0.0672, 0.1558, 0, 0, 0},
+    {true, 64, 16, 4, 1.55, 2.09, 0.0843, 0.0802, 0, 0, 0},
+    {true, 64, 32, 4, 3.58, 0.59, 0.0900, 0.1987, 0, 0, 0},
+    {true, 96, 16, 4, 1.46, 2.35, 0.1126, 0.0899, 0, 0, 0},
+    {true, 128, 16, 4, 1.38, 2.83, 0.1445, 0.0962, 0, 0, 0},
+    {false, 64, 128, 4, 4.15, 0.51, 0.330, 0, 3.34, 0.335, 0.119},
+    {false, 128, 128, 4, 4.89, 0, 0.534, 0, 3.48, 0.276, 0.141},
+    {false, 128, 128, 8, 2.71, 2.59, 0.505, 0, 3.41, 0.363, 0.081},
+    {false, 128, 256, 8, 2.60, 3.38, 0.731, 0, 3.59, 0.295, 0.112},
+    {false, 192, 256, 8, 5.39, 1.70, 1.068, 0, 3.46, 0.206, 0.145},
+    {false, 256, 256, 8, 8.10, 0, 1.2818, 0, 4.49, 0.139, 0.128},
 };
 
 // Workgroups of a kind of tile that run at once.

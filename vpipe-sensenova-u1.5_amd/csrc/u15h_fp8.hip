@@ -426,56 +426,58 @@ fp8_work(const Fp8Batch& B, int nb, int w)
   return t;
 }
 
-// LDS of a workgroup: R stages of scales (the tile's rows', then its columns'),
-// R stages of activations, WS = R - 2 of weights.
-template <int BM, int FI, int NW, int R>
-struct Fp8Lds {
-  static constexpr int WS = R - 2;
+// A workgroup's tile: WM x WN waves, each FJ fragments of activation rows by FI
+// of weight rows.  Its LDS: NS stages of scales (the tile's rows', then its
+// columns'), of activations and of weights.
+template <int WM, int WN, int FJ, int FI, int NS>
+struct Fp8Tile {
+  static constexpr int kWaves = WM * WN;
+  static constexpr int BM = 16 * WM * FJ, BN = 16 * WN * FI;
   static constexpr int kRowScales = (BM + 63) / 64 * 64;
   static constexpr int kScales = kRowScales + 64;                // floats per stage
-  static constexpr int kAct = (R * kScales * 4 + 1023) / 1024 * 1024;
-  static constexpr int kWeight = kAct + R * BM * 128;
-  static constexpr int kBytes = kWeight + NW * WS * FI * 2048;
+  static constexpr int kAct = (NS * kScales * 4 + 1023) / 1024 * 1024;
+  static constexpr int kWeight = kAct + NS * BM * 128;
+  static constexpr int kBytes = kWeight + NS * BN * 128;
+  static constexpr int kPerCu = std::max(std::min(160 * 1024 / kBytes, 8 / kWaves), 1);
 };
 
-// NW waves, each all BM activation rows x 16 FI weight rows; one stage is one
-// block of K.  Both operands come through LDS by direct loads of 1 KiB (8 rows x
-// 128 bytes: 12 cycles each; loaded to registers in a fragment's layout, 16 rows
-// x 64 bytes, the same bytes take 64).
-// The activation rows are shared: R stages of them, handed over by one barrier
-// a stage.  A wave's weights are its own: it reads a stage's fragments into
-// registers during the stage before and refills their place at once, waiting
-// for no other wave.
+// One stage is one block of K.  Both operands come through LDS by direct loads
+// of 1 KiB (8 rows x 128 bytes: 12 cycles each; loaded to registers in a
+// fragment's layout, 16 rows x 64 bytes, the same bytes take 64).
+// A wave holds a stage's weight fragments and walks its activation fragments
+// j, read A = FB - 1 ahead; the results of the step before join the sums (one
+// multiply-add each) while the matrix unit works.  What bounds the large tiles
+// is the LDS's reads and their power, hence nearly square tiles per wave.
+// One barrier a stage, where fragment j + A is the next stage's first: there
+// every wave has read this stage's places, which the loads of the stage after
+// next refill, and the next stage's loads, issued a stage ago, have landed.
 // Row r's 16-byte chunk c sits at position c ^ ((r >> 1) & 7), which spreads
 // the 16 rows of a fragment read over the bank groups; the loads put it there
-// by fetching the chunk that belongs at their landing position.  Fragment j
-// takes activation rows j, FJ + j, 2 FJ + j, ..: a lane's FJ rows are
-// neighbours, and their scales one run.
+// by fetching the chunk that belongs at their landing position.  They also
+// order the rows: fragment j of a wave takes its rows j, FJ + j, 2 FJ + j, ..,
+// so a lane's FJ rows are neighbours and their scales one run; of two weight
+// fragments 2 p and 2 p + 1 a lane's results are 8 consecutive columns.
 //
-// A stage walks the activation fragments j.  The results of the step before
-// join the sums (one multiply-add each) while the matrix unit works.
-//
-// Persistent: the loads run R - 1 stages ahead of the products, over the end of
-// a tile into the next one, whose first stages land while this one's results
-// are stored.
-template <int BM, int FI, int NW, int R, int FB>
+// Persistent: the loads run ahead over the end of a tile into the next one,
+// whose first stages land while this one's results are stored.
+template <int WM, int WN, int FJ, int FI, int FB, int NS>
 __device__ __forceinline__ void
 fp8_tiles(const Fp8Batch& B, char* lds)
 {
-  using L = Fp8Lds<BM, FI, NW, R>;
-  constexpr int BN = 16 * FI * NW, FJ = BM / 16, WS = L::WS;
-  constexpr int kStage = BM * 128;
-  constexpr int kBlocks = BM / 8;                    // 1 KiB loads per stage
-  constexpr int LB = (kBlocks + NW - 1) / NW;        // per wave
-  constexpr int kA = LB + 1, kW = 2 * FI;            // a wave's loads per stage
-  static_assert(R >= 3 && L::kRowScales / 64 < NW, "a wave for the columns' scales");
+  using L = Fp8Tile<WM, WN, FJ, FI, NS>;
+  constexpr int BM = L::BM, BN = L::BN, NW = L::kWaves;
+  constexpr int kStageA = BM * 128, kStageW = BN * 128;
+  constexpr int LA = BM / 8 / NW, LW = BN / 8 / NW;  // a wave's loads per stage
+  constexpr int kOps = LA + LW + 1;
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NW % 2 == 0, "even shares of loads");
+  static_assert(L::kRowScales / 64 < NW && FI % 2 == 0, "a wave for the columns' scales");
   float* const scales = reinterpret_cast<float*>(lds);
 
   const int K = B.K, nb = (K + 127) / 128, sa_pitch = B.sa_pitch;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lh = lane >> 4;
-  const int wcol = wave * 16 * FI;                   // the wave's columns of a tile
+  const int wm = wave % WM, wn = wave / WM;
 
   // Items go in rounds of gridDim.x; workgroups b, b + 8, .. run on XCD b % 8,
   // and of each round every XCD takes a contiguous run.
@@ -490,7 +492,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   };
 
   // ---- loads ---------------------------------------------------------------
-  // What the loads of the stage R - 1 ahead need, stepped along with the stages;
+  // What the loads of the stage two ahead need, stepped along with the stages;
   // past the last item they fetch its last block again, for nobody.
   struct {
     __amdgpu_buffer_rsrc_t a, w;
@@ -522,42 +524,33 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     ld.left = uniform(t.nst);
     ld.last = uniform(t.kbeg == nb - 1 ? -1 : 0);
   };
-  // a load's lane l fills chunk position l % 8 of row l / 8 of its 8 rows
-  // activations: wave w fills blocks w, w + NW, .. of the stage (the same one
-  // twice where there are fewer blocks than waves); LDS row 16 j + i is row i FJ + j
-  const int blk = wave % kBlocks;
-  int aoff[LB];
-  const int prow = 8 * blk + (lane >> 3);
-  const int chunk = (lane & 7) ^ ((prow >> 1) & 7);
-#pragma unroll
-  for (int b = 0; b < LB; ++b) {
-    const int p = prow + 8 * NW * b;
-    aoff[b] = (p % 16 * FJ + p / 16) * K + (chunk << 4);
-  }
-  const int atail = (nb - 1) * 128 + (chunk << 4) < K ? 0 : kOobOffset;
-  // weights: blocks of 8 rows; the chunk depends on the block's parity
-  const int wrow = lane >> 3;
-  const int wchunk[2] = {(lane & 7) ^ (wrow >> 1), (lane & 7) ^ (4 + (wrow >> 1))};
-  int woff[2], wtail[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    woff[h] = (wcol + 8 * h + wrow) * K + (wchunk[h] << 4);
-    wtail[h] = (nb - 1) * 128 + (wchunk[h] << 4) < K ? 0 : kOobOffset;
-  }
+  // A load's lane l fills chunk position l % 8 of row l / 8 of its 8 LDS rows.
+  // Wave w fills blocks w, w + NW, .. of 8 rows, all of one parity (a half of
+  // 16), so its lanes' chunk is one.
+  const int half = (wave & 1) * 8 + (lane >> 3);     // the row of its 16
+  const int chunk = (lane & 7) ^ (half >> 1);
+  const int tail = (nb - 1) * 128 + (chunk << 4) < K ? 0 : kOobOffset;
+  // .. and of its rows the part that differs from lane to lane
+  const int alane = half * FJ * K + (chunk << 4);
+  const int wlane = ((half >> 2) * 8 + (half & 3)) * K + (chunk << 4);
+  const int w2 = uniform(wave >> 1);
   // scales: a lane each; the columns' are nb apart
   constexpr int kColBlocks = (BN + 127) / 128;
   const int soff = row_wave ? lane * 4 : lane < kColBlocks ? lane * nb * 4 : kOobOffset;
-  char* const mine = lds + L::kWeight + wave * (WS * FI * 2048);
   auto dma16 = [](const __amdgpu_buffer_rsrc_t& r, char* to, int v, int s) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
         r, (__attribute__((address_space(3))) void*)to, 16, v, s, 0, 0);
   };
-  // Instruction op of the kA of a stage's activations (the last its scales),
-  // and of the kW of its weights.
-  auto load_a = [&](int slot, int op) {
-    if (op < LB) {
-      dma16(ld.a, lds + L::kAct + slot * kStage + (blk + NW * op) * 1024,
-            aoff[op] | (atail & ld.last), ld.ko);
+  // Load op of a stage's kOps, to place `slot`: its weights, activations, scales.
+  auto load = [&](int slot, int op) {
+    if (op < LW) {
+      const int f = w2 + NW / 2 * op;                // of the tile's fragments
+      dma16(ld.w, lds + L::kWeight + slot * kStageW + (wave + NW * op) * 1024,
+            (wlane | (tail & ld.last)) + ((f >> 1) * 32 + (f & 1) * 4) * K, ld.ko);
+    } else if (op < LW + LA) {
+      const int o = op - LW, f = w2 + NW / 2 * o;
+      dma16(ld.a, lds + L::kAct + slot * kStageA + (wave + NW * o) * 1024,
+            (alane | (tail & ld.last)) + (f / FJ * (16 * FJ) + f % FJ) * K, ld.ko);
     } else {
       const int g = row_wave ? wave * 64 : L::kRowScales;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -565,10 +558,6 @@ fp8_tiles(const Fp8Batch& B, char* lds)
           (__attribute__((address_space(3))) void*)(scales + slot * L::kScales + g), 4, soff, 0,
           0, 0);
     }
-  };
-  auto load_w = [&](int slot, int op) {
-    dma16(ld.w, mine + slot * (FI * 2048) + op * 1024,
-          (woff[op & 1] + (op >> 1) * 16 * K) | (wtail[op & 1] & ld.last), ld.ko);
   };
   auto advance = [&] {
     if (ld.left > 1) {
@@ -594,22 +583,36 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
   };
   auto read_a = [&](int slot, int j) {
-    return read_frag(lds + L::kAct + slot * kStage + j * 2048);
+    return read_frag(lds + L::kAct + wm * (FJ * 2048) + slot * kStageA + j * 2048);
   };
-  constexpr int SV = FJ < 4 ? FJ : 4;                // row scales read at a time
+  auto read_w = [&](int slot, int i) {
+    return read_frag(lds + L::kWeight + wn * (FI * 2048) + slot * kStageW + i * 2048);
+  };
+  constexpr int SV = FJ % 4 == 0 ? 4 : 2;            // row scales read at a time
   typedef float sv_t __attribute__((ext_vector_type(SV)));
-  auto read_s = [&](int slot, int j) {
-    return *reinterpret_cast<const sv_t*>(scales + slot * L::kScales + lr * FJ + j);
-  };
-  auto read_w = [&](int slot) { return scales[slot * L::kScales + L::kRowScales + wcol / 128]; };
 
-  constexpr int FH = FI < 2 ? 1 : 2, HS = FI / FH;   // products per step, steps per fragment
+  constexpr int A = FB - 1;                          // fragments read ahead
+  constexpr int FH = 2, HS = FI / FH;                // products per step, steps per fragment
+  constexpr int kSteps = FJ * HS;
+  constexpr int JB = FJ - A;                         // the barrier's fragment
+  static_assert(FJ % FB == 0 && kSteps % 2 == 0, "the fragment buffers come round with a stage");
+  // A stage's loads begin behind the barrier, few a step (a wave waits to issue
+  // one while others' go out), the last of them in the next stage's first steps:
+  // over all of a stage's time, but with two places only over two thirds, as
+  // the next barrier but one waits for them.
+  constexpr int kSpan = NS > 2 ? kSteps : 2 * kSteps / 3;
+  auto step_of = [](int op) { return (JB * HS + op * kSpan / kOps) % kSteps; };
+  constexpr int kEarly =
+      std::min(kOps, ((kSteps - JB * HS) * kOps + kSpan - 1) / kSpan);   // before its end
+  static_assert((NS - 2) * kOps + kEarly < 64, "the counter has 6 bits");
   f32x4_t acc[FI][FJ], d[2][FH];
-  i32x8_t fa[2][FI], fb[FB];
-  // row scales of two groups of SV fragments, the columns' scale of this stage
-  // and the next, and the scale that the last step's results wait for
-  sv_t sv[2];
-  float w, wnext, pending;
+  // Weight fragments of this stage and the next; where registers are short, the
+  // next one's take the places of this one's as its last products leave them.
+  constexpr bool kAhead = FJ * FI <= 16;
+  i32x8_t fa[kAhead ? 2 : 1][FI], fb[FB];
+  float sc[FJ];                                      // the stage's scales, rows' times columns'
+  sv_t sv[FJ / SV];                                  // the next stage's, apart
+  float w, pending;                                  // .. and the one the last results wait for
   auto clear = [&] {
 #pragma unroll
     for (int i = 0; i < FI; ++i) {
@@ -617,31 +620,26 @@ fp8_tiles(const Fp8Batch& B, char* lds)
       for (int j = 0; j < FJ; ++j) { acc[i][j] = f32x4_t{}; }
     }
 #pragma unroll
-    for (int i = 0; i < FH; ++i) { d[0][i] = d[1][i] = f32x4_t{}; }
+    for (int i = 0; i < FH; ++i) { d[1][i] = f32x4_t{}; }
     pending = 0.0f;
   };
-  auto add = [&](int jp, int hp, int par, float sc) {
+  auto add = [&](int j, int h, int par, float s) {
 #pragma unroll
     for (int i = 0; i < FH; ++i) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        acc[hp * FH + i][jp][e] = fmaf(d[par][i][e], sc, acc[hp * FH + i][jp][e]);
+        acc[h * FH + i][j][e] = fmaf(d[par][i][e], s, acc[h * FH + i][j][e]);
       }
     }
   };
-  constexpr int kSvs = FJ / SV;                      // scale reads per stage
-  // Where in a stage: its activation loads before fragment JR, there the next
-  // stage's weights are read, and from JW on their place is refilled.
-  constexpr int JR = FJ >= 12 ? 6 : FJ >= 8 ? 3 : FJ >= 4 ? 1 : 0;
-  constexpr int JW = FJ >= 12 ? 9 : FJ >= 8 ? 6 : FJ - 1;
-  constexpr int kAPerJ = JR > 0 ? (kA + JR - 1) / JR : kA;
-  constexpr int kWPerJ = (kW + FJ - JW - 1) / (FJ - JW);
-  // Loads that may be in flight behind the awaited ones (a stage issues its
-  // kA, then its kW, and so do the first stages' loads below), and a tile's
-  // stores between.
-  constexpr int kStores = FI * FJ;
-  constexpr int kWaitA = (R - 3) * (kA + kW) + kW, kWaitW = (WS - 1) * (kA + kW) + kA;
-  static_assert(kWaitW + kStores < 64 && kWaitA + kStores < 64, "the counter has 6 bits");
+  auto read_scales = [&](int slot) {
+    const float* const at = scales + slot * L::kScales;
+#pragma unroll
+    for (int g = 0; g < FJ / SV; ++g) {
+      sv[g] = *reinterpret_cast<const sv_t*>(at + wm * (16 * FJ) + lr * FJ + g * SV);
+    }
+    w = at[L::kRowScales + wn * (16 * FI) / 128];
+  };
   // The sums so far stay where they are computed: nothing of a stage moves past
   // a branch, where it would hold its operands' registers.
   auto settle = [&] {
@@ -651,63 +649,48 @@ fp8_tiles(const Fp8Batch& B, char* lds)
       for (int j = 0; j < FJ; ++j) { asm volatile("" : "+v"(acc[i][j])); }
     }
   };
-  // One stage: par its parity, slot its activations' place, next the next
-  // stage's, ahead the last one's, ws where the next stage's weights are;
-  // stored: a tile's results were stored just before.
-  auto stage = [&](auto par_c, bool stored, int slot, int next, int ahead, int ws) {
-    constexpr int par = decltype(par_c)::value;
-    constexpr int f = 0, g = par * kSvs;               // (a stage's fragments come round)
-    // the next stage's activations have landed in every wave, and every wave
-    // has read the last stage's
-    if (par == 0 && stored) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitA + kStores) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitA) : "memory");
-    }
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    w = wnext;
+  // One stage, its operands in place `cur`, the next one's in `next`, the last
+  // one's in `prev`.
+  auto stage = [&](auto par_c, int prev, int cur, int next) {
+    constexpr int par = kAhead ? decltype(par_c)::value : 0;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) { sc[j] = sv[j / SV][j % SV] * w; }
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
-      // the scale of fragment j - 1
-      const float before = j == 0 ? pending : sv[(g + (j - 1) / SV) & 1][(j - 1) % SV] * w;
-#pragma unroll
-      for (int o = j * kAPerJ; o < (j + 1) * kAPerJ && o < kA; ++o) { load_a(ahead, o); }
-      if (j == JR) {
-        if (par == 0) {
-          settle();
-          if (stored) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW + kStores) : "memory");
-          } else {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW) : "memory");
-          }
-        } else {
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kWaitW) : "memory");
-        }
+      if (j == JB) {
+        settle();
+        advance();
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * kOps) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      fb[(j + A) % FB] = j + A < FJ ? read_a(cur, j + A) : read_a(next, j + A - FJ);
+      if (j == (JB + 1 < FJ ? JB + 1 : JB)) { read_scales(next); }
+      if (kAhead && j >= JB) {
 #pragma unroll
         for (int i = 0; i < FI; ++i) {
-          fa[par ^ 1][i] = read_frag(mine + ws * (FI * 2048) + i * 2048);
+          if (JB + i * A / FI == j) { fa[par ^ kAhead][i] = read_w(next, i); }
         }
       }
-      // the next group's scales, and the next stage's columns', two steps ahead
-      if (j % SV == (SV > 2 ? SV - 2 : 0)) {
-        const int to = j / SV + 1;
-        sv[(g + to) & 1] = to < kSvs ? read_s(slot, to * SV) : read_s(next, 0);
-      }
-      if (j == (FJ > 2 ? FJ - 2 : 0)) { wnext = read_w(next); }
-      constexpr int A = FB - 1;                      // fragments read ahead
-      fb[(f + j + A) % FB] = j + A < FJ ? read_a(slot, j + A) : read_a(next, j + A - FJ);
 #pragma unroll
       for (int h = 0; h < HS; ++h) {
-        const int now = ((f + j) * HS + h) & 1, other = now ^ 1;
+        const int step = j * HS + h, now = step & 1, before = now ^ 1;
 #pragma unroll
         for (int i = 0; i < FH; ++i) {
-          d[now][i] = mfma_block(fa[par][h * FH + i], fb[(f + j) % FB]);
+          d[now][i] = mfma_block(fa[par][h * FH + i], fb[j % FB]);
         }
-        if (h == 0) {
-          add((j + FJ - 1) % FJ, HS - 1, other, before);
+        if (step == 0) {
+          add(FJ - 1, HS - 1, before, pending);
         } else {
-          add(j, h - 1, other, sv[(g + j / SV) & 1][j % SV] * w);
+          add(h > 0 ? j : j - 1, h > 0 ? h - 1 : HS - 1, before, sc[h > 0 ? j : j - 1]);
+        }
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) {
+          if (step_of(o) == step) { load(o < kEarly ? cur : prev, o); }
+        }
+        if (!kAhead && j == FJ - 1) {
+#pragma unroll
+          for (int i = 0; i < FH; ++i) { fa[0][h * FH + i] = read_w(next, h * FH + i); }
         }
 #pragma unroll
         for (int i = 0; i < FH; ++i) {
@@ -715,25 +698,11 @@ fp8_tiles(const Fp8Batch& B, char* lds)
           if (i == 0 && h == 0) { __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); }  // reads
           __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);        // the sums
         }
-        if (h + 1 < HS) { __builtin_amdgcn_sched_barrier(0); }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (j >= JW) {
-        if (j == JW) {
-          __builtin_amdgcn_sched_barrier(0);
-          // the next weights are in registers: their place is free
-#pragma unroll
-          for (int i = 0; i < FI; ++i) { asm volatile("" : "+v"(fa[par ^ 1][i])); }
-        }
-#pragma unroll
-        for (int o = (j - JW) * kWPerJ; o < (j - JW + 1) * kWPerJ && o < kW; ++o) {
-          load_w(ws, o);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
     }
-    pending = sv[(g + kSvs - 1) & 1][SV - 1] * w;
+    pending = sc[FJ - 1];
     settle();
-    advance();
   };
 
   // ---- the first item's first stages -------------------------------------------
@@ -741,95 +710,77 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   if (it < 0) { return; }
   ld.round = 0;
   load_item(it);
-  // the loads' order is a stage's: activations, then the next stage's weights,
-  // the first stage's before all
 #pragma unroll
-  for (int o = 0; o < kW; ++o) { load_w(0, o); }
-  __builtin_amdgcn_sched_barrier(0);
+  for (int r = 0; r < NS; ++r) {
 #pragma unroll
-  for (int r = 0; r < R - 1; ++r) {
-#pragma unroll
-    for (int o = 0; o < kA; ++o) { load_a(r, o); }
+    for (int o = 0; o < (r < NS - 1 ? kOps : kEarly); ++o) { load(r, o); }
+    if (r < NS - 1) { advance(); }
     __builtin_amdgcn_sched_barrier(0);
-    if (r > 0 && r < WS) {
-#pragma unroll
-      for (int o = 0; o < kW; ++o) { load_w(r, o); }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (r < R - 2) { advance(); }
   }
-  // stage 0 has landed
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R - 2) * kA + (WS - 1) * kW) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * kOps + kEarly) : "memory");   // stage 0's
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < FI; ++i) { fa[0][i] = read_frag(mine + i * 2048); }
+  for (int i = 0; i < FI; ++i) { fa[0][i] = read_w(0, i); }
 #pragma unroll
-  for (int a = 0; a < FB - 1; ++a) { fb[a] = read_a(0, a); }
-  sv[0] = read_s(0, 0);
-  wnext = read_w(0);
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int i = 0; i < FI; ++i) { asm volatile("" : "+v"(fa[0][i])); }
-#pragma unroll
-  for (int o = 0; o < kW; ++o) { load_w(0, o); }
-  __builtin_amdgcn_sched_barrier(0);
-  advance();
-  static_assert(FJ % FB == 0 && FJ * HS % 2 == 0, "the fragment buffers come round with a stage");
+  for (int j = 0; j < A; ++j) { fb[j] = read_a(0, j); }
+  read_scales(0);
 
-  int cur = 0, next = 1, behind = R - 1, ws = WS > 1 ? 1 : 0, round = 0;
+  int prev = NS - 1, cur = 0, next = 1, round = 0;
   using std::integral_constant;
-  auto step = [&](auto par_c, bool stored) {
-    stage(par_c, stored, cur, next, behind, ws);
-    behind = cur;
+  auto step = [&](auto par_c) {
+    stage(par_c, prev, cur, next);
+    prev = cur;
     cur = next;
-    next = next + 1 == R ? 0 : next + 1;
-    ws = ws + 1 == WS ? 0 : ws + 1;
+    next = next + 1 == NS ? 0 : next + 1;
   };
   clear();
   for (;;) {
     const Fp8Work t = fp8_work<BM, BN>(B, nb, it);
     const Fp8Problem& P = B.p[t.prob];
-    for (int k = 0; k + 1 < t.nst; k += 2) {
-      step(integral_constant<int, 0>{}, k == 0 && round > 0);
-      step(integral_constant<int, 1>{}, false);
+    int k = 0;
+    if constexpr (kAhead) {
+      for (; k + 1 < t.nst; k += 2) {
+        step(integral_constant<int, 0>{});
+        step(integral_constant<int, 1>{});
+      }
     }
-    if (t.nst & 1) {
-      step(integral_constant<int, 0>{}, t.nst == 1 && round > 0);
-      // the next stage is an even one again
+    for (; k < t.nst; ++k) {
+      step(integral_constant<int, 0>{});
+      if constexpr (kAhead) {
 #pragma unroll
-      for (int i = 0; i < FI; ++i) { fa[0][i] = fa[1][i]; }
-      if constexpr (kSvs % 2 == 1) { sv[0] = sv[1]; }
+        for (int i = 0; i < FI; ++i) { fa[0][i] = fa[1][i]; }
+      }
     }
     add(FJ - 1, HS - 1, 1, pending);
 
-    // ---- results: kStores stores whatever the tile's edges, which drop some ------
-    const int rows = min(BM, P.rows - t.row0);
-    const int n0 = t.col0 + wcol + lh * 4;
+    // ---- results -----------------------------------------------------------------
+    const int rows = min(BM, P.rows - t.row0), r0 = wm * (16 * FJ) + lr * FJ;
     if (t.is_split) {
+      // as they lie, 1 KiB each
       const __amdgpu_buffer_rsrc_t to = make_rsrc(
-          B.ws + (size_t)((t.tile - B.split_begin) * B.split + t.share) * (BM * BN), rows * BN * 4);
+          B.ws + (size_t)((t.tile - B.split_begin) * B.split + t.share) * (BM * BN), BM * BN * 4);
 #pragma unroll
       for (int j = 0; j < FJ; ++j) {
+        const int at = r0 + j < rows ? lane * 16 : kOobOffset;
 #pragma unroll
         for (int i = 0; i < FI; ++i) {
-          __builtin_amdgcn_raw_buffer_store_b128(
-              __builtin_bit_cast(u32x4_t, acc[i][j]), to,
-              ((lr * FJ + j) * BN + wcol + i * 16 + lh * 4) * 4, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[i][j]), to, at,
+                                                 ((wave * FJ + j) * FI + i) * 1024, 0);
         }
       }
     } else {
-      const __amdgpu_buffer_rsrc_t to =
-          make_rsrc(P.y + (size_t)t.row0 * P.n, rows * P.n * 2);
+      const __amdgpu_buffer_rsrc_t to = make_rsrc(P.y + (size_t)t.row0 * P.n, rows * P.n * 2);
 #pragma unroll
-      for (int j = 0; j < FJ; ++j) {
+      for (int p = 0; p < FI / 2; ++p) {
+        const int n = t.col0 + wn * (16 * FI) + p * 32 + lh * 8;
 #pragma unroll
-        for (int i = 0; i < FI; ++i) {
-          const int n = n0 + i * 16;
-          __builtin_amdgcn_raw_buffer_store_b64(
-              u32x2_t{pack_bf16x2(acc[i][j][0], acc[i][j][1]),
-                      pack_bf16x2(acc[i][j][2], acc[i][j][3])},
-              to, n < P.n ? ((lr * FJ + j) * P.n + n) * 2 : kOobOffset, 0, 0);
+        for (int j = 0; j < FJ; ++j) {
+          const f32x4_t &u = acc[2 * p][j], &v = acc[2 * p + 1][j];
+          __builtin_amdgcn_raw_buffer_store_b128(
+              u32x4_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
+                      pack_bf16x2(v[2], v[3])},
+              to, n < P.n ? ((r0 + j) * P.n + n) * 2 : kOobOffset, 0, 0);
         }
       }
     }
@@ -841,12 +792,17 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-template <int BM, int FI, int NW, int R, int FB>
-__global__ __launch_bounds__(64 * NW, 2) void
+// (a tile's workgroups on a compute unit, and so its waves per SIMD, are what its
+// LDS leaves room for)
+template <int WM, int WN, int FJ, int FI, int NS>
+constexpr int kTileWaves = Fp8Tile<WM, WN, FJ, FI, NS>::kPerCu * WM * WN / 4;
+
+template <int WM, int WN, int FJ, int FI, int FB, int NS>
+__global__ __launch_bounds__(64 * WM * WN, (kTileWaves<WM, WN, FJ, FI, NS>)) void
 fp8_tile_kernel(const Fp8Batch B)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[Fp8Lds<BM, FI, NW, R>::kBytes];
-  fp8_tiles<BM, FI, NW, R, FB>(B, lds);
+  __shared__ __attribute__((aligned(1024))) char lds[Fp8Tile<WM, WN, FJ, FI, NS>::kBytes];
+  fp8_tiles<WM, WN, FJ, FI, FB, NS>(B, lds);
 }
 
 // ---- few rows: the weights' stream ---------------------------------------------
@@ -1000,40 +956,48 @@ fp8_narrow_kernel(const Fp8Batch B)
   }
 }
 
-// The shares of split tiles: one workgroup per 8 rows of a tile.
-template <int BM, int BN>
+// The shares of split tiles, added in their order: 256 threads take 8 results
+// each, which lie as the tiles' lanes held them.
+template <int WM, int WN, int FJ, int FI>
 __global__ __launch_bounds__(256) void
 fp8_reduce_kernel(const Fp8Batch B)
 {
-  const int tile = B.split_begin + blockIdx.x / (BM / 8);
+  constexpr int BM = 16 * WM * FJ, BN = 16 * WN * FI, kPer = BM * BN / 2048;
+  const int tile = B.split_begin + blockIdx.x / kPer;
   const int nb = (B.K + 127) / 128;
   const Fp8Work t = fp8_work<BM, BN>(B, nb, B.split_begin + (tile - B.split_begin) * B.split);
   const Fp8Problem& P = B.p[t.prob];
-  const float* const ws = B.ws + (size_t)(tile - B.split_begin) * B.split * (BM * BN);
-  for (int c = threadIdx.x; c < 8 * BN / 4; c += 256) {
-    const int m = blockIdx.x % (BM / 8) * 8 + c / (BN / 4), n = c % (BN / 4) * 4;
-    if (t.row0 + m >= P.rows || t.col0 + n >= P.n) { continue; }
-    f32x4_t v = *reinterpret_cast<const f32x4_t*>(ws + m * BN + n);
-    for (int q = 1; q < B.split; ++q) {
-      v += *reinterpret_cast<const f32x4_t*>(ws + (size_t)q * (BM * BN) + m * BN + n);
-    }
-    *reinterpret_cast<u32x2_t*>(P.y + (size_t)(t.row0 + m) * P.n + t.col0 + n) =
-        u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  const int lane = threadIdx.x & 63, lr = lane & 15, lh = lane >> 4;
+  // wave, fragment and pair of weight fragments
+  const int c = blockIdx.x % kPer * 4 + (threadIdx.x >> 6);
+  const int p = c % (FI / 2), j = c / (FI / 2) % FJ, wave = c / (FI / 2 * FJ);
+  const int m = t.row0 + wave % WM * (16 * FJ) + lr * FJ + j;
+  const int n = t.col0 + wave / WM * (16 * FI) + p * 32 + lh * 8;
+  if (m >= P.rows || n >= P.n) { return; }
+  const float* at = B.ws + (size_t)(tile - B.split_begin) * B.split * (BM * BN) + c * 512 + lane * 4;
+  f32x4_t u = *reinterpret_cast<const f32x4_t*>(at);
+  f32x4_t v = *reinterpret_cast<const f32x4_t*>(at + 256);
+  for (int q = 1; q < B.split; ++q) {
+    at += BM * BN;
+    u += *reinterpret_cast<const f32x4_t*>(at);
+    v += *reinterpret_cast<const f32x4_t*>(at + 256);
   }
+  *reinterpret_cast<u32x4_t*>(P.y + (size_t)m * P.n + n) =
+      u32x4_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
+              pack_bf16x2(v[2], v[3])};
 }
 
-template <int BM, int FI, int NW, int R, int FB>
+template <int WM, int WN, int FJ, int FI, int FB, int NS>
 hipError_t
 tile_launch(const Fp8Batch& b, hipStream_t s)
 {
+  using L = Fp8Tile<WM, WN, FJ, FI, NS>;
   const int tail = b.total_tiles - b.split_begin;
   const int items = b.split_begin + tail * b.split;
-  // as many workgroups as run at once
-  constexpr int kPerCu = std::min(160 * 1024 / Fp8Lds<BM, FI, NW, R>::kBytes, 8 / NW * 2);
-  fp8_tile_kernel<BM, FI, NW, R, FB>
-      <<<std::min(items, b.cus * std::max(kPerCu, 1)), 64 * NW, 0, s>>>(b);
+  fp8_tile_kernel<WM, WN, FJ, FI, FB, NS>
+      <<<std::min(items, b.cus * L::kPerCu), 64 * L::kWaves, 0, s>>>(b);   // all at once
   if (b.split > 1 && tail > 0) {
-    fp8_reduce_kernel<BM, 16 * FI * NW><<<tail * (BM / 8), 256, 0, s>>>(b);
+    fp8_reduce_kernel<WM, WN, FJ, FI><<<tail * (L::BM * L::BN / 2048), 256, 0, s>>>(b);
   }
   return hipGetLastError();
 }
@@ -1058,13 +1022,14 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 
 }  // namespace
 
-// The tile builds: X(BM, FI, NW, R, FB).
+// The tile builds: X(WM, WN, FJ, FI, FB, NS).
 #define U15H_FP8_TILES(X) \
-  X(256, 2, 8, 3, 4)      \
-  X(192, 2, 8, 3, 4)      \
-  X(128, 2, 8, 4, 4)      \
-  X(128, 2, 4, 3, 4)      \
-  X(64, 2, 4, 4, 4)
+  X(2, 4, 8, 4, 4, 2)     \
+  X(2, 4, 6, 4, 3, 2)     \
+  X(2, 4, 4, 4, 4, 3)     \
+  X(2, 4, 4, 2, 4, 4)     \
+  X(2, 2, 4, 4, 4, 2)     \
+  X(1, 4, 4, 2, 4, 3)
 
 #define U15H_FP8_NARROW(X) \
   X(1, 1, 4, 4)            \
@@ -1093,8 +1058,10 @@ launch_fp8_gemm(const Fp8Batch& b, hipStream_t s)
   }
   U15H_FP8_NARROW(U15H_CASE)
 #undef U15H_CASE
-#define U15H_CASE(BM, FI, NW, R, FB)                                  \
-  if (!b.narrow && b.bm == BM && b.bn == 16 * FI * NW && b.waves == NW) { return tile_launch<BM, FI, NW, R, FB>(b, s); }
+#define U15H_CASE(WM, WN, FJ, FI, FB, NS)                                                     \
+  if (!b.narrow && b.bm == 16 * WM * FJ && b.bn == 16 * WN * FI && b.waves == WM * WN) {  \
+    return tile_launch<WM, WN, FJ, FI, FB, NS>(b, s);                                         \
+  }
   U15H_FP8_TILES(U15H_CASE)
 #undef U15H_CASE
   return hipErrorInvalidValue;
@@ -1154,9 +1121,9 @@ fp8_kernels_loadable()
 #define U15H_FN(MT, FI, NW, D) reinterpret_cast<const void*>(&fp8_narrow_kernel<MT, FI, NW, D>),
       U15H_FP8_NARROW(U15H_FN)
 #undef U15H_FN
-#define U15H_FN(BM, FI, NW, R, FB)                                                    \
-  reinterpret_cast<const void*>(&fp8_tile_kernel<BM, FI, NW, R, FB>),                 \
-      reinterpret_cast<const void*>(&fp8_reduce_kernel<BM, 16 * FI * NW>),
+#define U15H_FN(WM, WN, FJ, FI, FB, NS)                                       \
+  reinterpret_cast<const void*>(&fp8_tile_kernel<WM, WN, FJ, FI, FB, NS>),     \
+      reinterpret_cast<const void*>(&fp8_reduce_kernel<WM, WN, FJ, FI>),
       U15H_FP8_TILES(U15H_FN)
 #undef U15H_FN
   };
