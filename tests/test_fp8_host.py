@@ -1,0 +1,129 @@
+"""The fp8 tier's checks and plans on the host: the entry points' own source
+with the launchers replaced by ones that print what they are asked for and
+refuse what the kernels would (tests/fp8_host.cc)."""
+import pathlib
+import random
+import re
+import shutil
+import subprocess
+
+import pytest
+
+REPO = pathlib.Path(__file__).resolve().parent.parent
+CSRC = REPO / "vpipe-sensenova-u1.5_amd" / "csrc"
+ROCM_INCLUDE = pathlib.Path("/opt/rocm/include")
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    if shutil.which("g++") is None or not ROCM_INCLUDE.exists():
+        pytest.skip("g++ or the HIP headers not available")
+    exe = tmp_path_factory.mktemp("fp8") / "fp8_host"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-D__HIP_PLATFORM_AMD__",
+                    f"-I{ROCM_INCLUDE}", f"-I{REPO / 'include'}", f"-I{CSRC}",
+                    str(REPO / "tests" / "fp8_host.cc"), "-o", str(exe)], check=True, timeout=300)
+
+    def run(calls, cus=256):
+        out = subprocess.run([str(exe), str(cus)], input="\n".join(calls) + "\n",
+                             capture_output=True, text=True, check=True, timeout=300).stdout
+        lines = out.splitlines()
+        assert len(lines) == len(calls)
+        return [tuple(line.split(" ; ", 1)) for line in lines]
+    return run
+
+
+def kernel_builds():
+    """(bm, bn, waves) of every product kernel, narrow and tiled, as built."""
+    text = (CSRC / "u15h_fp8.hip").read_text()
+
+    def rows(macro):
+        block = re.search(rf"#define {macro}\(X\)((?:.*\\\n)*.*)", text).group(1)
+        return [tuple(map(int, r.split(","))) for r in re.findall(r"X\(([\d, ]+)\)", block)]
+    narrow = {("narrow", 16 * mt, 16 * fi, nw) for mt, fi, nw, _ in rows("U15H_FP8_NARROW")}
+    tiles = {("tiles", 16 * wm * fj, 16 * wn * fi, wm * wn)
+             for wm, wn, fj, fi, *_ in rows("U15H_FP8_TILES")}
+    return narrow | tiles
+
+
+def parsed(launch):
+    m = re.match(r"(narrow|tiles) (\d+)x(\d+)x(\d+) n=(\d+) tail=(\d+) shares=(\d+)", launch)
+    return (m.group(1), *map(int, m.groups()[1:4])), *map(int, m.groups()[4:])
+
+
+def random_gemms(n):
+    rng = random.Random(7)
+    calls = []
+    for _ in range(n):
+        mu, mg = rng.choice([(1, 0), (0, 1), (1, 1)])
+        mu *= int(2 ** rng.uniform(0, 13))
+        mg *= int(2 ** rng.uniform(0, 13))
+        K = 16 * int(2 ** rng.uniform(0, 10))
+        Ns = [8 * int(2 ** rng.uniform(0, 12)) for _ in range(rng.randint(1, 4))]
+        calls.append(f"gemm {mu} {mg} {K} " + " ".join(map(str, Ns)))
+    return calls
+
+
+def test_every_build_is_reached_and_no_other(host):
+    got = {parsed(launch)[0] for launch, st in host(random_gemms(4000)) if st == "ok"}
+    assert got == kernel_builds()
+
+
+@pytest.mark.parametrize("cus", [256, 208, 64, 1])
+def test_every_product_has_a_plan(host, cus):
+    """The launcher's own conditions and the workspace's size hold for each."""
+    calls = random_gemms(1500)
+    split = 0
+    for call, (launch, st) in zip(calls, host(calls, cus)):
+        assert st == "ok", (call, st)
+        split += parsed(launch)[3] > 1
+    assert split > 50 or cus == 1     # (one unit has no partial round of large tiles)
+
+
+def test_the_largest_sizes(host):
+    big = 1 << 22
+    ok = [f"gemm {big} 0 131072 1048576", f"gemm 0 {big} 16 8", "gemm 1 0 131072 1048576",
+          f"gemm 1 {big - 1} 128 1048576 1048576 8 8", f"rows {big} 131072",
+          f"swiglu {big} 131072 1", f"norm {big} 0 16384 1 1 1", "blocks 1048576 131072"]
+    for call, (launch, st) in zip(ok, host(ok)):
+        assert st == "ok" and launch != "-", (call, st)
+    no = [f"gemm {big} 1 128 8", "gemm 1 0 131088 8", "gemm 1 0 128 1048584",
+          f"gemm 2147483647 2147483647 128 8", f"rows {big + 1} 16", "rows 1 131088",
+          f"swiglu {big + 1} 16 0", f"norm 1 {big} 16 0 0 0", "norm 1 0 16400 0 0 0",
+          "blocks 1048577 16", "blocks 1 131088"]
+    for call, (launch, st) in zip(no, host(no)):
+        assert launch == "-" and st.startswith("refused: "), (call, launch, st)
+
+
+def test_the_larger_group_of_rows_comes_first(host):
+    (launch, st), = host(["gemm 128 4096 4096 12288 12288"])
+    assert st == "ok" and launch.endswith("rows 4096 4096 128 128")
+
+
+def test_no_rows_no_launch(host):
+    calls = ["gemm 0 0 256 8", "rows 0 256", "swiglu 0 256 0", "norm 0 0 256 1 1 0",
+             "blocks 0 256"]
+    assert host(calls) == [("-", "ok")] * len(calls)
+
+
+@pytest.mark.parametrize("call", [
+    "rows 4 0", "rows 4 8", "rows 4 -16", "rows -1 256", "swiglu 4 264 0", "blocks -8 256",
+    "blocks 8 24", "norm 4 0 0 0 0 0", "norm -1 4 256 0 0 0", "gemm 1 0 120 8", "gemm 1 0 0 8",
+    "gemm 1 0 128 4", "gemm 1 0 128 0", "gemm 1 0 128 8 12", "gemm -1 4 128 8", "gemm 4 -1 128 8",
+    "gemm 4 0 128", "gemm 4 0 128 8 8 8 8 8"])
+def test_sizes_refused(host, call):
+    (launch, st), = host([call])
+    assert launch == "-" and st.startswith("refused: ") and len(st) > 12, (launch, st)
+
+
+@pytest.mark.parametrize("which", [
+    "rows.x", "rows.q", "rows.s", "blocks.w", "blocks.q", "swiglu.up", "swiglu.h", "norm.delta",
+    "norm.x_out", "norm.w_gen", "norm.eps", "norm.nan", "norm.y", "gemm.y", "gemm.wq_und",
+    "gemm.sw_gen", "gemm.nproj", "gemm.proj", "gemm.sx", "context"])
+def test_operands_refused(host, which):
+    (launch, st), = host([f"bad {which}"])
+    assert launch == "-" and st.startswith("refused: "), (launch, st)
+
+
+def test_a_group_without_rows_needs_no_weights(host):
+    (launch, st), = host(["bad none.gemm"])
+    assert st == "ok" and launch != "-"

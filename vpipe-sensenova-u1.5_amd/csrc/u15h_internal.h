@@ -296,10 +296,6 @@ struct Fp8Batch {
   int split;
   float* ws;
 };
-inline size_t fp8_split_bytes(const Fp8Batch& b)
-{
-  return (size_t)(b.total_tiles - b.split_begin) * b.split * b.bm * b.bn * 4;
-}
 hipError_t launch_fp8_gemm(const Fp8Batch& b, hipStream_t s);
 // Codes [rows][K] and scales [ceil(K / 128)][rows] of bf16 rows, or with `up`
 // of silu(x) * up, whose bf16 values go to h where that is not null.
