@@ -99,30 +99,30 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
 //           `part` per MB of their sums;
 //   and `weight` per MB of weights.
 // Fitted to 8858 timings (a graph, weights rotated; M 1-4224, K 256-12288, N
-// 512-24576, every kind and 1 to 16 shares), each to 4-9% on the mean; the kind
-// and shares with the least estimate take 1.2% longer than the fastest of all,
-// on the mean over the 338 sizes, and 36% at worst (65 rows, K 8192, N 1024:
-// 16.3 against 12.0 us).
+// 512-24576, every kind and 1 to 16 shares), each to 5-9% on the mean; the kind
+// and shares with the least estimate take 0.9% longer than the fastest of all,
+// on the mean over the 338 sizes, and 16% at worst (1152 rows, K 8192, N 1024:
+// 29.7 against 25.5 us).
 struct Kind {
   bool narrow;
   int bm, bn, waves;
   double fixed, round, stage, stream, split, part, weight;
 };
 constexpr Kind kKinds[] = {
-    {true, 16, 16, 4, 2.56, 0.61, 0.0410, 0.0615, 0, 0, 0},
-    {true, 16, 32, 4, 2.27, 1.13, 0.0513, 0.1562, 0, 0, 0},
-    {true, 32, 16, 4, 1.78, 1.65, 0.0618, 0.0570, 0, 0, 0},
-    {true, 32, 32, 4, 2.41, 1.28, 0.0672, 0.1558, 0, 0, 0},
-    {true, 64, 16, 4, 1.55, 2.09, 0.0843, 0.0802, 0, 0, 0},
-    {true, 64, 32, 4, 3.58, 0.59, 0.0900, 0.1987, 0, 0, 0},
-    {true, 96, 16, 4, 1.46, 2.35, 0.1126, 0.0899, 0, 0, 0},
-    {true, 128, 16, 4, 1.38, 2.83, 0.1445, 0.0962, 0, 0, 0},
-    {false, 64, 128, 4, 4.15, 0.51, 0.330, 0, 3.34, 0.335, 0.119},
-    {false, 128, 128, 4, 4.89, 0, 0.534, 0, 3.48, 0.276, 0.141},
-    {false, 128, 128, 8, 2.71, 2.59, 0.505, 0, 3.41, 0.363, 0.081},
-    {false, 128, 256, 8, 2.60, 3.38, 0.731, 0, 3.59, 0.295, 0.112},
-    {false, 192, 256, 8, 5.39, 1.70, 1.068, 0, 3.46, 0.206, 0.145},
-    {false, 256, 256, 8, 8.10, 0, 1.2818, 0, 4.49, 0.139, 0.128},
+    {true, 16, 16, 4, 2.40, 0.48, 0.0511, 0.0463, 0, 0, 0},
+    {true, 16, 32, 4, 1.92, 1.34, 0.0831, 0.0992, 0, 0, 0},
+    {true, 32, 16, 4, 1.74, 1.43, 0.0696, 0.0466, 0, 0, 0},
+    {true, 32, 32, 4, 2.13, 1.42, 0.1017, 0.0953, 0, 0, 0},
+    {true, 64, 16, 4, 1.42, 1.97, 0.1176, 0.0552, 0, 0, 0},
+    {true, 64, 32, 4, 3.05, 0.90, 0.1480, 0.1202, 0, 0, 0},
+    {true, 96, 16, 4, 1.42, 2.10, 0.1673, 0.0489, 0, 0, 0},
+    {true, 128, 16, 4, 1.42, 2.43, 0.2098, 0.0525, 0, 0, 0},
+    {false, 64, 128, 4, 4.17, 0.17, 0.344, 0, 3.45, 0.355, 0.115},
+    {false, 128, 128, 4, 4.63, 0, 0.563, 0, 3.67, 0.275, 0.138},
+    {false, 128, 128, 8, 2.75, 2.26, 0.518, 0, 3.46, 0.384, 0.080},
+    {false, 128, 256, 8, 2.73, 2.99, 0.765, 0, 3.71, 0.310, 0.104},
+    {false, 192, 256, 8, 5.78, 1.13, 1.097, 0, 3.65, 0.216, 0.141},
+    {false, 256, 256, 8, 7.98, 0, 1.309, 0, 4.81, 0.137, 0.125},
 };
 
 // Workgroups of a kind of tile that run at once.
@@ -179,37 +179,38 @@ plan(Fp8Batch& b, size_t workspace)
     }
   };
   for (const Kind& k : kKinds) {
-    double tiles = 0, valid = 0, padded = 0;
+    if (k.narrow && rows > k.bm) { continue; }
+    long long tiles = 0, valid = 0, padded = 0;
     for (int i = 0; i < b.nprob; ++i) {
-      const double tn = (b.p[i].n + k.bn - 1) / k.bn, tm = (b.p[i].rows + k.bm - 1) / k.bm;
+      const long long tn = (b.p[i].n + k.bn - 1) / k.bn, tm = (b.p[i].rows + k.bm - 1) / k.bm;
       tiles += tm * tn;
       valid += b.p[i].rows * tn;
       padded += tm * k.bm * tn;
     }
     if (k.narrow) {
-      if (rows > k.bm) { continue; }
-      const double load = std::ceil(tiles / C);
-      consider(k, 1, k.fixed + load * (k.round + nb * k.stage) + tiles * nb / C * k.stream);
+      const long long load = (tiles + C - 1) / C;
+      consider(k, 1, k.fixed + load * (k.round + nb * k.stage) + (double)tiles * nb / C * k.stream);
       continue;
     }
     const int slots = slots_of(k, C), two = slots / C;
-    const double full = std::floor(tiles / slots), rem = tiles - full * slots;
+    const long long full = tiles / slots, rem = tiles % slots;
     const double fixed = k.fixed + mb * k.weight + full * (k.round + nb * two * k.stage);
+    if (best != nullptr && fixed >= least) { continue; }
     const double tile_mb = 4e-6 * k.bm * k.bn;
     for (int S = 1; S <= 16; S += S < 4 ? 1 : S < 8 ? 2 : 4) {
-      if (S > 1 && (rem == 0 || S > nb / 2 || rem * S > 2.0 * slots ||
-                    rem * S * tile_mb * 1e6 > workspace)) {
+      if (S > 1 && (rem == 0 || S > nb / 2 || rem * S > 2 * slots ||
+                    (size_t)(rem * S * k.bm * k.bn) * 4 > workspace)) {
         break;
       }
       double us = fixed;
       if (rem > 0) {
         const int nst = (nb + S - 1) / S;
-        const double rounds = std::ceil(rem * S / slots);
+        const long long rounds = (rem * S + slots - 1) / slots;
         // the last of them may have a CU to each workgroup
-        const double last = rem * S - (rounds - 1) * slots > C ? two : 1;
+        const int last = rem * S - (rounds - 1) * slots > C ? two : 1;
         us += rounds * k.round + ((rounds - 1) * two + last) * nst * k.stage;
       }
-      if (S > 1) { us += k.split + rem * S * tile_mb * (valid / padded) * k.part; }
+      if (S > 1) { us += k.split + rem * S * tile_mb * valid / padded * k.part; }
       consider(k, S, us);
     }
   }

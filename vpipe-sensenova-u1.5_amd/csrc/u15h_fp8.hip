@@ -812,6 +812,12 @@ fp8_tile_kernel(const Fp8Batch B)
 // rows, row scales) through D places of its own in LDS by direct loads, so all
 // of D stages are in flight from the start; the weight scales are a register
 // each of 64 blocks, read by lane.
+// Bound by the weights' bytes where rows are few (and by latency where K is
+// short): one row takes 7.1 us with 6144 columns of K 4096, 21.0 us with 24576
+// (4.8 TB/s); 64 rows of 6144 columns 11.7 us.  A model's weights are read once
+// a step and do not fit the caches, so they go past them (non-temporal): loaded
+// plainly these take 8.0, 22.5 and 12.3 us, and only weights that stay in the
+// 256 MB cache from call to call come faster so (5.7, 18.5 and 8.5 us).
 template <int MT, int FI, int NW, int D>
 struct Fp8NarrowLds {
   static constexpr int kSlot = FI * 2048 + MT * 2048 + (MT + 3) / 4 * 256;
@@ -859,9 +865,13 @@ fp8_narrow_kernel(const Fp8Batch B)
     for (int r = 0; r < 2 * (FI + MT); ++r) {
       const int h = r & 1, v = off[h] + ((kt == nb - 1 ? tail[h] : 0) | past);
       const bool weights = r < 2 * FI;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          weights ? rw : ra, (__attribute__((address_space(3))) void*)(to + r * 1024), 16,
-          v + (weights ? r : r - 2 * FI) / 2 * 16 * K, ko, 0, 0);
+      auto* const dst = (__attribute__((address_space(3))) void*)(to + r * 1024);
+      if (weights) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, dst, 16, v + r / 2 * 16 * K, ko, 0,
+                                                 kNonTemporal);
+      } else {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, dst, 16, v + (r - 2 * FI) / 2 * 16 * K, ko, 0, 0);
+      }
     }
     const __amdgpu_buffer_rsrc_t rs = make_rsrc(sa + (size_t)kt * sa_pitch, scale_bytes);
 #pragma unroll
@@ -974,13 +984,25 @@ fp8_reduce_kernel(const Fp8Batch B)
   const int m = t.row0 + wave % WM * (16 * FJ) + lr * FJ + j;
   const int n = t.col0 + wave / WM * (16 * FI) + p * 32 + lh * 8;
   if (m >= P.rows || n >= P.n) { return; }
-  const float* at = B.ws + (size_t)(tile - B.split_begin) * B.split * (BM * BN) + c * 512 + lane * 4;
-  f32x4_t u = *reinterpret_cast<const f32x4_t*>(at);
-  f32x4_t v = *reinterpret_cast<const f32x4_t*>(at + 256);
-  for (int q = 1; q < B.split; ++q) {
-    at += BM * BN;
-    u += *reinterpret_cast<const f32x4_t*>(at);
-    v += *reinterpret_cast<const f32x4_t*>(at + 256);
+  const float* const at =
+      B.ws + (size_t)(tile - B.split_begin) * B.split * (BM * BN) + c * 512 + lane * 4;
+  // four shares' loads at a time; those past the last are its own again, not added
+  f32x4_t u = {}, v = {};
+  for (int q0 = 0; q0 < B.split; q0 += 4) {
+    f32x4_t su[4], sv[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float* const from = at + (size_t)min(q0 + q, B.split - 1) * (BM * BN);
+      su[q] = *reinterpret_cast<const f32x4_t*>(from);
+      sv[q] = *reinterpret_cast<const f32x4_t*>(from + 256);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q0 + q < B.split) {
+        u += su[q];
+        v += sv[q];
+      }
+    }
   }
   *reinterpret_cast<u32x4_t*>(P.y + (size_t)m * P.n + n) =
       u32x4_t{pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3]), pack_bf16x2(v[0], v[1]),
