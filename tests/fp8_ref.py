@@ -117,3 +117,40 @@ def check_codes(q, s, v, rel):
         slack = (2 * rel + 2.0 ** -21) * ideal.abs()
         most = torch.maximum(ideal.abs() * 2.0 ** -4, torch.full_like(ideal, 2.0 ** -10))
         assert bool((off <= most + slack).all()), (b, float((off - most).max()))
+
+
+# Sizes (M_und, M_gen, K, Ns) at which the product takes each of its kernels on
+# 256 compute units: the kernel, whether shares of K are split, and whether the
+# workgroups run more than one round of tiles.
+KINDS = [
+    ((3, 0, 528, (264,)), "narrow 16x16x4", False, False),
+    ((1, 1, 400, (2064,)), "narrow 16x32x4", False, False),
+    ((0, 23, 656, (40, 8)), "narrow 32x16x4", False, False),
+    ((2, 20, 272, (680, 1464)), "narrow 32x32x4", False, False),
+    ((35, 10, 784, (72,)), "narrow 64x16x4", False, False),
+    ((10, 36, 144, (2128,)), "narrow 64x32x4", False, False),
+    ((70, 0, 1040, (136,)), "narrow 96x16x4", False, False),
+    ((98, 5, 400, (136,)), "narrow 128x16x4", False, False),
+    ((0, 132, 144, (200,)), "tiles 64x128x4", False, False),
+    ((132, 5, 144, (8360, 7984)), "tiles 64x128x4", False, True),
+    ((129, 4, 1680, (8,)), "tiles 64x128x4", True, False),
+    ((209, 4, 16, (6688, 14192)), "tiles 128x128x4", False, False),
+    ((648, 9, 16, (11272,)), "tiles 128x128x4", False, True),
+    ((2358, 3176, 7520, (80,)), "tiles 128x128x4", True, False),
+    ((68, 21, 288, (11768,)), "tiles 128x128x8", False, False),
+    ((332, 1, 2336, (16176, 32)), "tiles 128x128x8", False, True),
+    ((7, 106, 3904, (3936,)), "tiles 128x128x8", True, False),
+    ((17, 44, 3936, (16256, 312)), "tiles 128x128x8", True, True),
+    ((18, 321, 288, (256, 15272)), "tiles 128x256x8", False, False),
+    ((866, 1, 592, (14464,)), "tiles 128x256x8", False, True),
+    ((0, 145, 7760, (40, 5344)), "tiles 128x256x8", True, False),
+    ((305, 1, 3264, (16304, 584)), "tiles 128x256x8", True, True),
+    ((3496, 3, 416, (2224, 16)), "tiles 192x256x8", False, False),
+    ((1, 864, 288, (5064, 15584)), "tiles 192x256x8", False, True),
+    ((0, 576, 8080, (6736,)), "tiles 192x256x8", True, False),
+    ((1756, 0, 6096, (752, 5864)), "tiles 192x256x8", True, True),
+    ((3327, 25, 400, (3592, 8)), "tiles 256x256x8", False, False),
+    ((3299, 0, 16, (9848, 9000)), "tiles 256x256x8", False, True),
+    ((0, 392, 6448, (9736,)), "tiles 256x256x8", True, False),
+    ((3540, 0, 1680, (4712,)), "tiles 256x256x8", True, True),
+]

@@ -9,6 +9,8 @@ import subprocess
 
 import pytest
 
+import fp8_ref as ref
+
 REPO = pathlib.Path(__file__).resolve().parent.parent
 CSRC = REPO / "vpipe-sensenova-u1.5_amd" / "csrc"
 ROCM_INCLUDE = pathlib.Path("/opt/rocm/include")
@@ -127,3 +129,18 @@ def test_operands_refused(host, which):
 def test_a_group_without_rows_needs_no_weights(host):
     (launch, st), = host(["bad none.gemm"])
     assert st == "ok" and launch != "-"
+
+
+def test_the_sizes_that_stand_for_the_kernels(host):
+    """Every build, and of the tiles each with and without shares of K and with
+    one round of workgroups and more."""
+    calls = ["gemm {} {} {} ".format(*size[:3]) + " ".join(map(str, size[3]))
+             for size, *_ in ref.KINDS]
+    seen = set()
+    for (size, name, split, rounds), (launch, st) in zip(ref.KINDS, host(calls)):
+        build, tiles, tail, shares = parsed(launch)
+        slots = 512 if build[3] == 4 else 256
+        assert st == "ok" and launch.startswith(name + " "), (size, launch)
+        assert (shares > 1) == split and (name[0] == "n" or (tiles > slots) == rounds), launch
+        seen.add(build)
+    assert seen == kernel_builds()
