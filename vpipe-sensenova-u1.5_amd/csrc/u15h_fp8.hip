@@ -444,13 +444,27 @@ struct Fp8Tile {
 // One stage is one block of K.  Both operands come through LDS by direct loads
 // of 1 KiB (8 rows x 128 bytes: 12 cycles each; loaded to registers in a
 // fragment's layout, 16 rows x 64 bytes, the same bytes take 64).
-// A wave holds a stage's weight fragments and walks its activation fragments
-// j, read A = FB - 1 ahead; the results of the step before join the sums (one
-// multiply-add each) while the matrix unit works.  What bounds the large tiles
-// is the LDS's reads and their power, hence nearly square tiles per wave.
-// One barrier a stage, where fragment j + A is the next stage's first: there
-// every wave has read this stage's places, which the loads of the stage after
-// next refill, and the next stage's loads, issued a stage ago, have landed.
+// A wave holds a stage's weight fragments and walks its activation fragments,
+// read a pair ahead; the results of the step before join the sums (one
+// multiply-add each) while the matrix unit works.
+// One barrier a stage, before the last pair, during which the next stage's
+// first pair is read: there every wave has read this stage's places, which the
+// loads of the stage NS ahead refill, and the next stage's loads have landed.
+//
+// What bounds it: a 256 x 256 stage takes 2900 cycles on a compute unit of which
+// the products need 2048 (58% of all cycles with the rest of a launch); without
+// its loads it takes 2430 (they share the LDS and wait to issue), without its
+// multiply-adds 2700.  With every unit busy the clock falls to 1.6 to 1.8 GHz,
+// so what costs power costs time: square tiles per wave (128 x 64, two thirds
+// of the LDS reads that 256 x 32 makes) gained 5%.  Products and
+// multiply-adds alone, from registers, reach 3.7 to 4.0 PFLOP/s; 4096 rows of
+// K 12288 and 4096 columns run at 2.35 (175 us), 4224 rows of two times 12288
+// columns at 2.07 (412 us).
+// The smaller tiles have few products a stage to hide its barrier and reads
+// behind, so they have more places (NS) and their weights' fragments a stage
+// ahead: 1024 rows of K 4096 and 4096 columns take 28 us on 128 x 128 tiles of
+// eight waves, 34 on four waves with half the places and 31 on 64 x 128; of
+// 2048 rows it is 51, 44 and 55 us.
 // Row r's 16-byte chunk c sits at position c ^ ((r >> 1) & 7), which spreads
 // the 16 rows of a fragment read over the bank groups; the loads put it there
 // by fetching the chunk that belongs at their landing position.  They also
@@ -591,19 +605,24 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   constexpr int SV = FJ % 4 == 0 ? 4 : 2;            // row scales read at a time
   typedef float sv_t __attribute__((ext_vector_type(SV)));
 
-  constexpr int A = FB - 1;                          // fragments read ahead
-  constexpr int FH = 2, HS = FI / FH;                // products per step, steps per fragment
+  // A step is the products of one activation fragment and FH weight fragments.
+  // Activation fragments go in pairs: both with the first weight fragments, then
+  // both with the next ones, so that a weight fragment's place, refilled behind
+  // the pair's last product of it, is next needed three steps later.
+  constexpr int FH = 2, HS = FI / FH;
   constexpr int kSteps = FJ * HS;
-  constexpr int JB = FJ - A;                         // the barrier's fragment
-  static_assert(FJ % FB == 0 && kSteps % 2 == 0, "the fragment buffers come round with a stage");
+  auto frag_of = [](int step) { return 2 * (step / (2 * HS)) + step % 2; };
+  auto half_of = [](int step) { return step % (2 * HS) / 2; };
+  constexpr int kBarrier = kSteps - 2 * HS;          // the barrier's step: the last pair
+  static_assert(FJ % 2 == 0 && FB >= 4 && FJ % FB == 0, "fragment buffers come round with a stage");
   // A stage's loads begin behind the barrier, few a step (a wave waits to issue
   // one while others' go out), the last of them in the next stage's first steps:
   // over all of a stage's time, but with two places only over two thirds, as
   // the next barrier but one waits for them.
   constexpr int kSpan = NS > 2 ? kSteps : 2 * kSteps / 3;
-  auto step_of = [](int op) { return (JB * HS + op * kSpan / kOps) % kSteps; };
+  auto step_of = [](int op) { return (kBarrier + op * kSpan / kOps) % kSteps; };
   constexpr int kEarly =
-      std::min(kOps, ((kSteps - JB * HS) * kOps + kSpan - 1) / kSpan);   // before its end
+      std::min(kOps, ((kSteps - kBarrier) * kOps + kSpan - 1) / kSpan);   // before its end
   static_assert((NS - 2) * kOps + kEarly < 64, "the counter has 6 bits");
   f32x4_t acc[FI][FJ], d[2][FH];
   // Weight fragments of this stage and the next; where registers are short, the
@@ -656,50 +675,50 @@ fp8_tiles(const Fp8Batch& B, char* lds)
 #pragma unroll
     for (int j = 0; j < FJ; ++j) { sc[j] = sv[j / SV][j % SV] * w; }
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) {
-      if (j == JB) {
+    for (int step = 0; step < kSteps; ++step) {
+      const int j = frag_of(step), h = half_of(step);
+      if (step == kBarrier) {
         settle();
         advance();
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * kOps) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
-      fb[(j + A) % FB] = j + A < FJ ? read_a(cur, j + A) : read_a(next, j + A - FJ);
-      if (j == (JB + 1 < FJ ? JB + 1 : JB)) { read_scales(next); }
-      if (kAhead && j >= JB) {
+      if (h == 0) {
+        fb[(j + 2) % FB] = j + 2 < FJ ? read_a(cur, j + 2) : read_a(next, j + 2 - FJ);
+      }
+      if (step == kBarrier + 1) { read_scales(next); }
+      if (kAhead && step >= kBarrier) {
 #pragma unroll
         for (int i = 0; i < FI; ++i) {
-          if (JB + i * A / FI == j) { fa[par ^ kAhead][i] = read_w(next, i); }
+          if (kBarrier + i * 2 * HS / FI == step) { fa[par ^ kAhead][i] = read_w(next, i); }
         }
       }
+      const int now = step & 1, before = now ^ 1;
 #pragma unroll
-      for (int h = 0; h < HS; ++h) {
-        const int step = j * HS + h, now = step & 1, before = now ^ 1;
-#pragma unroll
-        for (int i = 0; i < FH; ++i) {
-          d[now][i] = mfma_block(fa[par][h * FH + i], fb[j % FB]);
-        }
-        if (step == 0) {
-          add(FJ - 1, HS - 1, before, pending);
-        } else {
-          add(h > 0 ? j : j - 1, h > 0 ? h - 1 : HS - 1, before, sc[h > 0 ? j : j - 1]);
-        }
-#pragma unroll
-        for (int o = 0; o < kOps; ++o) {
-          if (step_of(o) == step) { load(o < kEarly ? cur : prev, o); }
-        }
-        if (!kAhead && j == FJ - 1) {
-#pragma unroll
-          for (int i = 0; i < FH; ++i) { fa[0][h * FH + i] = read_w(next, h * FH + i); }
-        }
-#pragma unroll
-        for (int i = 0; i < FH; ++i) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
-          if (i == 0 && h == 0) { __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); }  // reads
-          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);        // the sums
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < FH; ++i) {
+        d[now][i] = mfma_block(fa[par][h * FH + i], fb[j % FB]);
       }
+      if (step == 0) {
+        add(FJ - 1, HS - 1, before, pending);
+      } else {
+        add(frag_of(step - 1), half_of(step - 1), before, sc[frag_of(step - 1)]);
+      }
+#pragma unroll
+      for (int o = 0; o < kOps; ++o) {
+        if (step_of(o) == step) { load(o < kEarly ? cur : prev, o); }
+      }
+      if (!kAhead && j == FJ - 1) {
+#pragma unroll
+        for (int i = 0; i < FH; ++i) { fa[0][h * FH + i] = read_w(next, h * FH + i); }
+      }
+#pragma unroll
+      for (int i = 0; i < FH; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
+        if (i == 0) { __builtin_amdgcn_sched_group_barrier(0x100, 8, 0); }    // reads
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);        // the sums
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     pending = sc[FJ - 1];
     settle();
@@ -723,7 +742,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
 #pragma unroll
   for (int i = 0; i < FI; ++i) { fa[0][i] = read_w(0, i); }
 #pragma unroll
-  for (int j = 0; j < A; ++j) { fb[j] = read_a(0, j); }
+  for (int j = 0; j < 2; ++j) { fb[j] = read_a(0, j); }
   read_scales(0);
 
   int prev = NS - 1, cur = 0, next = 1, round = 0;
@@ -1047,7 +1066,7 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 // The tile builds: X(WM, WN, FJ, FI, FB, NS).
 #define U15H_FP8_TILES(X) \
   X(2, 4, 8, 4, 4, 2)     \
-  X(2, 4, 6, 4, 3, 2)     \
+  X(2, 4, 6, 4, 6, 2)     \
   X(2, 4, 4, 4, 4, 3)     \
   X(2, 4, 4, 2, 4, 4)     \
   X(2, 2, 4, 4, 4, 2)     \
