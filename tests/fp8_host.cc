@@ -54,7 +54,7 @@ end_call(u15h_ctx* ctx, hipError_t e, const char* what)
   return e == hipSuccess ? U15H_OK : set_error(ctx, U15H_ELAUNCH, what);
 }
 
-int num_cus(const u15h_ctx* ctx) { return ctx->cus; }
+int gemm_cus(const u15h_ctx* ctx) { return ctx->cus; }
 
 u15h_status
 split_workspace(u15h_ctx*, void** ws)

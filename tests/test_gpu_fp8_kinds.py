@@ -76,6 +76,17 @@ def test_every_kernel(ops, size, name, split, rounds):
 SPLIT = [size for size, _, split, _ in ref.KINDS if split and size[0] + size[1] < 400]
 
 
+@pytest.mark.parametrize("knob,value", [("U15H_SPLIT", "0"), ("U15H_GEMM_CUS", "192")])
+def test_knobs(monkeypatch, knob, value):
+    """A context that splits no tiles, one whose rounds leave units free."""
+    monkeypatch.setenv(knob, value)
+    o = u15h.Ops(0)
+    for size in SPLIT + [ref.KINDS[12][0]]:
+        run(o, size)
+    torch.cuda.synchronize()
+    o.close()
+
+
 def test_two_graphs_of_one_context():
     """Graphs that share the context's workspace, replayed in turns with eager
     calls between, each replay on new inputs."""

@@ -760,9 +760,9 @@ u15h::end_call(u15h_ctx* ctx, hipError_t e, const char* what)
 }
 
 int
-u15h::num_cus(const u15h_ctx* ctx)
+u15h::gemm_cus(const u15h_ctx* ctx)
 {
-  return ctx->num_cu;
+  return ctx->gemm_cus;
 }
 
 u15h_status
@@ -776,7 +776,7 @@ u15h::split_workspace(u15h_ctx* ctx, void** ws)
 size_t
 u15h::split_workspace_bytes(const u15h_ctx* ctx)
 {
-  return split_ws_capacity(ctx);
+  return ctx->split_on ? split_ws_capacity(ctx) : 0;
 }
 
 extern "C" {

@@ -360,7 +360,7 @@ u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream, const uint8_t* xq, const fl
     const u15h_mot_proj_fp8& p = proj[i];
     add_problem(b, xq, sx, p.wq_und, p.sw_und, p.y, M_und, p.N);
   }
-  b.cus = u15h::num_cus(ctx);
+  b.cus = u15h::gemm_cus(ctx);
   if (!plan(b, u15h::split_workspace_bytes(ctx))) { return refuse(ctx, "%s: too many tiles", what); }
   if (b.split > 1) {
     void* ws = nullptr;

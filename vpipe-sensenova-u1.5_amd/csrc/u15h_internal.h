@@ -286,7 +286,7 @@ struct Fp8Batch {
   int bm, bn;             // tile: activation rows x weight rows
   int waves;              // per workgroup
   bool narrow;
-  int cus;                // compute units
+  int cus;                // compute units to use
   int total_tiles;
   // Tiles [split_begin, total_tiles) run as `split` workgroups each, every
   // one a contiguous share of the blocks of K whose f32 sums go to ws
@@ -321,12 +321,13 @@ hipError_t launch_fp8_norm(const Fp8NormArgs& a, hipStream_t s);
 bool fp8_kernels_loadable();
 
 // What entry points outside u15h_api.cc need of the context: the device made
-// current; a launch's result as the call's status; the number of CUs.
+// current; a launch's result as the call's status; the CUs that a GEMM's rounds
+// are planned for.
 u15h_status begin_call(u15h_ctx* ctx);
 u15h_status end_call(u15h_ctx* ctx, hipError_t e, const char* what);
-int num_cus(const u15h_ctx* ctx);
+int gemm_cus(const u15h_ctx* ctx);
 // The context's split-K workspace (allocated on first use, also under stream
-// capture) and its size.
+// capture) and its size (0 where splitting is switched off).
 u15h_status split_workspace(u15h_ctx* ctx, void** ws);
 size_t split_workspace_bytes(const u15h_ctx* ctx);
 
