@@ -208,3 +208,31 @@ def test_product_past_32_bits(ops):
     ops.mot_gemm_fp8(xq, sx, mu, mg, K, projs)
     check(xq, sx, projs, mu, rows=[0, 6, 7, 8, 262143, 262144, 262150, 299998, 299999])
     assert not bool(projs[0]["y"].isnan().any())
+
+
+def test_most_rows(ops):
+    """2^22 rows, the most that a call takes: the last ones are as they are
+    alone."""
+    rows, dim = 1 << 22, 4112
+    x = torch.zeros(rows, dim, dtype=BF16, device="cuda")
+    tail = torch.randn(5, dim, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    x[-5:] = tail
+    w = torch.ones(dim, dtype=BF16, device="cuda")
+    q, s = torch.empty(rows, dim, dtype=F8, device="cuda"), torch.empty(33, rows, device="cuda")
+    q5, s5 = torch.empty(5, dim, dtype=F8, device="cuda"), torch.empty(33, 5, device="cuda")
+    for call in (lambda a, m, qq, ss: ops.mot_rms_norm_fp8(a, 0, m, None, w, qq, ss),
+                 lambda a, m, qq, ss: ops.quant_rows_fp8(a, qq, ss),
+                 lambda a, m, qq, ss: ops.swiglu_quant_fp8(a, a, qq, ss)):
+        q.view(torch.uint8).fill_(0x55)
+        call(x, rows, q, s)
+        call(tail, 5, q5, s5)
+        assert torch.equal(q[-5:].view(torch.uint8), q5.view(torch.uint8))
+        assert torch.equal(s[:, -5:], s5)
+        assert not bool(q[rows // 2:rows // 2 + 4096].view(torch.uint8).any())
+        assert not bool(q[:4096].view(torch.uint8).any())
+    del x, q, s
+    K, N = 144, 8
+    xq, sx, projs = operands(0, rows, K, (N,))
+    ops.mot_gemm_fp8(xq, sx, 0, rows, K, projs)
+    check(xq, sx, projs, 0, rows=[0, 1, 63, 64, 1 << 21, rows - 65, rows - 64, rows - 1])
+    assert not bool(projs[0]["y"].isnan().any())

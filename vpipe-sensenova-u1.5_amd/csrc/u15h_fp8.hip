@@ -618,7 +618,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   // A stage's loads begin behind the barrier, few a step (a wave waits to issue
   // one while others' go out), the last of them in the next stage's first steps:
   // over all of a stage's time, but with two places only over two thirds, as
-  // the next barrier but one waits for them.
+  // the next barrier waits for them.
   constexpr int kSpan = NS > 2 ? kSteps : 2 * kSteps / 3;
   auto step_of = [](int op) { return (kBarrier + op * kSpan / kOps) % kSteps; };
   constexpr int kEarly =

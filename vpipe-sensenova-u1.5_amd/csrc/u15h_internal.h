@@ -289,9 +289,9 @@ struct Fp8Batch {
   int cus;                // compute units to use
   int total_tiles;
   // Tiles [split_begin, total_tiles) run as `split` workgroups each, every
-  // one a contiguous share of the blocks of K whose f32 sums go to ws
-  // ([(tile - split_begin) * split + share][bm][bn]); a second kernel adds
-  // the shares in order.
+  // one a contiguous share of the blocks of K whose f32 sums go to ws (bm * bn
+  // of them at (tile - split_begin) * split + share, in the order in which the
+  // tile's lanes hold them); a second kernel adds the shares in order.
   int split_begin;
   int split;
   float* ws;

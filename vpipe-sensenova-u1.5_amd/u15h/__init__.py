@@ -827,8 +827,7 @@ class Ops:
                                         len(projs))
         self._check(st, "u15h_mot_gemm_i8")
 
-    # ---- profiling -------------------------------------------------------
-    # ---- fp8 tier ------------------------------------------------------
+    # ---- fp8 tier --------------------------------------------------------
     # The smallest of these calls take less on the GPU than on the host, so a
     # tensor's checks and its address are one pass, and the stream is looked up
     # without asking whether CUDA is up (a checked tensor lives on it).
@@ -953,6 +952,7 @@ class Ops:
         if st:
             self._check(st, "u15h_mot_gemm_fp8")
 
+    # ---- profiling -------------------------------------------------------
     def profile_next_gemm(self, event):
         """Record the raw hipEvent_t `event` (a ctypes.c_void_p or int
         handle) right after the next GEMM kernel, before any split-K
