@@ -133,24 +133,21 @@ KINDS = [
     ((98, 5, 400, (136,)), "narrow 128x16x4", False, False),
     ((0, 132, 144, (200,)), "tiles 64x128x4", False, False),
     ((132, 5, 144, (8360, 7984)), "tiles 64x128x4", False, True),
-    ((129, 4, 1680, (8,)), "tiles 64x128x4", True, False),
-    ((209, 4, 16, (6688, 14192)), "tiles 128x128x4", False, False),
-    ((648, 9, 16, (11272,)), "tiles 128x128x4", False, True),
-    ((2358, 3176, 7520, (80,)), "tiles 128x128x4", True, False),
-    ((68, 21, 288, (11768,)), "tiles 128x128x8", False, False),
-    ((332, 1, 2336, (16176, 32)), "tiles 128x128x8", False, True),
-    ((7, 106, 3904, (3936,)), "tiles 128x128x8", True, False),
-    ((17, 44, 3936, (16256, 312)), "tiles 128x128x8", True, True),
+    ((2, 131, 2208, (8,)), "tiles 64x128x4", True, False),
+    ((140, 2, 432, (8408,)), "tiles 128x128x8", False, False),
+    ((35, 586, 736, (10832,)), "tiles 128x128x8", False, True),
+    ((69, 0, 4720, (5480,)), "tiles 128x128x8", True, False),
+    ((19, 1, 5968, (8248, 12248)), "tiles 128x128x8", True, True),
     ((18, 321, 288, (256, 15272)), "tiles 128x256x8", False, False),
-    ((866, 1, 592, (14464,)), "tiles 128x256x8", False, True),
-    ((0, 145, 7760, (40, 5344)), "tiles 128x256x8", True, False),
-    ((305, 1, 3264, (16304, 584)), "tiles 128x256x8", True, True),
-    ((3496, 3, 416, (2224, 16)), "tiles 192x256x8", False, False),
-    ((1, 864, 288, (5064, 15584)), "tiles 192x256x8", False, True),
-    ((0, 576, 8080, (6736,)), "tiles 192x256x8", True, False),
-    ((1756, 0, 6096, (752, 5864)), "tiles 192x256x8", True, True),
+    ((2, 3191, 368, (4808,)), "tiles 128x256x8", False, True),
+    ((14, 204, 6976, (6800,)), "tiles 128x256x8", True, False),
+    ((464, 10, 2368, (13320,)), "tiles 128x256x8", True, True),
+    ((6, 3632, 272, (128, 2712)), "tiles 192x256x8", False, False),
+    ((2771, 0, 144, (7672,)), "tiles 192x256x8", False, True),
+    ((0, 531, 8288, (7024,)), "tiles 192x256x8", True, False),
+    ((0, 3590, 2816, (6720,)), "tiles 192x256x8", True, True),
     ((3327, 25, 400, (3592, 8)), "tiles 256x256x8", False, False),
-    ((3299, 0, 16, (9848, 9000)), "tiles 256x256x8", False, True),
+    ((2590, 772, 144, (6056, 1496)), "tiles 256x256x8", False, True),
     ((0, 392, 6448, (9736,)), "tiles 256x256x8", True, False),
-    ((3540, 0, 1680, (4712,)), "tiles 256x256x8", True, True),
+    ((0, 1764, 1376, (9624,)), "tiles 256x256x8", True, True),
 ]

@@ -35,7 +35,8 @@ def host(tmp_path_factory):
 
 
 def kernel_builds():
-    """(bm, bn, waves) of every product kernel, narrow and tiled, as built."""
+    """(bm, bn, waves that multiply) of every product kernel, narrow and tiled, as
+    built."""
     text = (CSRC / "u15h_fp8.hip").read_text()
 
     def rows(macro):

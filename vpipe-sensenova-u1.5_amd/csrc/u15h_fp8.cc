@@ -95,34 +95,34 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
 //   narrow: `round` per workgroup of the busiest CU, `stage` per block of K of
 //           those, `stream` per block of all of them over the CUs;
 //   tiles:  `round` and `stage` per round of workgroups (a CU that runs two
-//           takes two stages), `split` for the second launch with K shares and
-//           `part` per MB of their sums;
+//           takes two stages), `split` for the second launch with K shares,
+//           `share` for each of them and `part` per MB of their sums;
 //   and `weight` per MB of weights.
-// Fitted to 8858 timings (a graph, weights rotated; M 1-4224, K 256-12288, N
+// Fitted to 7096 timings (a graph, weights rotated; M 1-4224, K 256-12288, N
 // 512-24576, every kind and 1 to 16 shares), each to 5-9% on the mean; the kind
-// and shares with the least estimate take 0.9% longer than the fastest of all,
-// on the mean over the 338 sizes, and 16% at worst (1152 rows, K 8192, N 1024:
-// 29.7 against 25.5 us).
+// and shares with the least estimate take 0.7% longer than the fastest of all,
+// on the mean over the 338 sizes, and 18% at worst (64 rows, K 8192, N 1024:
+// 13.4 against 11.4 us).
+// `waves` are those that multiply.
 struct Kind {
   bool narrow;
   int bm, bn, waves;
-  double fixed, round, stage, stream, split, part, weight;
+  double fixed, round, stage, stream, split, part, weight, share;
 };
 constexpr Kind kKinds[] = {
-    {true, 16, 16, 4, 2.40, 0.48, 0.0511, 0.0463, 0, 0, 0},
-    {true, 16, 32, 4, 1.92, 1.34, 0.0831, 0.0992, 0, 0, 0},
-    {true, 32, 16, 4, 1.74, 1.43, 0.0696, 0.0466, 0, 0, 0},
-    {true, 32, 32, 4, 2.13, 1.42, 0.1017, 0.0953, 0, 0, 0},
-    {true, 64, 16, 4, 1.42, 1.97, 0.1176, 0.0552, 0, 0, 0},
-    {true, 64, 32, 4, 3.05, 0.90, 0.1480, 0.1202, 0, 0, 0},
-    {true, 96, 16, 4, 1.42, 2.10, 0.1673, 0.0489, 0, 0, 0},
-    {true, 128, 16, 4, 1.42, 2.43, 0.2098, 0.0525, 0, 0, 0},
-    {false, 64, 128, 4, 4.17, 0.17, 0.344, 0, 3.45, 0.355, 0.115},
-    {false, 128, 128, 4, 4.63, 0, 0.563, 0, 3.67, 0.275, 0.138},
-    {false, 128, 128, 8, 2.75, 2.26, 0.518, 0, 3.46, 0.384, 0.080},
-    {false, 128, 256, 8, 2.73, 2.99, 0.765, 0, 3.71, 0.310, 0.104},
-    {false, 192, 256, 8, 5.78, 1.13, 1.097, 0, 3.65, 0.216, 0.141},
-    {false, 256, 256, 8, 7.98, 0, 1.309, 0, 4.81, 0.137, 0.125},
+    {true, 16, 16, 4, 2.44, 0.45, 0.0505, 0.0470, 0, 0, 0, 0},
+    {true, 16, 32, 4, 1.98, 1.27, 0.0835, 0.0982, 0, 0, 0, 0},
+    {true, 32, 16, 4, 1.80, 1.37, 0.0697, 0.0481, 0, 0, 0, 0},
+    {true, 32, 32, 4, 2.32, 1.20, 0.1018, 0.0969, 0, 0, 0, 0},
+    {true, 64, 16, 4, 1.40, 1.97, 0.1188, 0.0541, 0, 0, 0, 0},
+    {true, 64, 32, 4, 3.06, 0.89, 0.1480, 0.1212, 0, 0, 0, 0},
+    {true, 96, 16, 4, 1.43, 2.09, 0.1667, 0.0494, 0, 0, 0, 0},
+    {true, 128, 16, 4, 1.45, 2.43, 0.2099, 0.0515, 0, 0, 0, 0},
+    {false, 64, 128, 4, 3.71, 0.25, 0.320, 0, 2.53, 0.345, 0.129, 0.168},
+    {false, 128, 128, 8, 3.27, 1.65, 0.455, 0, 2.63, 0.376, 0.090, 0.139},
+    {false, 128, 256, 8, 3.36, 2.44, 0.690, 0, 2.79, 0.297, 0.115, 0.148},
+    {false, 192, 256, 8, 5.87, 0.97, 1.100, 0, 2.69, 0.204, 0.143, 0.187},
+    {false, 256, 256, 8, 7.73, 0, 1.317, 0, 3.83, 0.121, 0.111, 0.235},
 };
 
 // Workgroups of a kind of tile that run at once.
@@ -210,7 +210,7 @@ plan(Fp8Batch& b, size_t workspace)
         const int last = rem * S - (rounds - 1) * slots > C ? two : 1;
         us += rounds * k.round + ((rounds - 1) * two + last) * nst * k.stage;
       }
-      if (S > 1) { us += k.split + rem * S * tile_mb * valid / padded * k.part; }
+      if (S > 1) { us += k.split + S * k.share + rem * S * tile_mb * valid / padded * k.part; }
       consider(k, S, us);
     }
   }

@@ -427,18 +427,19 @@ fp8_work(const Fp8Batch& B, int nb, int w)
 }
 
 // A workgroup's tile: WM x WN waves, each FJ fragments of activation rows by FI
-// of weight rows.  Its LDS: NS stages of scales (the tile's rows', then its
-// columns'), of activations and of weights.
-template <int WM, int WN, int FJ, int FI, int NS>
+// of weight rows, and LWV waves that only load (0: the others load).  Its LDS: NS
+// stages of scales (the tile's rows', then its columns'), of activations and of
+// weights.
+template <int WM, int WN, int FJ, int FI, int NS, int LWV>
 struct Fp8Tile {
-  static constexpr int kWaves = WM * WN;
+  static constexpr int kWaves = WM * WN + LWV;
   static constexpr int BM = 16 * WM * FJ, BN = 16 * WN * FI;
   static constexpr int kRowScales = (BM + 63) / 64 * 64;
   static constexpr int kScales = kRowScales + 64;                // floats per stage
   static constexpr int kAct = (NS * kScales * 4 + 1023) / 1024 * 1024;
   static constexpr int kWeight = kAct + NS * BM * 128;
   static constexpr int kBytes = kWeight + NS * BN * 128;
-  static constexpr int kPerCu = std::max(std::min(160 * 1024 / kBytes, 8 / kWaves), 1);
+  static constexpr int kPerCu = std::max(std::min(160 * 1024 / kBytes, 8 / (WM * WN)), 1);
 };
 
 // One stage is one block of K.  Both operands come through LDS by direct loads
@@ -460,11 +461,14 @@ struct Fp8Tile {
 // multiply-adds alone, from registers, reach 3.7 to 4.0 PFLOP/s; 4096 rows of
 // K 12288 and 4096 columns run at 2.35 (175 us), 4224 rows of two times 12288
 // columns at 2.07 (412 us).
-// The smaller tiles have few products a stage to hide its barrier and reads
-// behind, so they have more places (NS) and their weights' fragments a stage
-// ahead: 1024 rows of K 4096 and 4096 columns take 28 us on 128 x 128 tiles of
-// eight waves, 34 on four waves with half the places and 31 on 64 x 128; of
-// 2048 rows it is 51, 44 and 55 us.
+// The smaller tiles have few products a stage to hide its barrier, reads and
+// loads behind, so they have more places (NS), their weights' fragments a stage
+// ahead where registers allow, and four waves that load for the others (a wave
+// waits to issue a load while others' go out: 12 cycles each, 40 to 48 of them
+// beside the 512 cycles of products of 128 x 128).  With them and without: a
+// stage of 128 x 128 takes 0.39 and 0.49 us, of 64 x 128 0.26 and 0.37; 2048
+// rows of K 8192 and 4096 columns take 64 and 74 us on 128 x 256.  The larger
+// two have no registers to spare for more waves.
 // Row r's 16-byte chunk c sits at position c ^ ((r >> 1) & 7), which spreads
 // the 16 rows of a fragment read over the bank groups; the loads put it there
 // by fetching the chunk that belongs at their landing position.  They also
@@ -474,12 +478,13 @@ struct Fp8Tile {
 //
 // Persistent: the loads run ahead over the end of a tile into the next one,
 // whose first stages land while this one's results are stored.
-template <int WM, int WN, int FJ, int FI, int FB, int NS>
+template <int WM, int WN, int FJ, int FI, int FB, int NS, int LWV>
 __device__ __forceinline__ void
 fp8_tiles(const Fp8Batch& B, char* lds)
 {
-  using L = Fp8Tile<WM, WN, FJ, FI, NS>;
-  constexpr int BM = L::BM, BN = L::BN, NW = L::kWaves;
+  using L = Fp8Tile<WM, WN, FJ, FI, NS, LWV>;
+  constexpr int BM = L::BM, BN = L::BN;
+  constexpr int NW = LWV > 0 ? LWV : WM * WN;        // the waves that load
   constexpr int kStageA = BM * 128, kStageW = BN * 128;
   constexpr int LA = BM / 8 / NW, LW = BN / 8 / NW;  // a wave's loads per stage
   constexpr int kOps = LA + LW + 1;
@@ -492,6 +497,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lh = lane >> 4;
   const int wm = wave % WM, wn = wave / WM;
+  const int lwave = LWV > 0 ? wave - WM * WN : wave;
 
   // Items go in rounds of gridDim.x; workgroups b, b + 8, .. run on XCD b % 8,
   // and of each round every XCD takes a contiguous run.
@@ -515,7 +521,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     int ko, left, last;   // the block's bytes into a row, blocks left, -1 in the last of K
     int round;
   } ld;
-  const bool row_wave = wave < L::kRowScales / 64;
+  const bool row_wave = lwave < L::kRowScales / 64;
   auto load_item = [&](int it) {
     const Fp8Work t = fp8_work<BM, BN>(B, nb, it);
     const Fp8Problem& P = B.p[t.prob];
@@ -523,9 +529,9 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     ld.a = make_rsrc(P.a + (size_t)t.row0 * K, rows * K);
     ld.w = make_rsrc(P.w + (size_t)t.col0 * K, cols * K);
     if (row_wave) {
-      ld.sc = P.sa + (size_t)t.kbeg * sa_pitch + t.row0 + wave * 64;
+      ld.sc = P.sa + (size_t)t.kbeg * sa_pitch + t.row0 + lwave * 64;
       ld.pitch = sa_pitch;
-      ld.count = max(0, min(64, rows - wave * 64)) * 4;
+      ld.count = max(0, min(64, rows - lwave * 64)) * 4;
     } else {
       ld.sc = P.sw + (size_t)(t.col0 / 128) * nb + t.kbeg;
       ld.pitch = 1;
@@ -541,13 +547,13 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   // A load's lane l fills chunk position l % 8 of row l / 8 of its 8 LDS rows.
   // Wave w fills blocks w, w + NW, .. of 8 rows, all of one parity (a half of
   // 16), so its lanes' chunk is one.
-  const int half = (wave & 1) * 8 + (lane >> 3);     // the row of its 16
+  const int half = (lwave & 1) * 8 + (lane >> 3);     // the row of its 16
   const int chunk = (lane & 7) ^ (half >> 1);
   const int tail = (nb - 1) * 128 + (chunk << 4) < K ? 0 : kOobOffset;
   // .. and of its rows the part that differs from lane to lane
   const int alane = half * FJ * K + (chunk << 4);
   const int wlane = ((half >> 2) * 8 + (half & 3)) * K + (chunk << 4);
-  const int w2 = uniform(wave >> 1);
+  const int w2 = uniform(lwave >> 1);
   // scales: a lane each; the columns' are nb apart
   constexpr int kColBlocks = (BN + 127) / 128;
   const int soff = row_wave ? lane * 4 : lane < kColBlocks ? lane * nb * 4 : kOobOffset;
@@ -559,14 +565,14 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   auto load = [&](int slot, int op) {
     if (op < LW) {
       const int f = w2 + NW / 2 * op;                // of the tile's fragments
-      dma16(ld.w, lds + L::kWeight + slot * kStageW + (wave + NW * op) * 1024,
+      dma16(ld.w, lds + L::kWeight + slot * kStageW + (lwave + NW * op) * 1024,
             (wlane | (tail & ld.last)) + ((f >> 1) * 32 + (f & 1) * 4) * K, ld.ko);
     } else if (op < LW + LA) {
       const int o = op - LW, f = w2 + NW / 2 * o;
-      dma16(ld.a, lds + L::kAct + slot * kStageA + (wave + NW * o) * 1024,
+      dma16(ld.a, lds + L::kAct + slot * kStageA + (lwave + NW * o) * 1024,
             (alane | (tail & ld.last)) + (f / FJ * (16 * FJ) + f % FJ) * K, ld.ko);
     } else {
-      const int g = row_wave ? wave * 64 : L::kRowScales;
+      const int g = row_wave ? lwave * 64 : L::kRowScales;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           make_rsrc(ld.sc, ld.count),
           (__attribute__((address_space(3))) void*)(scales + slot * L::kScales + g), 4, soff, 0,
@@ -587,6 +593,41 @@ fp8_tiles(const Fp8Batch& B, char* lds)
       }
     }
   };
+
+  // Loading waves of their own: a stage's loads behind each barrier, NS stages
+  // ahead, as many barriers as the others pass.
+  if constexpr (LWV > 0) {
+    if (wave >= WM * WN) {
+      int it = item_of(0), place = 0;
+      if (it < 0) { return; }
+      ld.round = 0;
+      load_item(it);
+#pragma unroll
+      for (int r = 0; r < NS; ++r) {
+#pragma unroll
+        for (int o = 0; o < kOps; ++o) { load(r, o); }
+        advance();
+      }
+      static_assert((NS - 1) * kOps < 64, "the counter has 6 bits");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * kOps) : "memory");
+      __builtin_amdgcn_s_barrier();
+      for (int round = 0; it >= 0; it = item_of(++round)) {
+        const int nst = fp8_work<BM, BN>(B, nb, it).nst;
+        for (int k = 0; k < nst; ++k) {
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * kOps) : "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int o = 0; o < kOps; ++o) { load(place, o); }
+          advance();
+          place = place + 1 == NS ? 0 : place + 1;
+        }
+      }
+      // no load may still be writing LDS when the workgroup ends
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      return;
+    }
+  }
 
   // ---- fragments -------------------------------------------------------------
   const int key = (lr >> 1) & 7;
@@ -615,11 +656,11 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   auto half_of = [](int step) { return step % (2 * HS) / 2; };
   constexpr int kBarrier = kSteps - 2 * HS;          // the barrier's step: the last pair
   static_assert(FJ % 2 == 0 && FB >= 4 && FJ % FB == 0, "fragment buffers come round with a stage");
-  // A stage's loads begin behind the barrier, few a step (a wave waits to issue
-  // one while others' go out), the last of them in the next stage's first steps:
-  // over all of a stage's time, but with two places only over two thirds, as
-  // the next barrier waits for them.
-  constexpr int kSpan = NS > 2 ? kSteps : 2 * kSteps / 3;
+  // Where the multiplying waves load: a stage's loads begin behind the barrier,
+  // about one a step, the last of them in the next stage's first steps, over two
+  // thirds of a stage's time, as the next barrier waits for them.
+  constexpr int kSpan = 2 * kSteps / 3;
+  static_assert(LWV > 0 || NS == 2, "which leaves them little time to land");
   auto step_of = [](int op) { return (kBarrier + op * kSpan / kOps) % kSteps; };
   constexpr int kEarly =
       std::min(kOps, ((kSteps - kBarrier) * kOps + kSpan - 1) / kSpan);   // before its end
@@ -627,7 +668,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   f32x4_t acc[FI][FJ], d[2][FH];
   // Weight fragments of this stage and the next; where registers are short, the
   // next one's take the places of this one's as its last products leave them.
-  constexpr bool kAhead = FJ * FI <= 16;
+  constexpr bool kAhead = FJ * FI <= 8;
   i32x8_t fa[kAhead ? 2 : 1][FI], fb[FB];
   float sc[FJ];                                      // the stage's scales, rows' times columns'
   sv_t sv[FJ / SV];                                  // the next stage's, apart
@@ -678,9 +719,13 @@ fp8_tiles(const Fp8Batch& B, char* lds)
     for (int step = 0; step < kSteps; ++step) {
       const int j = frag_of(step), h = half_of(step);
       if (step == kBarrier) {
-        settle();
-        advance();
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * kOps) : "memory");
+        if constexpr (LWV > 0) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        } else {
+          settle();
+          advance();
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * kOps) : "memory");
+        }
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
@@ -706,7 +751,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
       }
 #pragma unroll
       for (int o = 0; o < kOps; ++o) {
-        if (step_of(o) == step) { load(o < kEarly ? cur : prev, o); }
+        if (LWV == 0 && step_of(o) == step) { load(o < kEarly ? cur : prev, o); }
       }
       if (!kAhead && j == FJ - 1) {
 #pragma unroll
@@ -727,16 +772,18 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   // ---- the first item's first stages -------------------------------------------
   int it = item_of(0);
   if (it < 0) { return; }
-  ld.round = 0;
-  load_item(it);
+  if constexpr (LWV == 0) {
+    ld.round = 0;
+    load_item(it);
 #pragma unroll
-  for (int r = 0; r < NS; ++r) {
+    for (int r = 0; r < NS; ++r) {
 #pragma unroll
-    for (int o = 0; o < (r < NS - 1 ? kOps : kEarly); ++o) { load(r, o); }
-    if (r < NS - 1) { advance(); }
-    __builtin_amdgcn_sched_barrier(0);
+      for (int o = 0; o < (r < NS - 1 ? kOps : kEarly); ++o) { load(r, o); }
+      if (r < NS - 1) { advance(); }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * kOps + kEarly) : "memory");   // stage 0's
   }
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * kOps + kEarly) : "memory");   // stage 0's
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 #pragma unroll
@@ -813,15 +860,16 @@ fp8_tiles(const Fp8Batch& B, char* lds)
 
 // (a tile's workgroups on a compute unit, and so its waves per SIMD, are what its
 // LDS leaves room for)
-template <int WM, int WN, int FJ, int FI, int NS>
-constexpr int kTileWaves = Fp8Tile<WM, WN, FJ, FI, NS>::kPerCu * WM * WN / 4;
+template <int WM, int WN, int FJ, int FI, int NS, int LWV>
+constexpr int kTileWaves =
+    Fp8Tile<WM, WN, FJ, FI, NS, LWV>::kPerCu * Fp8Tile<WM, WN, FJ, FI, NS, LWV>::kWaves / 4;
 
-template <int WM, int WN, int FJ, int FI, int FB, int NS>
-__global__ __launch_bounds__(64 * WM * WN, (kTileWaves<WM, WN, FJ, FI, NS>)) void
+template <int WM, int WN, int FJ, int FI, int FB, int NS, int LWV>
+__global__ __launch_bounds__(64 * (WM * WN + LWV), (kTileWaves<WM, WN, FJ, FI, NS, LWV>)) void
 fp8_tile_kernel(const Fp8Batch B)
 {
-  __shared__ __attribute__((aligned(1024))) char lds[Fp8Tile<WM, WN, FJ, FI, NS>::kBytes];
-  fp8_tiles<WM, WN, FJ, FI, FB, NS>(B, lds);
+  __shared__ __attribute__((aligned(1024))) char lds[Fp8Tile<WM, WN, FJ, FI, NS, LWV>::kBytes];
+  fp8_tiles<WM, WN, FJ, FI, FB, NS, LWV>(B, lds);
 }
 
 // ---- few rows: the weights' stream ---------------------------------------------
@@ -1028,14 +1076,14 @@ fp8_reduce_kernel(const Fp8Batch B)
               pack_bf16x2(v[2], v[3])};
 }
 
-template <int WM, int WN, int FJ, int FI, int FB, int NS>
+template <int WM, int WN, int FJ, int FI, int FB, int NS, int LWV>
 hipError_t
 tile_launch(const Fp8Batch& b, hipStream_t s)
 {
-  using L = Fp8Tile<WM, WN, FJ, FI, NS>;
+  using L = Fp8Tile<WM, WN, FJ, FI, NS, LWV>;
   const int tail = b.total_tiles - b.split_begin;
   const int items = b.split_begin + tail * b.split;
-  fp8_tile_kernel<WM, WN, FJ, FI, FB, NS>
+  fp8_tile_kernel<WM, WN, FJ, FI, FB, NS, LWV>
       <<<std::min(items, b.cus * L::kPerCu), 64 * L::kWaves, 0, s>>>(b);   // all at once
   if (b.split > 1 && tail > 0) {
     fp8_reduce_kernel<WM, WN, FJ, FI><<<tail * (L::BM * L::BN / 2048), 256, 0, s>>>(b);
@@ -1063,14 +1111,13 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 
 }  // namespace
 
-// The tile builds: X(WM, WN, FJ, FI, FB, NS).
+// The tile builds: X(WM, WN, FJ, FI, FB, NS, LWV).
 #define U15H_FP8_TILES(X) \
-  X(2, 4, 8, 4, 4, 2)     \
-  X(2, 4, 6, 4, 6, 2)     \
-  X(2, 4, 4, 4, 4, 3)     \
-  X(2, 4, 4, 2, 4, 4)     \
-  X(2, 2, 4, 4, 4, 2)     \
-  X(1, 4, 4, 2, 4, 3)
+  X(2, 4, 8, 4, 4, 2, 0)  \
+  X(2, 4, 6, 4, 6, 2, 0)  \
+  X(2, 4, 4, 4, 4, 3, 4)  \
+  X(2, 4, 4, 2, 4, 4, 4)  \
+  X(1, 4, 4, 2, 4, 3, 4)
 
 #define U15H_FP8_NARROW(X) \
   X(1, 1, 4, 4)            \
@@ -1099,9 +1146,9 @@ launch_fp8_gemm(const Fp8Batch& b, hipStream_t s)
   }
   U15H_FP8_NARROW(U15H_CASE)
 #undef U15H_CASE
-#define U15H_CASE(WM, WN, FJ, FI, FB, NS)                                                     \
+#define U15H_CASE(WM, WN, FJ, FI, FB, NS, LWV)                                                     \
   if (!b.narrow && b.bm == 16 * WM * FJ && b.bn == 16 * WN * FI && b.waves == WM * WN) {  \
-    return tile_launch<WM, WN, FJ, FI, FB, NS>(b, s);                                         \
+    return tile_launch<WM, WN, FJ, FI, FB, NS, LWV>(b, s);                                         \
   }
   U15H_FP8_TILES(U15H_CASE)
 #undef U15H_CASE
@@ -1162,8 +1209,8 @@ fp8_kernels_loadable()
 #define U15H_FN(MT, FI, NW, D) reinterpret_cast<const void*>(&fp8_narrow_kernel<MT, FI, NW, D>),
       U15H_FP8_NARROW(U15H_FN)
 #undef U15H_FN
-#define U15H_FN(WM, WN, FJ, FI, FB, NS)                                       \
-  reinterpret_cast<const void*>(&fp8_tile_kernel<WM, WN, FJ, FI, FB, NS>),     \
+#define U15H_FN(WM, WN, FJ, FI, FB, NS, LWV)                                       \
+  reinterpret_cast<const void*>(&fp8_tile_kernel<WM, WN, FJ, FI, FB, NS, LWV>),     \
       reinterpret_cast<const void*>(&fp8_reduce_kernel<WM, WN, FJ, FI>),
       U15H_FP8_TILES(U15H_FN)
 #undef U15H_FN

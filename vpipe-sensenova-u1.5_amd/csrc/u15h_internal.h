@@ -284,7 +284,7 @@ struct Fp8Batch {
   int K;                  // % 16 == 0
   int sa_pitch;           // rows of the whole call
   int bm, bn;             // tile: activation rows x weight rows
-  int waves;              // per workgroup
+  int waves;              // per workgroup that multiply
   bool narrow;
   int cus;                // compute units to use
   int total_tiles;
