@@ -91,8 +91,7 @@ launch_fp8_gemm(const Fp8Batch& b, hipStream_t)
     return hipErrorInvalidValue;
   }
   std::ostringstream s;
-  s << (b.narrow ? "narrow " : "tiles ") << b.bm << "x" << b.bn << "x" << b.waves
-    << " n=" << b.total_tiles << " tail=" << tail << " shares=" << b.split << " rows";
+  s << (b.narrow ? "narrow " : "tiles ") << b.bm << "x" << b.bn << " n=" << b.total_tiles << " tail=" << tail << " shares=" << b.split << " rows";
   for (int i = 0; i < b.nprob; ++i) { s << " " << b.p[i].rows; }
   return emit(s.str());
 }

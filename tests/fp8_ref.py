@@ -123,31 +123,31 @@ def check_codes(q, s, v, rel):
 # 256 compute units: the kernel, whether shares of K are split, and whether the
 # workgroups run more than one round of tiles.
 KINDS = [
-    ((3, 0, 528, (264,)), "narrow 16x16x4", False, False),
-    ((1, 1, 400, (2064,)), "narrow 16x32x4", False, False),
-    ((0, 23, 656, (40, 8)), "narrow 32x16x4", False, False),
-    ((2, 20, 272, (680, 1464)), "narrow 32x32x4", False, False),
-    ((35, 10, 784, (72,)), "narrow 64x16x4", False, False),
-    ((10, 36, 144, (2128,)), "narrow 64x32x4", False, False),
-    ((70, 0, 1040, (136,)), "narrow 96x16x4", False, False),
-    ((98, 5, 400, (136,)), "narrow 128x16x4", False, False),
-    ((0, 132, 144, (200,)), "tiles 64x128x4", False, False),
-    ((132, 5, 144, (8360, 7984)), "tiles 64x128x4", False, True),
-    ((2, 131, 2208, (8,)), "tiles 64x128x4", True, False),
-    ((140, 2, 432, (8408,)), "tiles 128x128x8", False, False),
-    ((35, 586, 736, (10832,)), "tiles 128x128x8", False, True),
-    ((69, 0, 4720, (5480,)), "tiles 128x128x8", True, False),
-    ((19, 1, 5968, (8248, 12248)), "tiles 128x128x8", True, True),
-    ((18, 321, 288, (256, 15272)), "tiles 128x256x8", False, False),
-    ((2, 3191, 368, (4808,)), "tiles 128x256x8", False, True),
-    ((14, 204, 6976, (6800,)), "tiles 128x256x8", True, False),
-    ((464, 10, 2368, (13320,)), "tiles 128x256x8", True, True),
-    ((6, 3632, 272, (128, 2712)), "tiles 192x256x8", False, False),
-    ((2771, 0, 144, (7672,)), "tiles 192x256x8", False, True),
-    ((0, 531, 8288, (7024,)), "tiles 192x256x8", True, False),
-    ((0, 3590, 2816, (6720,)), "tiles 192x256x8", True, True),
-    ((3327, 25, 400, (3592, 8)), "tiles 256x256x8", False, False),
-    ((2590, 772, 144, (6056, 1496)), "tiles 256x256x8", False, True),
-    ((0, 392, 6448, (9736,)), "tiles 256x256x8", True, False),
-    ((0, 1764, 1376, (9624,)), "tiles 256x256x8", True, True),
+    ((3, 0, 528, (264,)), "narrow 16x16", False, False),
+    ((1, 1, 400, (2064,)), "narrow 16x32", False, False),
+    ((0, 23, 656, (40, 8)), "narrow 32x16", False, False),
+    ((2, 20, 272, (680, 1464)), "narrow 32x32", False, False),
+    ((35, 10, 784, (72,)), "narrow 64x16", False, False),
+    ((10, 36, 144, (2128,)), "narrow 64x32", False, False),
+    ((70, 0, 1040, (136,)), "narrow 96x16", False, False),
+    ((98, 5, 400, (136,)), "narrow 128x16", False, False),
+    ((0, 132, 144, (200,)), "tiles 64x128", False, False),
+    ((132, 5, 144, (8360, 7984)), "tiles 64x128", False, True),
+    ((2, 131, 2208, (8,)), "tiles 64x128", True, False),
+    ((140, 2, 432, (8408,)), "tiles 128x128", False, False),
+    ((35, 586, 736, (10832,)), "tiles 128x128", False, True),
+    ((69, 0, 4720, (5480,)), "tiles 128x128", True, False),
+    ((17, 44, 3936, (16256, 312)), "tiles 128x128", True, True),
+    ((18, 321, 288, (256, 15272)), "tiles 128x256", False, False),
+    ((2, 3191, 368, (4808,)), "tiles 128x256", False, True),
+    ((0, 82, 8048, (1752, 15544)), "tiles 128x256", True, False),
+    ((464, 10, 2368, (13320,)), "tiles 128x256", True, True),
+    ((6, 3632, 272, (128, 2712)), "tiles 192x256", False, False),
+    ((2771, 0, 144, (7672,)), "tiles 192x256", False, True),
+    ((0, 912, 9584, (4328,)), "tiles 192x256", True, False),
+    ((0, 1676, 2992, (14520,)), "tiles 192x256", True, True),
+    ((3327, 25, 400, (3592, 8)), "tiles 256x256", False, False),
+    ((2590, 772, 144, (6056, 1496)), "tiles 256x256", False, True),
+    ((0, 392, 6448, (9736,)), "tiles 256x256", True, False),
+    ((0, 1764, 1376, (9624,)), "tiles 256x256", True, True),
 ]

@@ -100,37 +100,30 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
 //   and `weight` per MB of weights.
 // Fitted to 7096 timings (a graph, weights rotated; M 1-4224, K 256-12288, N
 // 512-24576, every kind and 1 to 16 shares), each to 5-9% on the mean; the kind
-// and shares with the least estimate take 0.7% longer than the fastest of all,
+// and shares with the least estimate take 0.8% longer than the fastest of all,
 // on the mean over the 338 sizes, and 18% at worst (64 rows, K 8192, N 1024:
 // 13.4 against 11.4 us).
-// `waves` are those that multiply.
 struct Kind {
   bool narrow;
-  int bm, bn, waves;
+  int bm, bn;
+  int per_cu;          // workgroups of tiles that a CU runs at once
   double fixed, round, stage, stream, split, part, weight, share;
 };
 constexpr Kind kKinds[] = {
-    {true, 16, 16, 4, 2.44, 0.45, 0.0505, 0.0470, 0, 0, 0, 0},
-    {true, 16, 32, 4, 1.98, 1.27, 0.0835, 0.0982, 0, 0, 0, 0},
-    {true, 32, 16, 4, 1.80, 1.37, 0.0697, 0.0481, 0, 0, 0, 0},
-    {true, 32, 32, 4, 2.32, 1.20, 0.1018, 0.0969, 0, 0, 0, 0},
-    {true, 64, 16, 4, 1.40, 1.97, 0.1188, 0.0541, 0, 0, 0, 0},
-    {true, 64, 32, 4, 3.06, 0.89, 0.1480, 0.1212, 0, 0, 0, 0},
-    {true, 96, 16, 4, 1.43, 2.09, 0.1667, 0.0494, 0, 0, 0, 0},
-    {true, 128, 16, 4, 1.45, 2.43, 0.2099, 0.0515, 0, 0, 0, 0},
-    {false, 64, 128, 4, 3.71, 0.25, 0.320, 0, 2.53, 0.345, 0.129, 0.168},
-    {false, 128, 128, 8, 3.27, 1.65, 0.455, 0, 2.63, 0.376, 0.090, 0.139},
-    {false, 128, 256, 8, 3.36, 2.44, 0.690, 0, 2.79, 0.297, 0.115, 0.148},
-    {false, 192, 256, 8, 5.87, 0.97, 1.100, 0, 2.69, 0.204, 0.143, 0.187},
-    {false, 256, 256, 8, 7.73, 0, 1.317, 0, 3.83, 0.121, 0.111, 0.235},
+    {true, 16, 16, 0, 2.39, 0.50, 0.0502, 0.0471, 0, 0, 0, 0},
+    {true, 16, 32, 0, 1.97, 1.30, 0.0822, 0.1000, 0, 0, 0, 0},
+    {true, 32, 16, 0, 1.70, 1.48, 0.0698, 0.0466, 0, 0, 0, 0},
+    {true, 32, 32, 0, 2.42, 1.12, 0.1004, 0.0987, 0, 0, 0, 0},
+    {true, 64, 16, 0, 1.40, 1.97, 0.1184, 0.0536, 0, 0, 0, 0},
+    {true, 64, 32, 0, 2.95, 0.99, 0.1478, 0.1196, 0, 0, 0, 0},
+    {true, 96, 16, 0, 1.42, 2.11, 0.1672, 0.0479, 0, 0, 0, 0},
+    {true, 128, 16, 0, 1.38, 2.48, 0.2095, 0.0507, 0, 0, 0, 0},
+    {false, 64, 128, 2, 3.67, 0.34, 0.316, 0, 2.63, 0.335, 0.130, 0.164},
+    {false, 128, 128, 1, 3.09, 1.70, 0.426, 0, 2.69, 0.364, 0.100, 0.141},
+    {false, 128, 256, 1, 3.14, 2.63, 0.674, 0, 2.76, 0.284, 0.119, 0.165},
+    {false, 192, 256, 1, 5.86, 0.98, 1.093, 0, 2.67, 0.200, 0.144, 0.198},
+    {false, 256, 256, 1, 7.82, 0, 1.307, 0, 3.91, 0.117, 0.109, 0.235},
 };
-
-// Workgroups of a kind of tile that run at once.
-int
-slots_of(const Kind& k, int cus)
-{
-  return k.waves == 4 ? 2 * cus : cus;
-}
 
 // Counts a batch's tiles on a kind and cuts its last partial round in `shares`
 // shares of K; false if the tiles are too many.
@@ -140,7 +133,6 @@ set_tiles(Fp8Batch& b, const Kind& k, int shares)
   b.narrow = k.narrow;
   b.bm = k.bm;
   b.bn = k.bn;
-  b.waves = k.waves;
   long long tiles = 0;
   for (int i = 0; i < b.nprob; ++i) {
     Fp8Problem& q = b.p[i];
@@ -152,7 +144,7 @@ set_tiles(Fp8Batch& b, const Kind& k, int shares)
   }
   b.total_tiles = b.split_begin = (int)tiles;
   b.split = shares;
-  if (shares > 1) { b.split_begin -= b.total_tiles % slots_of(k, b.cus); }
+  if (shares > 1) { b.split_begin -= b.total_tiles % (k.per_cu * b.cus); }
   return true;
 }
 
@@ -192,7 +184,7 @@ plan(Fp8Batch& b, size_t workspace)
       consider(k, 1, k.fixed + load * (k.round + nb * k.stage) + (double)tiles * nb / C * k.stream);
       continue;
     }
-    const int slots = slots_of(k, C), two = slots / C;
+    const int two = k.per_cu, slots = two * C;
     const long long full = tiles / slots, rem = tiles % slots;
     const double fixed = k.fixed + mb * k.weight + full * (k.round + nb * two * k.stage);
     if (best != nullptr && fixed >= least) { continue; }

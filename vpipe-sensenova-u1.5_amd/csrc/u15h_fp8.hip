@@ -463,12 +463,13 @@ struct Fp8Tile {
 // columns at 2.07 (412 us).
 // The smaller tiles have few products a stage to hide its barrier, reads and
 // loads behind, so they have more places (NS), their weights' fragments a stage
-// ahead where registers allow, and four waves that load for the others (a wave
-// waits to issue a load while others' go out: 12 cycles each, 40 to 48 of them
-// beside the 512 cycles of products of 128 x 128).  With them and without: a
-// stage of 128 x 128 takes 0.39 and 0.49 us, of 64 x 128 0.26 and 0.37; 2048
-// rows of K 8192 and 4096 columns take 64 and 74 us on 128 x 256.  The larger
-// two have no registers to spare for more waves.
+// ahead where registers allow, and four waves that load for four that multiply
+// (a wave waits to issue a load while others' go out: 12 cycles each, 40 to 48
+// of them beside the 512 cycles of products of 128 x 128).  A stage of 64 x 128
+// takes 0.26 us where it took 0.37 with four waves that do both, of 128 x 128
+// 0.37 (0.49 with eight, 0.39 with eight and four more that load); 4096 rows of
+// K 8192 and 4096 columns take 124 us on 128 x 256 (138 and 130).  The larger two
+// have no registers to spare for more waves.
 // Row r's 16-byte chunk c sits at position c ^ ((r >> 1) & 7), which spreads
 // the 16 rows of a fragment read over the bank groups; the loads put it there
 // by fetching the chunk that belongs at their landing position.  They also
@@ -668,7 +669,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   f32x4_t acc[FI][FJ], d[2][FH];
   // Weight fragments of this stage and the next; where registers are short, the
   // next one's take the places of this one's as its last products leave them.
-  constexpr bool kAhead = FJ * FI <= 8;
+  constexpr bool kAhead = FJ * FI <= 16;
   i32x8_t fa[kAhead ? 2 : 1][FI], fb[FB];
   float sc[FJ];                                      // the stage's scales, rows' times columns'
   sv_t sv[FJ / SV];                                  // the next stage's, apart
@@ -1115,8 +1116,8 @@ rows_launch(const uint16_t* x, const uint16_t* up, int rows, int K, uint16_t* h,
 #define U15H_FP8_TILES(X) \
   X(2, 4, 8, 4, 4, 2, 0)  \
   X(2, 4, 6, 4, 6, 2, 0)  \
-  X(2, 4, 4, 4, 4, 3, 4)  \
-  X(2, 4, 4, 2, 4, 4, 4)  \
+  X(1, 4, 8, 4, 4, 3, 4)  \
+  X(2, 2, 4, 4, 4, 4, 4)  \
   X(1, 4, 4, 2, 4, 3, 4)
 
 #define U15H_FP8_NARROW(X) \
@@ -1140,14 +1141,14 @@ launch_fp8_gemm(const Fp8Batch& b, hipStream_t s)
     return hipErrorInvalidValue;
   }
 #define U15H_CASE(MT, FI, NW, D)                                                          \
-  if (b.narrow && b.bm == 16 * MT && b.bn == 16 * FI && b.waves == NW) {              \
+  if (b.narrow && b.bm == 16 * MT && b.bn == 16 * FI) {                                \
     fp8_narrow_kernel<MT, FI, NW, D><<<b.total_tiles, 64 * NW, 0, s>>>(b);               \
     return hipGetLastError();                                                            \
   }
   U15H_FP8_NARROW(U15H_CASE)
 #undef U15H_CASE
 #define U15H_CASE(WM, WN, FJ, FI, FB, NS, LWV)                                                     \
-  if (!b.narrow && b.bm == 16 * WM * FJ && b.bn == 16 * WN * FI && b.waves == WM * WN) {  \
+  if (!b.narrow && b.bm == 16 * WM * FJ && b.bn == 16 * WN * FI) {                        \
     return tile_launch<WM, WN, FJ, FI, FB, NS, LWV>(b, s);                                         \
   }
   U15H_FP8_TILES(U15H_CASE)

@@ -284,8 +284,7 @@ struct Fp8Batch {
   int K;                  // % 16 == 0
   int sa_pitch;           // rows of the whole call
   int bm, bn;             // tile: activation rows x weight rows
-  int waves;              // per workgroup that multiply
-  bool narrow;
+  bool narrow;            // few rows: the weights' stream
   int cus;                // compute units to use
   int total_tiles;
   // Tiles [split_begin, total_tiles) run as `split` workgroups each, every
