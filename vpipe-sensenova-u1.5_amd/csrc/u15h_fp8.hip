@@ -464,8 +464,8 @@ struct Fp8Tile {
 // The smaller tiles have few products a stage to hide its barrier, reads and
 // loads behind, so they have more places (NS), their weights' fragments a stage
 // ahead where registers allow, and four waves that load for four that multiply
-// (a wave waits to issue a load while others' go out: 12 cycles each, 40 to 48
-// of them beside the 512 cycles of products of 128 x 128).  A stage of 64 x 128
+// (a wave waits to issue a load while others' go out: 12 cycles each, 36 of
+// them beside the 512 cycles of products of 128 x 128).  A stage of 64 x 128
 // takes 0.26 us where it took 0.37 with four waves that do both, of 128 x 128
 // 0.37 (0.49 with eight, 0.39 with eight and four more that load); 4096 rows of
 // K 8192 and 4096 columns take 124 us on 128 x 256 (138 and 130).  The larger two
