@@ -132,13 +132,35 @@ pack8(const float (&v)[8])
                  pack_bf16x2(v[6], v[7])};
 }
 
-// silu(g) * u in f32: g * rcp(1 + 2^(-g log2 e)) with the hardware's exp2
-// and reciprocal (about 1 ulp each).
-__device__ __forceinline__ float
-swiglu_f32(float g, float u)
+// silu(g) * u in f32: g * rcp(1 + 2^(-g log2 e)) with the hardware's exp2 and
+// reciprocal (about 1 ulp each).  The reciprocal loses results below 2^-126, as
+// gates below -87.3 have; there 1 + e^g is 1, and silu(g) u = g e^g u is
+// multiplied up from four quarters of e^g, each a normal number down to -349,
+// so that nothing vanishes that f32 can hold (silu(-88) is -5e-37).  One test
+// for a lane's eight gates (0.3 of 43 us at 4224 rows of 12288); which form a
+// value takes is its own gate's matter.
+constexpr float kFarGate = -87.0f;
+
+__device__ __forceinline__ void
+swiglu8(float (&v)[8], const float (&u)[8])
 {
-  const float e = __builtin_amdgcn_exp2f(g * -1.4426950408889634f);
-  return (g * __builtin_amdgcn_rcpf(1.0f + e)) * u;
+  float g[8];
+  uint32_t least = 0;          // as bits, which order negative gates downwards
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    g[e] = v[e];
+    least = max(least, __float_as_uint(g[e]));
+    const float x = __builtin_amdgcn_exp2f(g[e] * -1.4426950408889634f);
+    v[e] = (g[e] * __builtin_amdgcn_rcpf(1.0f + x)) * u[e];
+  }
+  if (__builtin_expect(least > __float_as_uint(kFarGate), 0)) {
+    asm volatile("");          // keeps it a branch
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = __builtin_amdgcn_exp2f(g[e] * (0.25f * 1.4426950408889634f));
+      if (g[e] < kFarGate) { v[e] = ((g[e] * t) * t) * ((u[e] * t) * t); }
+    }
+  }
 }
 
 // ---- rows: codes and block-major scales --------------------------------------
@@ -191,8 +213,7 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
     if constexpr (SWIGLU) {
       float u[8];
       unpack8(uv[i], u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { v[e] = swiglu_f32(v[e], u[e]); }
+      swiglu8(v, u);
       if (h != nullptr) {
         const __amdgpu_buffer_rsrc_t hs = make_rsrc(h + base, valid * K * 2);
         __builtin_amdgcn_raw_buffer_store_b128(pack8(v), hs, at * 2 + oob, 0, 0);
