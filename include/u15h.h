@@ -611,11 +611,15 @@ typedef struct {
  * with f32 sums.  xq [M][K], sx [KB][M] over the rows of both groups.
  * Precision: the matrix unit multiplies e4m3 codes exactly, but of the 8
  * products of 8 neighbouring k it keeps each only down to 2^-13 of the
- * binary order of the largest (a rule of the hardware; the rounding of y to
- * bf16 is larger).  Tiles that leave a partial round split K over
- * workgroups, whose f32 sums go to the context's split-K workspace.  Profiling
- * events (u15h_profile_next_gemm and _kernels) stay pending for the next bf16
- * or int8 call.
+ * binary order of the largest (a rule of the hardware).  So such a group is
+ * off by at most 7 * 2^-13 of its largest |x| times its largest |w|, scales
+ * included, besides the roundings of the f32 sums.  In a sum of ordinary
+ * size that is less than the rounding of y to bf16; where a group's products
+ * cancel it can be all of what is left of them (1 - 1 + 2^-14 gives 0).
+ * Tiles that leave a partial round split K over workgroups, whose f32 sums
+ * go to the context's split-K workspace.  Profiling events
+ * (u15h_profile_next_gemm and _kernels) stay pending for the next bf16 or
+ * int8 call.
  * Limits: 1 <= nproj <= U15H_MAX_PROJ, K % 16 == 0, K <= 131072,
  * N % 8 == 0, N <= 2^20, M_und + M_gen <= 2^22. */
 u15h_status u15h_mot_gemm_fp8(u15h_ctx* ctx, u15h_stream stream,
