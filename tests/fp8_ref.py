@@ -151,3 +151,21 @@ KINDS = [
     ((0, 392, 6448, (9736,)), "tiles 256x256", True, False),
     ((0, 1764, 1376, (9624,)), "tiles 256x256", True, True),
 ]
+
+# Sizes (M_und, M_gen, K, Ns) of long K, the kernel that takes each on 256
+# compute units, and whether shares of K are split.  A narrow kernel's four
+# waves take more than 64 blocks each above K 32768.
+LONG = [
+    ((1, 0, 33280, (1024,)), "narrow 16x16", False),
+    ((1, 0, 131072, (4096,)), "narrow 16x16", False),
+    ((1, 1, 33040, (16384,)), "narrow 16x32", False),
+    ((20, 0, 33040, (4096,)), "narrow 32x16", False),
+    ((17, 0, 33040, (8192,)), "narrow 32x32", False),
+    ((1, 0, 33280, (264,)), "tiles 64x128", True),
+    ((300, 0, 131072, (264,)), "tiles 64x128", True),
+    ((5, 200, 40976, (512,)), "tiles 64x128", True),
+    ((128, 0, 33040, (8192,)), "tiles 128x128", True),
+    ((600, 0, 33040, (4096,)), "tiles 128x256", True),
+    ((0, 700, 33040, (2048,)), "tiles 192x256", True),
+    ((2048, 0, 33040, (8192,)), "tiles 256x256", False),
+]

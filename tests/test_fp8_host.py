@@ -144,3 +144,14 @@ def test_the_sizes_that_stand_for_the_kernels(host):
         assert (shares > 1) == split and (name[0] == "n" or (tiles > slots) == rounds), launch
         seen.add(build)
     assert seen == kernel_builds()
+
+
+def test_the_sizes_of_long_k(host):
+    """The narrow ones pass 64 blocks of K a wave, the tiles have both whole
+    rounds and shares."""
+    calls = ["gemm {} {} {} ".format(*size[:3]) + " ".join(map(str, size[3]))
+             for size, *_ in ref.LONG]
+    for (size, name, split), (launch, st) in zip(ref.LONG, host(calls)):
+        assert st == "ok" and launch.startswith(name + " "), (size, launch)
+        assert (parsed(launch)[3] > 1) == split, (size, launch)
+        assert ref.blocks(size[2]) > 4 * 64
