@@ -155,3 +155,29 @@ def test_the_sizes_of_long_k(host):
         assert st == "ok" and launch.startswith(name + " "), (size, launch)
         assert (parsed(launch)[3] > 1) == split, (size, launch)
         assert ref.blocks(size[2]) > 4 * 64
+
+
+def test_split_tails_are_partial_rounds(host):
+    """What is split is what whole rounds of workgroups leave, a round being what
+    the chip runs at once: on each unit as many tiles as its 160 KiB of LDS hold
+    (NS stages of a float for each of 64 rows or columns and of 128 codes a row
+    or column), at most eight multiplying waves."""
+    text = (CSRC / "u15h_fp8.hip").read_text()
+    rows = re.search(r"#define U15H_FP8_TILES\(X\)((?:.*\\\n)*.*)", text).group(1)
+    per_cu = {}
+    for row in re.findall(r"X\(([\d, ]+)\)", rows):
+        wm, wn, fj, fi, _, ns, _ = map(int, row.split(","))
+        bm, bn = 16 * wm * fj, 16 * wn * fi
+        scales = -(-ns * 4 * (-(-bm // 64) * 64 + 64) // 1024) * 1024
+        lds = scales + ns * 128 * (bm + bn)
+        per_cu["tiles", bm, bn] = max(min(160 * 1024 // lds, 8 // (wm * wn)), 1)
+    sized = ["gemm {} {} {} ".format(*size[:3]) + " ".join(map(str, size[3]))
+             for size, *_ in ref.KINDS + ref.LONG]
+    for cus in (256, 208):
+        calls, seen = random_gemms(1500) + sized, set()
+        for call, (launch, st) in zip(calls, host(calls, cus)):
+            build, tiles, tail, shares = parsed(launch)
+            if shares > 1:
+                assert tail == tiles % (cus * per_cu[build]), (call, launch)
+                seen.add(build)
+        assert seen == set(per_cu) or cus != 256

@@ -106,23 +106,22 @@ add_problem(Fp8Batch& b, const uint8_t* a, const float* sa, const uint8_t* w, co
 struct Kind {
   bool narrow;
   int bm, bn;
-  int per_cu;          // workgroups of tiles that a CU runs at once
   double fixed, round, stage, stream, split, part, weight, share;
 };
 constexpr Kind kKinds[] = {
-    {true, 16, 16, 0, 2.39, 0.50, 0.0502, 0.0471, 0, 0, 0, 0},
-    {true, 16, 32, 0, 1.97, 1.30, 0.0822, 0.1000, 0, 0, 0, 0},
-    {true, 32, 16, 0, 1.70, 1.48, 0.0698, 0.0466, 0, 0, 0, 0},
-    {true, 32, 32, 0, 2.42, 1.12, 0.1004, 0.0987, 0, 0, 0, 0},
-    {true, 64, 16, 0, 1.40, 1.97, 0.1184, 0.0536, 0, 0, 0, 0},
-    {true, 64, 32, 0, 2.95, 0.99, 0.1478, 0.1196, 0, 0, 0, 0},
-    {true, 96, 16, 0, 1.42, 2.11, 0.1672, 0.0479, 0, 0, 0, 0},
-    {true, 128, 16, 0, 1.38, 2.48, 0.2095, 0.0507, 0, 0, 0, 0},
-    {false, 64, 128, 2, 3.67, 0.34, 0.316, 0, 2.63, 0.335, 0.130, 0.164},
-    {false, 128, 128, 1, 3.09, 1.70, 0.426, 0, 2.69, 0.364, 0.100, 0.141},
-    {false, 128, 256, 1, 3.14, 2.63, 0.674, 0, 2.76, 0.284, 0.119, 0.165},
-    {false, 192, 256, 1, 5.86, 0.98, 1.093, 0, 2.67, 0.200, 0.144, 0.198},
-    {false, 256, 256, 1, 7.82, 0, 1.307, 0, 3.91, 0.117, 0.109, 0.235},
+    {true, 16, 16, 2.39, 0.50, 0.0502, 0.0471, 0, 0, 0, 0},
+    {true, 16, 32, 1.97, 1.30, 0.0822, 0.1000, 0, 0, 0, 0},
+    {true, 32, 16, 1.70, 1.48, 0.0698, 0.0466, 0, 0, 0, 0},
+    {true, 32, 32, 2.42, 1.12, 0.1004, 0.0987, 0, 0, 0, 0},
+    {true, 64, 16, 1.40, 1.97, 0.1184, 0.0536, 0, 0, 0, 0},
+    {true, 64, 32, 2.95, 0.99, 0.1478, 0.1196, 0, 0, 0, 0},
+    {true, 96, 16, 1.42, 2.11, 0.1672, 0.0479, 0, 0, 0, 0},
+    {true, 128, 16, 1.38, 2.48, 0.2095, 0.0507, 0, 0, 0, 0},
+    {false, 64, 128, 3.67, 0.34, 0.316, 0, 2.63, 0.335, 0.130, 0.164},
+    {false, 128, 128, 3.09, 1.70, 0.426, 0, 2.69, 0.364, 0.100, 0.141},
+    {false, 128, 256, 3.14, 2.63, 0.674, 0, 2.76, 0.284, 0.119, 0.165},
+    {false, 192, 256, 5.86, 0.98, 1.093, 0, 2.67, 0.200, 0.144, 0.198},
+    {false, 256, 256, 7.82, 0, 1.307, 0, 3.91, 0.117, 0.109, 0.235},
 };
 
 // Counts a batch's tiles on a kind and cuts its last partial round in `shares`
@@ -144,7 +143,7 @@ set_tiles(Fp8Batch& b, const Kind& k, int shares)
   }
   b.total_tiles = b.split_begin = (int)tiles;
   b.split = shares;
-  if (shares > 1) { b.split_begin -= b.total_tiles % (k.per_cu * b.cus); }
+  if (shares > 1) { b.split_begin -= b.total_tiles % (u15h::fp8_tiles_per_cu(k.bm, k.bn) * b.cus); }
   return true;
 }
 
@@ -184,7 +183,7 @@ plan(Fp8Batch& b, size_t workspace)
       consider(k, 1, k.fixed + load * (k.round + nb * k.stage) + (double)tiles * nb / C * k.stream);
       continue;
     }
-    const int two = k.per_cu, slots = two * C;
+    const int two = u15h::fp8_tiles_per_cu(k.bm, k.bn), slots = two * C;
     const long long full = tiles / slots, rem = tiles % slots;
     const double fixed = k.fixed + mb * k.weight + full * (k.round + nb * two * k.stage);
     if (best != nullptr && fixed >= least) { continue; }

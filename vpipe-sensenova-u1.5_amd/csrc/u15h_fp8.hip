@@ -1105,6 +1105,7 @@ tile_launch(const Fp8Batch& b, hipStream_t s)
   using L = Fp8Tile<WM, WN, FJ, FI, NS, LWV>;
   const int tail = b.total_tiles - b.split_begin;
   const int items = b.split_begin + tail * b.split;
+  static_assert(L::kPerCu == fp8_tiles_per_cu(L::BM, L::BN), "the plan's rounds are the grid's");
   fp8_tile_kernel<WM, WN, FJ, FI, FB, NS, LWV>
       <<<std::min(items, b.cus * L::kPerCu), 64 * L::kWaves, 0, s>>>(b);   // all at once
   if (b.split > 1 && tail > 0) {

@@ -295,6 +295,10 @@ struct Fp8Batch {
   int split;
   float* ws;
 };
+// Workgroups of a tile that a compute unit runs at once: what its LDS leaves
+// room for (the kernels assert it), and so the round that a plan counts in and
+// the persistent grid.
+constexpr int fp8_tiles_per_cu(int bm, int bn) { return bm * bn <= 64 * 128 ? 2 : 1; }
 hipError_t launch_fp8_gemm(const Fp8Batch& b, hipStream_t s);
 // Codes [rows][K] and scales [ceil(K / 128)][rows] of bf16 rows, or with `up`
 // of silu(x) * up, whose bf16 values go to h where that is not null.
