@@ -573,8 +573,10 @@ u15h_status u15h_quant_blocks_fp8(u15h_ctx* ctx, u15h_stream stream,
  *   q [rows][dim], s [KB][rows] = the codes and scales of n
  *   y [rows][dim] = bf16(n)                       (when y is not NULL)
  * The codes are those of the f32 values, rounded once (not of y).  x_out
- * may be x (the residual stream updated in place); delta and x_out are
- * given together or not at all; y must not be x_out.  dim <= 16384,
+ * may be x (the residual stream updated in place) or delta, y may be delta,
+ * and x where there is no delta; delta and x_out are given together or not
+ * at all; y must not be x_out.  A row whose squares add up past f32's range
+ * has inv 0 and comes out as zeros, as from u15h_rms_norm.  dim <= 16384,
  * eps >= 0. */
 u15h_status u15h_mot_rms_norm_fp8(u15h_ctx* ctx, u15h_stream stream,
                                   const u15h_bf16* x, const u15h_bf16* delta,
@@ -585,8 +587,8 @@ u15h_status u15h_mot_rms_norm_fp8(u15h_ctx* ctx, u15h_stream stream,
 
 /* The down projection's fp8 input in one pass: h = silu(gate) * up in f32,
  * its codes q [rows][inter] and scales s [ceil(inter / 128)][rows] (of the
- * f32 values, rounded once), and bf16(h) where h is not NULL.
- * inter <= 131072, rows <= 2^22. */
+ * f32 values, rounded once), and bf16(h) where h is not NULL; h may be gate
+ * or up.  inter <= 131072, rows <= 2^22. */
 u15h_status u15h_swiglu_quant_fp8(u15h_ctx* ctx, u15h_stream stream,
                                   const u15h_bf16* gate, const u15h_bf16* up,
                                   int rows, int inter, u15h_bf16* h,
@@ -608,7 +610,8 @@ typedef struct {
  * with b the blocks of K
  *   y[m][n] = bf16( sum_b (sx[b][m] * sw[n / 128][b]) *
  *                         sum_{k in b} xq[m][k] * wq[n][k] )
- * with f32 sums.  xq [M][K], sx [KB][M] over the rows of both groups.
+ * with f32 sums, and the product of the two scales in f32 as well.  xq
+ * [M][K], sx [KB][M] over the rows of both groups.
  * Precision: the matrix unit multiplies e4m3 codes exactly, but of the 8
  * products of 8 neighbouring k it keeps each only down to 2^-13 of the
  * binary order of the largest (a rule of the hardware).  So such a group is
