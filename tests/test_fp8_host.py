@@ -181,3 +181,17 @@ def test_split_tails_are_partial_rounds(host):
                 assert tail == tiles % (cus * per_cu[build]), (call, launch)
                 seen.add(build)
         assert seen == set(per_cu) or cus != 256
+
+
+def test_loaders_refuse_codes(tmp_path):
+    """e4m3 tensors of a checkpoint are the caller's to load: the loaders of the
+    other tiers say so and convert nothing."""
+    import torch
+    from safetensors.torch import save_file
+
+    import u15h
+    path = tmp_path / "w.safetensors"
+    save_file({"p.weight": torch.zeros(8, 128, dtype=torch.float8_e4m3fn)}, str(path))
+    with pytest.raises(u15h.U15hError) as err:
+        u15h.load_matrix(None, path, "p", 128)
+    assert err.value.status == u15h.EINVAL and "float8_e4m3fn" in str(err.value)

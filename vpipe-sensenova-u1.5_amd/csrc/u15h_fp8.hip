@@ -170,13 +170,13 @@ swiglu8(float (&v)[8], const float (&u)[8])
 // operand, or a row of two).  The scales of the workgroup's rows are gathered
 // in LDS and written as runs of 4 RPW.
 // Bound by memory: 2 bytes read (4 for SwiGLU) and 1 + 1/32 written per value.
-// Workgroups walk a row's columns first, so those that run together read whole
-// rows: 4224 rows of 12288 take 27.5 us (5.7 TB/s; SwiGLU 47 us, 5.6 TB/s)
-// against 33.5 (53) walking the rows first.  The operands are read once and
-// for the last time, so past the caches' other lines (non-temporal): 1.0 (1.2)
-// us of it.  The codes are stored plainly: stored past the caches these take 2
-// us less and the product that reads them 2 more.  Four rows of 4096: 2.0 us,
-// a launch.
+// 4224 rows of 12288 take 26 us (6.0 TB/s; SwiGLU 43 us, 6.1 TB/s, with h 62
+// us, 5.9 TB/s), four rows of 4096 2.3 us, a launch.  Workgroups walk a row's
+// columns first, so those that run together read whole rows: walking the rows
+// first takes a fifth more time (SwiGLU an eighth).  The operands are read once
+// and for the last time, so past the caches' other lines (non-temporal): 1.0
+// (1.2) us of it.  The codes are stored plainly: stored past the caches these
+// take 2 us less and the product that reads them 2 more.
 template <bool SWIGLU, int RPW>
 __global__ __launch_bounds__(256) void
 fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ up, int rows,
@@ -237,9 +237,9 @@ fp8_quant_rows_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict
 // ---- weights: a scale per 128 x 128 ------------------------------------------
 // One workgroup of four waves per block; a wave reads four rows' 256 bytes at a
 // time (lane l: row l / 16, columns 8 (l % 16)..), eight such reads in flight.
-// Bound by memory: 3 bytes per value, 12288 x 4096 in 27.7 us (5.5 TB/s).  A
+// Bound by memory: 3 bytes per value, 12288 x 4096 in 26.4 us (5.7 TB/s).  A
 // weight is read once and its codes wait for a later use, so both go past the
-// caches' other lines (non-temporal); plainly it is 30.4 us.
+// caches' other lines (non-temporal); plainly it takes a tenth more.
 __global__ __launch_bounds__(256) void
 fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* __restrict__ q,
                         float* __restrict__ sc)
@@ -292,13 +292,16 @@ fp8_quant_blocks_kernel(const uint16_t* __restrict__ w, int N, int K, uint8_t* _
 //   by xor shuffles, the row through LDS.
 // The codes are those of n itself, rounded once; y, where wanted, is bf16(n).
 // Every store of a row follows all of its loads, so x_out may be x.
-// Bound by memory: with the add 7 bytes per value (5 in, out 2 and the codes),
-// 4224 rows of 4096 in 23.7 us (5.1 TB/s); without it 3 bytes, 13.8 us (3.8
-// TB/s).  x, d and r go past the caches' other lines (non-temporal): d is read
-// for the last time and x's or r's next reader is half a layer away; plainly 25.4
-// and 15.1 us.  A row of 4096 has eight waves with the add, two loads each as
-// it has with four waves without it: eight against four take 2.3 against 2.4 us
-// for one row and 23 to 24 both for 4224 with the add, 15.1 against 13.8 without.
+// Bound by memory: with the add 7 bytes per value (4 in, 2 and the code out),
+// 4224 rows of 4096 in 22.5 us (5.4 TB/s; with y too 26.9 us, 5.8 TB/s);
+// without it 3 bytes, 13.3 us (3.9 TB/s; with y 18.3 us, 4.8 TB/s).  Each row's
+// workgroup also reads the weights from L2, as many bytes as its row: with them
+// the four forms move 6.5 to 7.1 TB/s.  x, d and r go past the caches' other
+// lines (non-temporal): d is read for the last time and x's or r's next reader
+// is half a layer away; plainly each takes a twelfth more.  A row
+// of 4096 has eight waves with the add, two loads each as it has with four waves
+// without it: eight against four are level with the add (one row and 4224) and a
+// tenth slower without.
 template <int WPR, int CPL, bool ADD>
 __global__ __launch_bounds__(64 * WPR) void
 fp8_norm_kernel(const Fp8NormArgs A)
@@ -481,7 +484,7 @@ struct Fp8Tile {
 // of the LDS reads that 256 x 32 makes) gained 5%.  Products and
 // multiply-adds alone, from registers, reach 3.7 to 4.0 PFLOP/s; 4096 rows of
 // K 12288 and 4096 columns run at 2.35 (175 us), 4224 rows of two times 12288
-// columns at 2.07 (412 us).
+// columns at 2.1 (400 us).
 // The smaller tiles have few products a stage to hide its barrier, reads and
 // loads behind, so they have more places (NS), their weights' fragments a stage
 // ahead where registers allow, and four waves that load for four that multiply
@@ -534,7 +537,7 @@ fp8_tiles(const Fp8Batch& B, char* lds)
   };
 
   // ---- loads ---------------------------------------------------------------
-  // What the loads of the stage two ahead need, stepped along with the stages;
+  // What the loads of the stage NS ahead need, stepped along with the stages;
   // past the last item they fetch its last block again, for nobody.
   struct {
     __amdgpu_buffer_rsrc_t a, w;
