@@ -371,6 +371,153 @@ u15h_status u15h_transpose_into_cache(u15h_ctx* ctx, u15h_stream stream,
                                       int offset);
 
 /* ------------------------------------------------------------------ */
+/* Many requests at once: rotary positions, the paged cache, attention  */
+/* behind a shared prefix                                               */
+/* ------------------------------------------------------------------ */
+
+/* A rotation of the columns of a head by the token's position.  Part p turns
+ * columns [start, start + width) by the position on its axis: pair i of the
+ * width / 2 is columns (start + i, start + i + width / 2), or with
+ * `neighbours` (start + 2 i, start + 2 i + 1), and
+ *   angle = pos * freq[i]                                (in 64 bits)
+ *   y_a = x_a cos - x_b sin,  y_b = x_b cos + x_a sin     (in f32, rounded once)
+ * with cos and sin times `scale`.  Columns in no part are passed on as they
+ * are.  One part of the whole head is ordinary RoPE; three with axes of their
+ * own are the model's t | h | w (u15h_split_rope, whose f32 tables this does
+ * without: the angle is formed here, so any position has the same precision).
+ * Parts do not overlap; width is even. */
+#define U15H_MAX_ROPE_PARTS 3
+typedef struct {
+  const double* freq;    /* device, [width / 2] radians per position          */
+  int           start;
+  int           width;
+  int           axis;    /* row of the positions, 0 <= axis < MAX_ROPE_PARTS  */
+} u15h_rope_part;
+typedef struct {
+  u15h_rope_part part[U15H_MAX_ROPE_PARTS];
+  int            nparts;      /* 1 .. U15H_MAX_ROPE_PARTS                     */
+  int            neighbours;  /* pairs: 0 the halves, 1 neighbouring columns  */
+  float          scale;       /* of cos and sin (1 where nothing is scaled)   */
+} u15h_rope_spec;
+
+/* How frequencies are scaled for contexts past the trained one. */
+typedef enum {
+  U15H_ROPE_PLAIN  = 0,  /* f_i = theta^(-2 i / width)                        */
+  U15H_ROPE_LINEAR = 1,  /* f_i / factor: positions squeezed                  */
+  U15H_ROPE_NTK    = 2,  /* theta * factor^(width / (width - 2)) as the base  */
+  U15H_ROPE_YARN   = 3,  /* f_i / factor for pairs that turn less than `slow`
+                            times within `trained` positions, f_i for those
+                            that turn more than `fast` times, a ramp over the
+                            pair's number between; *scale = 0.1 ln(factor) + 1 */
+  U15H_ROPE_BANDS  = 4   /* the same with the ramp over the number of turns   */
+} u15h_rope_scaling;
+
+/* Fills freq[width / 2] (HOST memory) and *scale for one part.  HOST function,
+ * no context; the caller copies freq to the device.  factor, trained, slow and
+ * fast are read where the scaling names them: factor >= 1, trained > 0,
+ * 0 < slow < fast (YaRN's are 1 and 32).  theta > 1, width even and
+ * <= 512. */
+u15h_status u15h_rope_freqs(int width, double theta, int scaling, double factor,
+                            double trained, double slow, double fast,
+                            double* freq, float* scale);
+
+/* y = x turned: x, y [tokens] x [heads] x [head_dim] bf16, token t's head h at
+ * t * tok + h * head elements (token-major and head-major, and column ranges
+ * of wider matrices alike).  pos: device int32 [axes][tokens], any values.
+ * With `inverse` the angle is taken negative, which is also the gradient: of
+ * y = rope(x), dx = inverse rope(dy).  y may be x with equal strides; else
+ * they must not overlap, and neither may heads or tokens within y.
+ * Limits: head_dim <= 512, heads <= 4096, strides >= 0.  Pointers 2-byte
+ * aligned, as an exception; parts, strides and pointers that are multiples of
+ * 8 elements (16 bytes) take the wide loads. */
+u15h_status u15h_rope(u15h_ctx* ctx, u15h_stream stream,
+                      const u15h_rope_spec* rope, const int32_t* pos,
+                      const u15h_bf16* x, int64_t x_tok, int64_t x_head,
+                      u15h_bf16* y, int64_t y_tok, int64_t y_head, int tokens,
+                      int heads, int head_dim, int inverse);
+
+/* A paged K/V cache (one layer's): page p's head h holds `page` slots of
+ * head_dim, k and v at p * page_stride + (h * page + slot) * head_dim.  So a
+ * page is a small cache of u15h_sdpa's layout, k and v may be halves of one
+ * allocation, and a page of a whole context is a contiguous cache.
+ * Limits: page a power of two in [16, 2^20], head_dim 32, 64 or 128,
+ * page_stride >= kv_heads * page * head_dim and a multiple of 8,
+ * pages * page < 2^31; pointers 16-byte aligned. */
+typedef struct {
+  u15h_bf16* k;
+  u15h_bf16* v;
+  int64_t    page_stride;   /* elements; 0: kv_heads * page * head_dim        */
+  int        pages;
+  int        page;          /* slots of a page                                */
+  int        kv_heads;
+  int        head_dim;
+} u15h_paged_kv;
+
+/* A step's keys and values into the cache, in one launch with the rotation:
+ *   cache k[slot[t]] <- rope(k[t]),  cache v[slot[t]] <- v[t]
+ *   q_out[t]         <- rope(q[t])                 (where q is not NULL)
+ * slot: device int32 [tokens], page * kv->page + place within it, distinct.  A
+ * token whose slot is outside the cache (-1, say) is passed over: nothing of
+ * it is written, q_out neither.  k and v are [tokens][kv_heads * head_dim], q
+ * and q_out [tokens][hq * head_dim], rows *_stride elements apart (multiples
+ * of 8), so all three may be columns of one product.  rope NULL: nothing is
+ * turned (q must be NULL).  q_out may be q.  pos as u15h_rope's.  The
+ * counterpart of split_rope and transpose_into_cache
+ * (src/u15-backbone.cc:205-216) for many requests. */
+u15h_status u15h_paged_append(u15h_ctx* ctx, u15h_stream stream,
+                              const u15h_paged_kv* kv, const int32_t* slot,
+                              const u15h_rope_spec* rope, const int32_t* pos,
+                              const u15h_bf16* k, int64_t k_stride,
+                              const u15h_bf16* v, int64_t v_stride,
+                              const u15h_bf16* q, int64_t q_stride,
+                              u15h_bf16* q_out, int64_t q_out_stride, int hq,
+                              int tokens);
+
+/* A step's batch: `batch` sequences whose keys are the first prefix_len of the
+ * pages in prefix_table, the same for all, and then the first kv_len[b] of the
+ * pages in row b of table.  Sequence b's queries are rows
+ * [q_start[b], q_start[b + 1]) of q, ascending; q_start NULL: one row each.
+ * kv_len counts the step's own keys (append first); with the causal mask,
+ * query i of n sees the prefix and the own keys [0, kv_len - n + i].
+ * The lengths are device memory and may change between replays of a captured
+ * graph; max_q and max_kv bound them on the host and choose the launches.
+ * What is out of bounds is not read: kv_len counts as at most max_kv and
+ * table_stride pages, a sequence as at most max_q queries within `tokens`
+ * rows, and a page number outside the cache as a page whose keys are masked. */
+typedef struct {
+  int            batch;
+  int            tokens;        /* rows of q and out                          */
+  int            max_q;
+  int            max_kv;
+  const int32_t* q_start;       /* [batch + 1] or NULL                        */
+  const int32_t* kv_len;        /* [batch]                                    */
+  const int32_t* table;         /* [batch][table_stride] page numbers         */
+  int            table_stride;
+  const int32_t* prefix_table;  /* [ceil(prefix_len / page)]                  */
+  int            prefix_len;    /* 0: none                                    */
+} u15h_paged_batch;
+
+/* out = softmax(q . k * scale) . v over the paged cache, for every row of
+ * every sequence; u15h_attention_token_major for many requests.  q, out
+ * [tokens][hq * head_dim] bf16, rows *_stride elements apart (multiples of 8);
+ * query head h reads kv head h / (hq / kv_heads); scale 0 stands for
+ * 1 / sqrt(head_dim); causal 0: every query sees all keys.  A query that sees
+ * no key gets zeros; rows of no sequence are left as they are.  out may not
+ * overlap q.
+ * The prefix is walked once for the whole batch where that is less work: its
+ * keys meet all sequences' queries as one matrix, and the sequences' own keys
+ * join through partial results in the context's attention scratch (u15h_sdpa;
+ * without it every sequence walks the prefix itself).
+ * Limits: hq % kv_heads == 0, hq <= 4096, batch <= 65536, tokens <= 2^22,
+ * max_kv and prefix_len < 2^30. */
+u15h_status u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream,
+                                 const u15h_paged_kv* kv,
+                                 const u15h_paged_batch* batch,
+                                 const u15h_bf16* q, int64_t q_stride,
+                                 u15h_bf16* out, int64_t out_stride, int hq,
+                                 float scale, int causal);
+
+/* ------------------------------------------------------------------ */
 /* The layer norms and the residual add (either side of the projections) */
 /* ------------------------------------------------------------------ */
 

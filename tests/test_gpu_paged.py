@@ -1,0 +1,441 @@
+"""Many requests at once on the GPU: rotary positions, the paged cache and
+attention behind a shared prefix, one by one and as a step calls them, against
+the definition in 64 bits on the host (tests/paged_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import paged_ref as ref
+import u15h
+
+pytestmark = pytest.mark.gpu
+
+BF16, I32, F64 = torch.bfloat16, torch.int32, torch.float64
+
+
+def bf16(seed, *shape, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(BF16)
+
+
+def bits(t):
+    return t.contiguous().view(torch.int16)
+
+
+# ---- rotary positions ---------------------------------------------------------
+
+def rotation(parts, neighbours=False, scaling="none", theta=(5e6, 1e4, 1e4)):
+    """(Rope, host parts, scale) of [(start, width, axis)]."""
+    host, scale = [], 1.0
+    for start, width, axis in parts:
+        f, sc = u15h.rope_freqs(width, theta[axis], scaling, factor=8.0, trained=4096)
+        host.append((f, start, axis))
+        scale = max(scale, sc)
+    return u15h.Rope([(f.cuda(), s, a) for f, s, a in host], neighbours, scale), host, scale
+
+
+def positions(seed, axes, tokens, most):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-most, most, (axes, tokens), generator=g).to(I32)
+
+
+ROPES = [
+    # tokens, heads, d, parts, neighbours, scaling
+    (1, 32, 128, [(0, 128, 0)], False, "none"),
+    (1, 1, 2, [(0, 2, 0)], True, "none"),
+    (3, 5, 16, [(0, 16, 0)], False, "linear"),          # one access unit a head
+    (7, 8, 128, [(0, 64, 0), (64, 32, 1), (96, 32, 2)], False, "yarn"),
+    (7, 3, 128, [(96, 32, 2), (0, 64, 0)], True, "bands"),
+    (33, 5, 96, [(8, 54, 0)], False, "ntk"),            # 27 pairs: single columns
+    (33, 5, 96, [(8, 52, 0)], False, "none"),           # 26: two columns
+    (33, 2, 80, [(0, 20, 0)], True, "none"),
+    (5, 2, 33, [(1, 6, 0), (9, 24, 1)], False, "none"),  # odd heads and starts
+    (5, 2, 33, [(1, 6, 0), (9, 24, 1)], True, "none"),
+    (1030, 2, 64, [(0, 64, 0)], False, "yarn"),         # groups of tokens, the last short
+    (1027, 1, 512, [(0, 512, 0)], True, "none"),
+    (2049, 3, 32, [(0, 16, 1)], False, "none"),
+]
+
+
+@pytest.mark.parametrize("tokens,heads,d,parts,neighbours,scaling", ROPES)
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rope(ops, tokens, heads, d, parts, neighbours, scaling, inverse):
+    rope, host, scale = rotation(parts, neighbours, scaling)
+    x = bf16(tokens + d, tokens, heads, d, std=2.0)
+    pos = positions(tokens, 3, tokens, 1 << 22)
+    y = torch.full((tokens, heads, d), math.nan, dtype=BF16, device="cuda")
+    ops.rope(x.cuda(), pos.cuda(), rope, y, inverse=inverse)
+    want, off = ref.turn(x, pos, host, neighbours, scale, inverse)
+    assert bool(((y.cpu().to(F64) - want).abs() <= off).all())
+
+
+def test_rope_far_positions(ops):
+    """The whole range of positions, with the fastest frequency."""
+    rope, host, _ = rotation([(0, 128, 0)])
+    pos = torch.tensor([[0, 1, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 30 + 1, 123456789]], dtype=I32)
+    x = bf16(1, 7, 4, 128)
+    y = torch.empty(7, 4, 128, dtype=BF16, device="cuda")
+    ops.rope(x.cuda(), pos.cuda(), rope, y)
+    want, off = ref.turn(x, pos, host)
+    assert bool(((y.cpu().to(F64) - want).abs() <= off).all())
+    assert torch.equal(bits(y[0].cpu()), bits(x[0]))
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2])
+@pytest.mark.parametrize("layout", ["columns", "head_major", "in_place"])
+def test_rope_strides(ops, layout, offset):
+    """Columns of a wider matrix, [heads][tokens][d], x itself; addresses that
+    keep whole, pairs of and single columns together.  The rest stays."""
+    T, H, d = 9, 3, 64
+    rope, host, _ = rotation([(0, 64, 0)])
+    pos = positions(3, 1, T, 1000)
+    whole = bf16(5, 4096).cuda()
+    before = whole.clone()
+    if layout == "head_major":
+        x = whole[offset:offset + T * H * d].view(H, T, d).transpose(0, 1)
+    else:
+        pitch = H * d + (16 if offset == 0 else offset)
+        x = torch.as_strided(whole, (T, H, d), (pitch, d, 1), offset)
+    xh = x.cpu()
+    out = torch.full((4096,), 7.0, dtype=BF16, device="cuda")
+    y = x if layout == "in_place" else torch.as_strided(out, x.shape, x.stride(), offset)
+    ops.rope(x, pos.cuda(), rope, y)
+    want, off = ref.turn(xh, pos, host)
+    assert bool(((y.cpu().to(F64) - want).abs() <= off).all())
+    touched = torch.zeros(4096, dtype=torch.bool)
+    torch.as_strided(touched, x.shape, x.stride(), offset).fill_(True)
+    rest = whole if layout == "in_place" else out
+    same = before if layout == "in_place" else torch.full_like(out, 7.0)
+    assert torch.equal(bits(rest)[~touched.cuda()], bits(same)[~touched.cuda()])
+
+
+def test_rope_gradient(ops):
+    """The inverse is the gradient: <dy, rope(x)> moves with x as <inverse
+    rope(dy), .> says, by differences of the definition and by the formula."""
+    T, H, d = 5, 2, 32
+    rope, host, scale = rotation([(0, 24, 0)], True, "yarn")
+    pos = positions(8, 1, T, 5000)
+    x, dy = bf16(1, T, H, d), bf16(2, T, H, d)
+    dx = torch.empty(T, H, d, dtype=BF16, device="cuda")
+    ops.rope(dy.cuda(), pos.cuda(), rope, dx, inverse=True)
+    leaf = x.to(F64).requires_grad_()
+    angle = pos[0].to(F64)[:, None] * host[0][0]
+    c, s = (torch.cos(angle) * scale)[:, None], (torch.sin(angle) * scale)[:, None]
+    a, b = leaf[..., 0:24:2], leaf[..., 1:24:2]
+    y = torch.cat([torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2), leaf[..., 24:]], -1)
+    (y * dy.to(F64)).sum().backward()
+    _, off = ref.turn(dy, pos, host, True, scale, True)
+    assert bool(((dx.cpu().to(F64) - leaf.grad).abs() <= off).all())
+    step = 2.0 ** -10
+    for at in [(0, 0, 0), (2, 1, 7), (4, 0, 23), (3, 1, 30)]:
+        moved = x.to(F64).clone()
+        moved[at] += step
+        up, _ = ref.turn(moved, pos, host, True, scale)
+        down, _ = ref.turn(x, pos, host, True, scale)
+        slope = ((up - down) * dy.to(F64)).sum() / step
+        assert abs(float(dx[at]) - float(slope)) <= float(off[at]) + 1e-9
+
+
+# ---- appending ----------------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,hq,hkv,d,page", [(1, 32, 8, 128, 16), (67, 6, 2, 64, 32),
+                                                  (1030, 4, 4, 32, 256), (40, 0, 1, 128, 16)])
+@pytest.mark.parametrize("parts", ["whole", "axes", "odd", None])
+def test_append(ops, tokens, hq, hkv, d, page, parts):
+    """Keys, values and queries from columns of one matrix into slots in any
+    order, padding passed over; every other slot keeps its bits."""
+    spec = {"whole": [(0, d, 0)], "axes": [(0, d // 2, 0), (d // 2, d // 4, 1),
+                                           (3 * d // 4, d // 4, 2)], "odd": [(1, 14, 0)]}
+    turned = parts is not None
+    hq = hq if turned else 0
+    rope, host, scale = rotation(spec[parts], parts == "odd") if turned else (None, [], 1.0)
+    qkv = bf16(tokens, tokens, hq + 2 * hkv, d)
+    dev = qkv.cuda()
+    pos = positions(2, 3, tokens, 100000)
+    pages = -(-tokens // page) + 2
+    both = bf16(9, pages, 2, hkv, page, d).cuda()          # k and v in one allocation
+    kv = u15h.PagedKV(both[:, 0], both[:, 1])
+    before = both.cpu()
+    slot = torch.randperm(pages * page, generator=torch.Generator().manual_seed(3))[:tokens]
+    slot[5::7] = -1
+    if tokens > 30:
+        slot[11], slot[12], slot[13] = pages * page, 2 ** 31 - 1, -2 ** 31
+    live = (slot >= 0) & (slot < pages * page)
+    q_out = torch.full((tokens, max(hq, 1), d), 3.0, dtype=BF16, device="cuda")
+    ops.paged_append(kv, dev[:, hq:hq + hkv], dev[:, hq + hkv:], slot.to(I32).cuda(),
+                     pos=pos.cuda() if turned else None, rope=rope, q=dev[:, :hq] if hq else None,
+                     q_out=q_out if hq else None)
+    after = both.cpu()
+    k, koff = ref.turn(qkv[:, hq:hq + hkv], pos, host, parts == "odd", scale)
+    p, o = slot[live] // page, slot[live] % page
+    got = after[p, 0, :, o].to(F64)
+    assert bool(((got - k[live]).abs() <= koff[live]).all())
+    assert torch.equal(bits(after[p, 1, :, o]), bits(qkv[live][:, hq + hkv:]))
+    rest = torch.ones(pages, page, dtype=torch.bool)
+    rest[p, o] = False
+    i, j = rest.nonzero(as_tuple=True)
+    assert torch.equal(bits(after[i, :, :, j]), bits(before[i, :, :, j]))
+    if hq:
+        want, off = ref.turn(qkv[:, :hq], pos, host, parts == "odd", scale)
+        out = q_out.cpu()
+        assert bool(((out.to(F64) - want).abs() <= off)[live].all())
+        assert bool((out[~live] == 3.0).all())
+
+
+def test_append_in_place(ops):
+    """Queries turned where they are, padding's rows left."""
+    T, H, d = 21, 4, 64
+    rope, host, _ = rotation([(0, 64, 0)])
+    q, kvr = bf16(1, T, H, d), bf16(2, T, 2, d)
+    pos = positions(4, 1, T, 5000)
+    slot = torch.arange(T)
+    slot[-4:] = -1
+    pool = torch.zeros(2, 2, 1, 16, d, dtype=BF16, device="cuda")
+    kv = u15h.PagedKV(pool[:, 0], pool[:, 1])
+    qd = q.cuda()
+    ops.paged_append(kv, kvr.cuda()[:, :1], kvr.cuda()[:, 1:], slot.to(I32).cuda(), pos.cuda(),
+                     rope, q=qd, q_out=qd)
+    want, off = ref.turn(q, pos, host)
+    assert bool(((qd.cpu().to(F64) - want).abs() <= off)[:-4].all())
+    assert torch.equal(bits(qd[-4:].cpu()), bits(q[-4:]))
+
+
+# ---- attention ----------------------------------------------------------------
+
+class Case:
+    """A paged cache with NaN wherever no key lies, a batch over it, queries."""
+
+    def __init__(self, lens, counts, prefix, hq, hkv, d, page, seed=0, pad=2, std=1.5, spare=2,
+                 stride=0):
+        g = torch.Generator().manual_seed(seed)
+        self.lens, self.counts, self.prefix, self.page = lens, counts, prefix, page
+        first = -(-prefix // page)
+        each = [-(-n // page) for n in lens]
+        pages = first + sum(each) + spare
+        order = torch.randperm(pages, generator=g)
+        shape = (pages, hkv, page, d)
+        self.kp = torch.full(shape, math.nan, dtype=BF16)
+        self.vp = torch.full(shape, math.nan, dtype=BF16)
+        self.prefix_table = order[:first].to(I32)
+        width = max(each + [1]) + stride
+        # entries past a sequence's pages are never read
+        self.table = torch.full((len(lens), width), 2 ** 31 - 1, dtype=I32)
+        at = first
+        for b, n in enumerate(each):
+            self.table[b, :n] = order[at:at + n].to(I32)
+            at += n
+        for table, n in [(self.prefix_table, prefix)] + [(t, n) for t, n in
+                                                         zip(self.table, lens)]:
+            for i in range(-(-n // page)):
+                k = min(page, n - i * page)
+                for pool in (self.kp, self.vp):
+                    pool[int(table[i]), :, :k] = torch.randn(hkv, k, d, generator=g).to(BF16)
+        self.rows = sum(counts)
+        self.q = (torch.randn(self.rows + pad, hq, d, generator=g) * std).to(BF16)
+        start = [0]
+        for c in counts:
+            start.append(start[-1] + c)
+        self.q_start = torch.tensor(start, dtype=I32)
+
+    def batch(self, max_q=None, max_kv=None, own_rows=True):
+        some = own_rows or any(c != 1 for c in self.counts)
+        return u15h.PagedBatch(torch.tensor(self.lens, dtype=I32).cuda(), self.table.cuda(),
+                               q_start=self.q_start.cuda() if some else None,
+                               max_q=max_q or max(self.counts + [1]),
+                               max_kv=max_kv, prefix_table=self.prefix_table.cuda(),
+                               prefix_len=self.prefix)
+
+    def run(self, ops, causal, scale=0.0, batch=None, pad_q=0, pad_out=0, stream=None):
+        """out [rows + pad][hq][d], guarded by rows of a wider matrix."""
+        n, hq, d = self.q.shape
+        kv = u15h.PagedKV(self.kp.cuda(), self.vp.cuda())
+        wide = torch.full((n, hq + 1, d), 5.0, dtype=BF16, device="cuda")
+        qw = torch.full((n, hq + pad_q, d), math.nan, dtype=BF16, device="cuda")
+        qw[:, :hq] = self.q.cuda()
+        ops.paged_attention(kv, batch or self.batch(), qw[:, :hq], wide[:, :hq], scale=scale,
+                            causal=causal, stream=stream)
+        host = wide.cpu()
+        assert bool((host[:, hq] == 5.0).all()), "beside the rows"
+        assert bool((host[self.rows:] == 5.0).all()), "rows of no sequence"
+        return host[:self.rows, :hq]
+
+    def want(self, causal, scale=0.0):
+        return ref.attend(self.q[:self.rows], self.kp, self.vp, self.prefix_table, self.prefix,
+                          self.table, self.lens, self.counts, causal, scale)
+
+
+def check(out, want):
+    o, bound = want
+    diff = (out.to(F64) - o).abs()
+    assert not bool(torch.isnan(diff).any())
+    worst = (diff / bound.clamp(min=1e-38)).max() if diff.numel() else torch.zeros(())
+    assert float(worst) <= 1.0, float(worst)
+
+
+HEADS = [(32, 8, 128), (4, 4, 64), (6, 2, 32), (10, 1, 128), (24, 1, 64), (70, 2, 32)]
+BATCHES = {
+    "one": ([1], [1]),
+    "tile_edges": ([15, 16, 17, 31, 32, 33], [1] * 6),
+    "none": ([0, 3, 0], [1, 0, 1]),
+    "more_queries_than_keys": ([5, 40], [9, 60]),
+    "drafts": ([5, 77, 130, 64], [5, 5, 4, 3]),
+    "chunks": ([130, 257, 1, 64, 300], [130, 33, 1, 64, 2]),
+    "long": ([1500], [1]),
+}
+
+
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+@pytest.mark.parametrize("name", list(BATCHES))
+@pytest.mark.parametrize("prefix,page,causal", [(0, 16, True), (33, 16, True), (100, 64, False),
+                                                (1, 32, True), (513, 16, False)])
+def test_attention(ops, hq, hkv, d, name, prefix, page, causal):
+    lens, counts = BATCHES[name]
+    c = Case(lens, counts, prefix, hq, hkv, d, page, seed=prefix + hq)
+    check(c.run(ops, causal), c.want(causal))
+
+
+@pytest.mark.parametrize("batch,prefix", [(40, 700), (100, 64), (17, 2000), (3, 1000)])
+def test_attention_decode(ops, batch, prefix):
+    """Many sequences of one query behind a shared prefix."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(1, 300, (batch,), generator=g).tolist()
+    c = Case(lens, [1] * batch, prefix, 8, 2, 128, 16, seed=batch)
+    out = c.run(ops, True)
+    check(out, c.want(True))
+    alone = c.run(ops, True, batch=c.batch(own_rows=False))
+    assert torch.equal(bits(alone), bits(out))            # one row each, said or not
+    assert torch.equal(bits(c.run(ops, False)), bits(out))    # and no key is ahead
+
+
+@pytest.mark.parametrize("count,prefix", [(200, 0), (300, 77), (129, 600)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_long_queries(ops, count, prefix, causal):
+    c = Case([count + 40, count], [count, count - 1], prefix, 8, 2, 128, 64, seed=count)
+    check(c.run(ops, causal), c.want(causal))
+
+
+def test_attention_scale_and_peaks(ops):
+    """A scale of one's own; scores far apart, so one key has all the weight."""
+    c = Case([50, 700], [3, 3], 300, 8, 2, 64, 16, std=12.0)
+    check(c.run(ops, True, scale=0.7), c.want(True, 0.7))
+    check(c.run(ops, True, scale=1e-3), c.want(True, 1e-3))
+
+
+def test_attention_rows_of_wider_matrices(ops):
+    c = Case([50, 70], [2, 1], 40, 8, 2, 128, 16)
+    plain = c.run(ops, True)
+    check(plain, c.want(True))
+    assert torch.equal(bits(c.run(ops, True, pad_q=3)), bits(plain))
+
+
+def test_attention_bad_pages(ops):
+    """Page numbers outside the cache, in the prefix and among own pages: their
+    keys are masked, and a row that is left with none gets zeros."""
+    c = Case([100, 40, 20], [2, 1, 1], 90, 8, 2, 128, 16)
+    c.table[0, 1], c.table[0, 4] = -1, 2 ** 31 - 1
+    c.table[1, :3] = torch.tensor([-2 ** 31, c.kp.shape[0], -5], dtype=I32)
+    c.prefix_table[2] = c.kp.shape[0]
+    check(c.run(ops, True), c.want(True))
+    c = Case([100, 40, 20], [2, 1, 1], 0, 8, 2, 128, 16)
+    c.table[1, :3] = -1
+    out = c.run(ops, True)
+    check(out, c.want(True))
+    assert bool((out[2] == 0).all())
+
+
+def test_attention_keeps_to_its_bounds(ops):
+    """Lengths and starts past max_kv, max_q and the rows count as those."""
+    c = Case([64, 64, 64], [4, 4, 4], 20, 4, 2, 64, 16)
+    lens = torch.tensor([1000, 64, -7], dtype=I32).cuda()
+    start = torch.tensor([-3, 4, 8, 100], dtype=I32).cuda()
+    kv = u15h.PagedKV(c.kp.cuda(), c.vp.cuda())
+    b = u15h.PagedBatch(lens, c.table.cuda(), q_start=start, max_q=4, max_kv=64,
+                        prefix_table=c.prefix_table.cuda(), prefix_len=20)
+    q = c.q.cuda()
+    out = torch.full_like(q, 5.0)
+    ops.paged_attention(kv, b, q, out, causal=False)
+    c.lens = [64, 64, 0]
+    check(out[:12].cpu(), c.want(False))
+    assert bool((out[12:] == 5.0).all())
+
+
+def test_attention_page_stride_and_offsets(ops):
+    """k and v in one allocation whose later pages lie past 2^31 elements."""
+    pages, hkv, page, d = 5, 1, 16, 64
+    stride = (1 << 29) + 8
+    whole = torch.zeros(4 * stride + 2 * hkv * page * d, dtype=BF16, device="cuda")
+    size = (pages, hkv, page, d)
+    k = torch.as_strided(whole, size, (stride, page * d, d, 1))
+    v = torch.as_strided(whole, size, (stride, page * d, d, 1), hkv * page * d)
+    c = Case([70], [1], 0, 4, 1, 64, 16, spare=0)
+    k.copy_(c.kp.cuda())
+    v.copy_(c.vp.cuda())
+    out = torch.empty(1, 4, 64, dtype=BF16, device="cuda")
+    ops.paged_attention(u15h.PagedKV(k, v), c.batch(), c.q[:1].cuda(), out)
+    check(out.cpu(), c.want(True))
+
+
+# ---- a step -------------------------------------------------------------------
+
+def test_step_with_the_layer_s_operators(ops):
+    """Three requests behind one prompt, two steps: append the prompt, then
+    each step's keys, and attend; against u15h_sdpa's caches of each request,
+    and against 64 bits."""
+    hq, hkv, d, page, P = 8, 2, 64, 16, 40
+    rope, host, _ = rotation([(0, 64, 0)])
+    pool = torch.zeros(12, 2, hkv, page, d, dtype=BF16, device="cuda")
+    kv = u15h.PagedKV(pool[:, 0], pool[:, 1])
+    prompt = bf16(1, P, 2 * hkv, d)
+    ppos = torch.arange(P, dtype=I32)[None]
+    prefix_table = torch.tensor([7, 2, 9], dtype=I32)
+    slot = (prefix_table[:, None] * page + torch.arange(page)).flatten()[:P].to(I32)
+    ops.paged_append(kv, prompt.cuda()[:, :hkv], prompt.cuda()[:, hkv:], slot.cuda(),
+                     ppos.cuda(), rope)
+    table = torch.tensor([[0, 1], [3, 4], [5, 6]], dtype=I32)
+    lens, counts = [0, 0, 0], [3, 1, 14]
+    rows = [[prompt], [prompt], [prompt]]
+    for step in range(3):
+        lens = [a + b for a, b in zip(lens, counts)]
+        T = sum(counts)
+        qkv = bf16(10 + step, T + 1, hq + 2 * hkv, d)
+        pos, slots, at = [], [], 0
+        for b, c in enumerate(counts):
+            own = torch.arange(lens[b] - c, lens[b])
+            pos.append(P + own)
+            slots.append(table[b][own // page] * page + own % page)
+            rows[b].append(qkv[at:at + c, hq:])
+            at += c
+        pos = torch.cat(pos + [torch.zeros(1)]).to(I32)[None]
+        slots = torch.cat(slots + [-torch.ones(1)]).to(I32)
+        dev = qkv.cuda()
+        ops.paged_append(kv, dev[:, hq:hq + hkv], dev[:, hq + hkv:], slots.cuda(), pos.cuda(),
+                         rope, q=dev[:, :hq], q_out=dev[:, :hq])
+        start = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=I32)
+        batch = u15h.PagedBatch(torch.tensor(lens, dtype=I32).cuda(), table.cuda(),
+                                q_start=start.cuda(), max_q=max(counts),
+                                prefix_table=prefix_table.cuda(), prefix_len=P)
+        out = torch.zeros(T + 1, hq, d, dtype=BF16, device="cuda")
+        ops.paged_attention(kv, batch, dev[:, :hq], out)
+        k, v = pool[:, 0].cpu(), pool[:, 1].cpu()
+        check(out[:T].cpu(), ref.attend(dev[:T, :hq].cpu(), k, v, prefix_table, P, table, lens,
+                                        counts, True))
+        assert bool((out[T] == 0).all())
+        # the contiguous cache's operators on each request by itself
+        at = 0
+        for b, c in enumerate(counts):
+            n = P + lens[b]
+            own = torch.cat(rows[b]).cuda()
+            turned = torch.empty(n, hkv, d, dtype=BF16, device="cuda")
+            ops.rope(own[:, :hkv], torch.arange(n, dtype=I32)[None].cuda(), rope, turned)
+            cache = turned.transpose(0, 1).contiguous()
+            vals = own[:, hkv:].transpose(0, 1).contiguous()
+            alone = torch.empty(c, hq * d, dtype=BF16, device="cuda")
+            ops.attention_token_major(dev[at:at + c, :hq].reshape(c, hq * d).contiguous(), cache,
+                                      vals, alone, hq, hkv, n, mode=1, q_offset=n - c)
+            one = out[at:at + c].reshape(c, hq * d).float()
+            # both within 2^-8 (weights) + 2^-8 (output) of the exact row
+            assert float((one - alone.float()).abs().max()) <= 4 * 2.0 ** -8 * float(
+                vals.float().abs().max())
+            at += c
+        counts = [1, 1, 2]

@@ -323,6 +323,59 @@ struct Fp8NormArgs {
 hipError_t launch_fp8_norm(const Fp8NormArgs& a, hipStream_t s);
 bool fp8_kernels_loadable();
 
+// ---- many requests: rotary positions, the paged cache (u15h_paged.hip) ------
+// Columns of a head that a rotation's part turns: pairs numbered from `pair`.
+struct RopePart {
+  const double* freq;     // [width / 2] radians per position
+  const int32_t* pos;     // its axis's positions [tokens]
+  int start, width, pair;
+};
+constexpr int kRopeMaxHeadDim = 512;
+// Rows of heads: token t's head h at p + t * tok + h * head elements.
+struct RopeRows {
+  const uint16_t* x;
+  uint16_t* y;
+  long long x_tok, x_head, y_tok, y_head;
+  int heads;
+};
+// rope: q's rows turned.  append: k's rows turned and v's copied into the
+// slots of a paged cache too.
+struct RopeArgs {
+  RopeRows q, k, v;       // k.y, v.y: the cache; their y strides unread
+  RopePart part[U15H_MAX_ROPE_PARTS];
+  int nparts, pairs;      // pairs of all parts
+  bool neighbours;
+  float scale;
+  float sign;             // -1: turned back
+  int tokens, d;
+  const int32_t* slot;    // append: [tokens], or null
+  long long page_stride;
+  int page_log2, slots;   // slots = pages * page
+  int vec;                // columns of a thread's access: 8, 2 or 1
+};
+hipError_t launch_rope(const RopeArgs& a, hipStream_t s);
+
+// Attention over a paged cache.  A row is one query head of one token; the
+// rows of a kv head (hq / hkv of each token) share its keys.
+struct PagedArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  long long q_tok, o_tok;
+  const uint16_t* k;
+  const uint16_t* v;
+  long long page_stride;
+  int pages, page_log2, hkv, d, hq;
+  const int32_t* q_start;       // or null: one query each
+  const int32_t* kv_len;
+  const int32_t* table;
+  const int32_t* prefix_table;
+  int table_stride, prefix, batch, tokens, max_q, max_kv;
+  bool causal;
+  float scale;                  // of the scores, log2(e) included
+};
+hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t s);
+bool paged_kernels_loadable();
+
 // What entry points outside u15h_api.cc need of the context: the device made
 // current; a launch's result as the call's status; the CUs that a GEMM's rounds
 // are planned for.

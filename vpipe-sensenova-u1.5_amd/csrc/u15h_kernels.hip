@@ -5109,7 +5109,7 @@ kernels_loadable()
     hipFuncAttributes a;
     if (hipFuncGetAttributes(&a, f) != hipSuccess) { return false; }
   }
-  return fp8_kernels_loadable() &&
+  return fp8_kernels_loadable() && paged_kernels_loadable() &&
          gemm_kernels_loadable<MmaBf16x16, MmaI8x16, 2>() &&
          gemm_kernels_loadable<MmaBf16x16, MmaI8x16, 4>() &&
          gemm_kernels_loadable<MmaBf16, MmaI8, 4>() &&

@@ -31,6 +31,8 @@ HEADER_PATH = REPO_DIR / "include" / "u15h.h"
 
 OK, EINVAL, ENODEV, ELAUNCH, ENOMEM = 0, 1, 2, 3, 4
 MAX_PROJ = 4
+MAX_ROPE_PARTS = 3
+ROPE_SCALING = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 _lib = None
 
@@ -68,6 +70,31 @@ class _LayerIO(ctypes.Structure):
 class _QkNorm(ctypes.Structure):
     _fields_ = [("q_t", ctypes.c_void_p), ("q_hw", ctypes.c_void_p),
                 ("k_t", ctypes.c_void_p), ("k_hw", ctypes.c_void_p)]
+
+
+class _RopePart(ctypes.Structure):
+    _fields_ = [("freq", ctypes.c_void_p), ("start", ctypes.c_int),
+                ("width", ctypes.c_int), ("axis", ctypes.c_int)]
+
+
+class _RopeSpec(ctypes.Structure):
+    _fields_ = [("part", _RopePart * MAX_ROPE_PARTS), ("nparts", ctypes.c_int),
+                ("neighbours", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
+class _PagedKV(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("page_stride", ctypes.c_int64), ("pages", ctypes.c_int),
+                ("page", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("head_dim", ctypes.c_int)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("tokens", ctypes.c_int),
+                ("max_q", ctypes.c_int), ("max_kv", ctypes.c_int),
+                ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("prefix_table", ctypes.c_void_p), ("prefix_len", ctypes.c_int)]
 
 
 class _LayerFullIO(ctypes.Structure):
@@ -167,6 +194,13 @@ def load_library() -> ctypes.CDLL:
         "u15h_build_rope_tables": (i, [vp, vp, vp, i, i, i, i,
                                        ctypes.c_double, ctypes.c_double, vp,
                                        vp]),
+        "u15h_rope_freqs": (i, [i, ctypes.c_double, i, ctypes.c_double, ctypes.c_double,
+                                ctypes.c_double, ctypes.c_double, vp, vp]),
+        "u15h_rope": (i, [vp, vp, vp, vp, vp, i64, i64, vp, i64, i64, i, i, i, i]),
+        "u15h_paged_append": (i, [vp, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp, i64, vp,
+                                  i64, i, i]),
+        "u15h_paged_attention": (i, [vp, vp, vp, vp, vp, i64, vp, i64, i,
+                                     ctypes.c_float, i]),
         "u15h_sdpa": (i, [vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i]),
         "u15h_sdpa_block_causal": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i,
                                        i, i, i]),
@@ -460,6 +494,118 @@ def build_rope_tables(pos_t, pos_h, pos_w, head_dim, d_t, d_h,
     if st != OK:
         raise U15hError(st, "u15h_build_rope_tables: invalid arguments")
     return cs[:T], sn[:T]
+
+
+def rope_freqs(width, theta, scaling="none", factor=1.0, trained=0, slow=None, fast=None):
+    """(freq, scale) of a part of `width` columns: radians per position of its
+    width / 2 pairs (f64, on the host) and what cosine and sine are times.
+    scaling: "none", "linear", "ntk", "yarn" or "bands" (u15h_rope_scaling);
+    slow and fast are turns within `trained` positions, 1 and 32 for YaRN and
+    1 and 4 for the bands where they are not given."""
+    if scaling not in ROPE_SCALING:
+        raise ValueError(f"scaling {scaling!r}: one of {', '.join(ROPE_SCALING)}")
+    slow = 1.0 if slow is None else slow
+    fast = (4.0 if scaling == "bands" else 32.0) if fast is None else fast
+    freq = torch.empty(max(int(width), 0) // 2, dtype=torch.float64)
+    scale = ctypes.c_float()
+    st = load_library().u15h_rope_freqs(width, theta, ROPE_SCALING[scaling], factor, trained,
+                                        slow, fast, freq.data_ptr(), ctypes.byref(scale))
+    if st != OK:
+        raise U15hError(st, "u15h_rope_freqs: invalid arguments")
+    return freq, scale.value
+
+
+def _table(t, device, name):
+    """A contiguous int32 tensor's address, on the given device."""
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected torch.int32")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name} must be on cuda:{device}")
+    return t.data_ptr()
+
+
+class Rope:
+    """A rotation (u15h_rope_spec), kept from call to call: `parts` is one to
+    three (freq, start, axis), freq a device f64 tensor as rope_freqs makes it,
+    start the part's first column, axis the row of the positions that turns
+    it."""
+
+    def __init__(self, parts, neighbours=False, scale=1.0):
+        if not 1 <= len(parts) <= MAX_ROPE_PARTS:
+            raise ValueError(f"1..{MAX_ROPE_PARTS} parts")
+        self._spec = _RopeSpec(nparts=len(parts), neighbours=int(bool(neighbours)), scale=scale)
+        self._kept = [p[0] for p in parts]
+        self.device = self._kept[0].get_device()
+        self.axes = 1 + max(int(p[2]) for p in parts)
+        for to, (freq, start, axis) in zip(self._spec.part, parts):
+            if freq.dtype is not torch.float64 or freq.dim() != 1 or not freq.is_contiguous() \
+                    or not freq.is_cuda or freq.get_device() != self.device:
+                raise ValueError("freq must be one contiguous f64 tensor a part, on one GPU")
+            if not 0 <= axis < MAX_ROPE_PARTS:
+                raise ValueError(f"axis {axis}: 0 to {MAX_ROPE_PARTS - 1}")
+            to.freq, to.start, to.width, to.axis = (freq.data_ptr(), start, 2 * freq.numel(),
+                                                    axis)
+        self._at = ctypes.addressof(self._spec)
+
+
+class PagedKV:
+    """A paged K/V cache (u15h_paged_kv): k and v [pages][kv_heads][page]
+    [head_dim] bf16, contiguous but for the distance between pages, which both
+    have alike (so they may be k = t[:, 0], v = t[:, 1] of one tensor)."""
+
+    def __init__(self, k, v):
+        for t, name in ((k, "k"), (v, "v")):
+            if t.dim() != 4 or t.dtype is not _BF16 or not t.is_cuda:
+                raise ValueError(f"{name} must be [pages][kv_heads][page][head_dim] bf16 on the "
+                                 "GPU")
+            _, h, p, d = t.shape
+            if t.numel() and t.stride()[1:] != (p * d, d, 1):
+                raise ValueError(f"{name}'s pages must be contiguous")
+        if k.shape != v.shape or k.stride(0) != v.stride(0) or k.get_device() != v.get_device():
+            raise ValueError("k and v must have one shape, distance between pages and device")
+        pages, heads, page, d = self.shape = tuple(k.shape)
+        self.k, self.v, self.device = k, v, k.get_device()
+        whole = heads * page * d
+        stride = k.stride(0) if pages > 1 else whole
+        if stride < whole:
+            raise ValueError("pages overlap")
+        self._kv = _PagedKV(k.data_ptr(), v.data_ptr(), stride, pages, page, heads, d)
+        self._at = ctypes.addressof(self._kv)
+
+
+class PagedBatch:
+    """A step's sequences (u15h_paged_batch), the same for all layers: kv_len
+    [batch] and table [batch][pages of a sequence] int32; q_start [batch + 1],
+    or None for one query each; the shared prefix's pages and length.  max_q
+    and max_kv bound the queries and own keys of a sequence (max_kv: the
+    table's width where not given).  The tensors may be rewritten in place
+    between calls or replays."""
+
+    def __init__(self, kv_len, table, q_start=None, max_q=1, max_kv=None, prefix_table=None,
+                 prefix_len=0):
+        self.device = kv_len.get_device()
+        if self.device < 0:
+            raise ValueError("kv_len must be on the GPU")
+        if kv_len.dim() != 1 or table.dim() != 2 or table.shape[0] != kv_len.numel():
+            raise ValueError("kv_len must be [batch], table [batch][pages]")
+        batch = kv_len.numel()
+        if q_start is not None and tuple(q_start.shape) != (batch + 1,):
+            raise ValueError(f"q_start must be [{batch + 1}]")
+        if q_start is None and max_q != 1:
+            raise ValueError("max_q > 1 needs q_start")
+        at = _table
+        dev = self.device
+        self.batch, self.max_q, self.width = batch, max_q, table.shape[1]
+        self.max_kv, self.prefix_len = max_kv, prefix_len
+        self.prefix_pages = 0 if prefix_table is None else prefix_table.numel()
+        self._kept = (kv_len, table, q_start, prefix_table)
+        self._b = _PagedBatch(
+            batch, 0, max_q, 0, None if q_start is None else at(q_start, dev, "q_start"),
+            at(kv_len, dev, "kv_len"), at(table, dev, "table"), self.width,
+            None if prefix_table is None else at(prefix_table, dev, "prefix_table"), prefix_len)
+        self._at = ctypes.addressof(self._b)
 
 
 def qweight_geometry(K, scales_cols, codes_cols):
@@ -1209,6 +1355,111 @@ class Ops:
         self._check(st, "u15h_add")
 
     # ---- attention -------------------------------------------------------
+    # ---- many requests at once ----------------------------------------------
+    def _rows(self, t, name):
+        """(address, distance of tokens, heads, head_dim) of [tokens][heads]
+        [head_dim] bf16 on this context's device whose heads are contiguous."""
+        if t.dtype is not _BF16 or t.dim() != 3 or t.get_device() != self.device:
+            raise ValueError(f"{name} must be [tokens][heads][head_dim] bf16 on "
+                             f"cuda:{self.device}")
+        _, h, d = t.shape
+        st, sh, sd = t.stride()
+        if (sd != 1 and d > 1) or (sh != d and h > 1):
+            raise ValueError(f"{name}'s heads must be contiguous")
+        return t.data_ptr(), st if t.shape[0] > 1 else h * d, h, d
+
+    def _turn(self, rope, pos, tokens):
+        """The addresses of a rotation and of its positions."""
+        if rope.device != self.device:
+            raise ValueError(f"the rotation is on cuda:{rope.device}, this context on "
+                             f"cuda:{self.device}")
+        if pos.dim() == 1 and rope.axes == 1:
+            good = pos.shape[0] == tokens
+        else:
+            good = pos.dim() == 2 and pos.shape[0] >= rope.axes and pos.shape[1] == tokens
+        if not good:
+            raise ValueError(f"pos must be [{rope.axes}][{tokens}]")
+        return rope._at, _table(pos, self.device, "pos")
+
+    def rope(self, x, pos, rope, y, inverse=False, stream=None):
+        """y = x [tokens][heads][head_dim] turned by its tokens' positions
+        [axes][tokens] (int32), or turned back; any strides between tokens and
+        heads; y may be x."""
+        for t, name in ((x, "x"), (y, "y")):
+            if t.dtype is not _BF16 or t.dim() != 3 or t.get_device() != self.device:
+                raise ValueError(f"{name} must be [tokens][heads][head_dim] bf16 on "
+                                 f"cuda:{self.device}")
+            if t.stride(2) != 1 and t.shape[2] > 1:
+                raise ValueError(f"{name}'s columns must be contiguous")
+        if x.shape != y.shape:
+            raise ValueError(f"y: shape {tuple(y.shape)}, expected {tuple(x.shape)}")
+        tokens, heads, d = x.shape
+        rp, pp = self._turn(rope, pos, tokens)
+        st = self._lib.u15h_rope(self._ctx, self._stream_here(stream), rp, pp, x.data_ptr(),
+                                 x.stride(0), x.stride(1), y.data_ptr(), y.stride(0),
+                                 y.stride(1), tokens, heads, d, inverse)
+        if st:
+            self._check(st, "u15h_rope")
+
+    def paged_append(self, kv, k, v, slot, pos=None, rope=None, q=None, q_out=None,
+                     stream=None):
+        """k [tokens][kv_heads][head_dim], turned, and v into the cache's slots
+        (int32 [tokens], page * page size + place; tokens whose slot is no
+        place are passed over), and q_out = q [tokens][heads][head_dim]
+        turned.  Rows may be columns of a wider matrix; q_out may be q."""
+        if kv.device != self.device:
+            raise ValueError(f"the cache is on cuda:{kv.device}, this context on "
+                             f"cuda:{self.device}")
+        kp, ks, h, d = self._rows(k, "k")
+        vp, vs, _, _ = self._rows(v, "v")
+        tokens = k.shape[0]
+        if k.shape != v.shape or h != kv.shape[1] or d != kv.shape[3]:
+            raise ValueError(f"k and v must be [tokens][{kv.shape[1]}][{kv.shape[3]}]")
+        if slot.dim() != 1 or slot.shape[0] != tokens:
+            raise ValueError(f"slot must be [{tokens}]")
+        rp = pp = qp = op = None
+        qs = os_ = hq = 0
+        if rope is not None:
+            if pos is None:
+                raise ValueError("a rotation needs positions")
+            rp, pp = self._turn(rope, pos, tokens)
+        if q is not None:
+            if q_out is None or q.shape != q_out.shape or q.shape[0] != tokens or \
+                    q.shape[2] != d:
+                raise ValueError(f"q and q_out must be [{tokens}][heads][{d}], both given")
+            qp, qs, hq, _ = self._rows(q, "q")
+            op, os_, _, _ = self._rows(q_out, "q_out")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        st = self._lib.u15h_paged_append(
+            self._ctx, self._stream_here(stream), kv._at, _table(slot, self.device, "slot"), rp,
+            pp, kp, ks, vp, vs, qp, qs, op, os_, hq, tokens)
+        if st:
+            self._check(st, "u15h_paged_append")
+
+    def paged_attention(self, kv, batch, q, out, scale=0.0, causal=True, stream=None):
+        """out = softmax(q . k * scale) . v for every sequence of the batch over
+        the shared prefix and its own keys; q, out [tokens][heads][head_dim]
+        (rows may be columns of a wider matrix); scale 0: 1/sqrt(head_dim)."""
+        if kv.device != self.device or batch.device != self.device:
+            raise ValueError(f"cache on cuda:{kv.device}, batch on cuda:{batch.device}, this "
+                             f"context on cuda:{self.device}")
+        qp, qs, h, d = self._rows(q, "q")
+        op, os_, _, _ = self._rows(out, "out")
+        if q.shape != out.shape or d != kv.shape[3]:
+            raise ValueError(f"q and out must be [tokens][heads][{kv.shape[3]}]")
+        b = batch._b
+        room = batch.width * kv.shape[2]
+        most = room if batch.max_kv is None else batch.max_kv
+        if most > room or batch.prefix_len > batch.prefix_pages * kv.shape[2]:
+            raise ValueError("the tables have fewer pages than max_kv or prefix_len keys")
+        b.tokens, b.max_kv = q.shape[0], most
+        st = self._lib.u15h_paged_attention(
+            self._ctx, self._stream_here(stream), kv._at, batch._at, qp, qs, op, os_, h, scale,
+            causal)
+        if st:
+            self._check(st, "u15h_paged_attention")
+
     def sdpa(self, q, k, v, out, hkv, tk, causal=False, q_offset=0,
              stream=None):
         """MetalOps::sdpa / sdpa_steel: q, out [hq][tq][d]; k, v caches
