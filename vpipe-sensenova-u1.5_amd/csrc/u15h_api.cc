@@ -773,6 +773,19 @@ u15h::split_workspace(u15h_ctx* ctx, void** ws)
   return st;
 }
 
+void*
+u15h::attention_scratch(const u15h_ctx* ctx, size_t* bytes)
+{
+  *bytes = ctx->attn_ws != nullptr ? kAttnWsBytes : 0;
+  return ctx->attn_ws;
+}
+
+int
+u15h::compute_units(const u15h_ctx* ctx)
+{
+  return ctx->num_cu;
+}
+
 size_t
 u15h::split_workspace_bytes(const u15h_ctx* ctx)
 {

@@ -372,7 +372,40 @@ struct PagedArgs {
   int table_stride, prefix, batch, tokens, max_q, max_kv;
   bool causal;
   float scale;                  // of the scores, log2(e) included
+  // The plan.  Sequences of at most kPagedShortRows rows a kv head run on the
+  // streaming kernel, longer ones on the tile kernel.
+  bool shorts, longs;           // there may be sequences of either kind
+  // > 0: the prefix is walked once for all rows, in that many shares of
+  // p_chunk keys, on the tile kernel or the streaming one; 0: every sequence
+  // walks it before its own keys.
+  int p_shares, p_chunk;
+  bool p_tile;
+  // Shares of what a sequence walks itself (chunks in keys, multiples of 128).
+  int s_shares, s_chunk, t_shares, t_chunk;
+  int nr;                       // 16-row blocks of a streaming workgroup: 1, 2
+  // With more than one part (p_shares + the larger of the others): their
+  // unnormalised outputs [part][tokens * hq][d] f32, then the rows' running
+  // maxima (base 2) and sums.
+  float* ws;
 };
+constexpr int kPagedShortRows = 64;
+__host__ __device__ inline int
+paged_own_parts(const PagedArgs& a)
+{
+  const int s = a.shorts ? a.s_shares : 1, t = a.longs ? a.t_shares : 1;
+  return s > t ? s : t;
+}
+__host__ __device__ inline int
+paged_parts(const PagedArgs& a)
+{
+  return a.p_shares + paged_own_parts(a);
+}
+inline size_t
+paged_ws_bytes(const PagedArgs& a)
+{
+  const int n = paged_parts(a);
+  return n > 1 ? (size_t)n * a.tokens * a.hq * (a.d + 2) * 4 : 0;
+}
 hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t s);
 bool paged_kernels_loadable();
 
@@ -386,6 +419,10 @@ int gemm_cus(const u15h_ctx* ctx);
 // capture) and its size (0 where splitting is switched off).
 u15h_status split_workspace(u15h_ctx* ctx, void** ws);
 size_t split_workspace_bytes(const u15h_ctx* ctx);
+// The scratch of attention split over the keys, null where there is none, and
+// the device's compute units.
+void* attention_scratch(const u15h_ctx* ctx, size_t* bytes);
+int compute_units(const u15h_ctx* ctx);
 
 // Forces every kernel's code object to load; false if any cannot.
 bool kernels_loadable();

@@ -145,6 +145,63 @@ check_rows(u15h_ctx* ctx, const char* what, const char* name, const void* p, int
   return U15H_OK;
 }
 
+// Shares of `keys` so that `base` workgroups each become about `want`, none
+// under `least` keys; the chunk in keys, a multiple of 128.
+void
+shares_of(long long keys, long long base, long long want, int least, int* shares, int* chunk)
+{
+  long long n = std::max(1LL, std::min(want / std::max(base, 1LL), keys / least));
+  long long c = ((keys + n - 1) / n + 127) / 128 * 128;
+  c = std::max(c, 128LL);
+  *chunk = (int)c;
+  *shares = (int)std::max(1LL, (keys + c - 1) / c);
+}
+
+// How a call is cut (PagedArgs): what the prefix phase and the sequences'
+// workgroups walk.
+void
+plan(PagedArgs& a, int cus, void* ws, size_t bytes)
+{
+  const int G = a.hq / a.hkv;
+  const long long R1 = (long long)a.max_q * G;
+  a.longs = R1 > u15h::kPagedShortRows;
+  a.shorts = G <= u15h::kPagedShortRows;
+  a.ws = static_cast<float*>(ws);
+  const long long rows = (long long)a.tokens * G;
+  const int want = 1 * cus;
+  const int pwant = 1 * cus;
+  const int least = 256;
+  bool phase = a.prefix >= 256 && a.batch >= 2 && (long long)a.batch * a.prefix >= 4096 &&
+               rows / a.batch <= 64;
+  a.nr = R1 <= 16 || !a.shorts ? 1 : 2;
+  for (int tries = 0; tries < 2; ++tries, phase = false) {
+    a.p_shares = 0;
+    if (phase && ws != nullptr) {
+      a.p_tile = rows > 64;
+      if (!a.p_tile && rows > 16) { a.nr = 2; }
+      const int rb = a.p_tile ? 128 : 16 * a.nr;
+      shares_of(a.prefix, (rows + rb - 1) / rb * a.hkv, pwant, least, &a.p_shares, &a.p_chunk);
+    }
+    const long long keys = (a.p_shares > 0 ? 0 : (a.prefix + 63) / 64 * 64) + a.max_kv;
+    const int rb = 16 * a.nr;
+    const long long sblocks = (std::min<long long>(R1, u15h::kPagedShortRows) + rb - 1) / rb;
+    shares_of(keys, sblocks * a.hkv * a.batch, want, least, &a.s_shares, &a.s_chunk);
+    shares_of(keys, (rows / 128 + a.batch) * a.hkv, want, least, &a.t_shares, &a.t_chunk);
+    if (ws == nullptr) { a.s_shares = a.t_shares = 1; }
+    while (u15h::paged_ws_bytes(a) > bytes && a.s_shares + a.t_shares > 2) {
+      if (a.s_shares > 1) { --a.s_shares; }
+      if (a.t_shares > 1) { --a.t_shares; }
+      a.s_chunk = (int)(((keys + a.s_shares - 1) / a.s_shares + 127) / 128 * 128);
+      a.t_chunk = (int)(((keys + a.t_shares - 1) / a.t_shares + 127) / 128 * 128);
+    }
+    while (u15h::paged_ws_bytes(a) > bytes && a.p_shares > 1) {
+      --a.p_shares;
+      a.p_chunk = (int)(((a.prefix + a.p_shares - 1) / a.p_shares + 127) / 128 * 128);
+    }
+    if (u15h::paged_ws_bytes(a) <= bytes) { break; }
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -374,6 +431,9 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
   a.max_kv = bt->max_kv;
   a.causal = causal != 0;
   a.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)kv->head_dim)) * 1.4426950408889634f;
+  size_t bytes = 0;
+  void* ws = u15h::attention_scratch(ctx, &bytes);
+  plan(a, u15h::compute_units(ctx), ws, bytes);
   if ((st = u15h::begin_call(ctx)) != U15H_OK) { return st; }
   return u15h::end_call(
       ctx, u15h::launch_paged_attention(a, reinterpret_cast<hipStream_t>(stream)), what);

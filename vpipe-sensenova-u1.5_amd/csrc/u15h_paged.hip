@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "u15h_internal.h"
 
@@ -314,14 +315,51 @@ sequence(const PagedArgs& A, int b)
   return {uniform(s0), uniform(min(s1 - s0, A.max_q)), uniform(min(max(A.kv_len[b], 0), most))};
 }
 
-// The tiles of 32 keys that a workgroup walks: [0, prefix_tiles) the prefix's,
-// then the own keys'.
+// The partial results of part p: row r's output, and its maximum and sum (the
+// sum kNoKey where the part saw no key of it, kFinal in part 0 where the row's
+// output is written already).
+constexpr float kNoKey = -1.0f, kFinal = -2.0f;
+struct Part {
+  float* o;
+  float2* ml;
+};
+__device__ __forceinline__ Part
+part_of(const PagedArgs& A, int p)
+{
+  const long long rows = (long long)A.tokens * A.hq;
+  return {A.ws + p * rows * A.d,
+          reinterpret_cast<float2*>(A.ws + paged_parts(A) * rows * A.d) + p * rows};
+}
+__device__ __forceinline__ long long
+part_row(const PagedArgs& A, int token, int head)
+{
+  return (long long)token * A.hq + head;
+}
+// Marks the rows [row0, row0 + n) of a kv head in the parts [from, to).
+__device__ __forceinline__ void
+mark_parts(const PagedArgs& A, int from, int to, int first, int G, int kvh, int row0, int n,
+           float what)
+{
+  for (int p = from; p < to; ++p) {
+    const Part P = part_of(A, p);
+    for (int r = threadIdx.x; r < n; r += 256) {
+      const int row = row0 + r;
+      P.ml[part_row(A, first + row / G, kvh * G + row % G)] = make_float2(-INFINITY, what);
+    }
+  }
+}
+
+// What a workgroup walks: prefix keys, then own keys, each from a tile's start,
+// of which the tiles [begin, end).
 struct Walk {
   const int32_t* table;        // the sequence's pages
-  int prefix, keys;            // keys of either
-  int prefix_tiles;
+  int prefix, keys;
+  int prefix_tiles, begin, end;
 };
 
+// One workgroup: up to RB rows of a kv head over a share of keys.  The first
+// workgroups take the prefix's shares for all rows (where the plan has them on
+// this kernel), the others a sequence each.
 template <int D, int NR>
 __global__ __launch_bounds__(256) void
 paged_stream_kernel(const PagedArgs A)
@@ -336,29 +374,67 @@ paged_stream_kernel(const PagedArgs A)
   __shared__ float sm[W][RB], sl[W][RB];
 
   const int G = A.hq / A.hkv;
-  const int blocks = (A.max_q * G + RB - 1) / RB;
-  const int kvh = blockIdx.x % A.hkv;
-  const int rb = (blockIdx.x / A.hkv) % blocks;
-  const int b = blockIdx.x / (A.hkv * blocks);
-  const Sequence S = sequence(A, b);
+  int item = blockIdx.x;
+  const int p_shares = A.p_tile ? 0 : A.p_shares;
+  const int p_blocks = (A.tokens * G + RB - 1) / RB;
+  const int p_items = p_shares * p_blocks * A.hkv;
+  const bool phase = item < p_items;
+  Sequence S;
+  Walk K;
+  int kvh, row0, part, share, share_tiles;
+  if (phase) {
+    // the blocks of rows of one share of one head 8 apart: one die's L2
+    const int runs = p_shares * A.hkv;
+    int run;
+    if (runs % 8 == 0) {
+      run = item / (8 * p_blocks) * 8 + item % 8;
+      row0 = item / 8 % p_blocks * RB;
+    } else {
+      run = item / p_blocks;
+      row0 = item % p_blocks * RB;
+    }
+    kvh = run % A.hkv;
+    share = run / A.hkv;
+    part = share;
+    S = {0, A.tokens, 0};
+    K = {nullptr, A.prefix, 0, (A.prefix + 31) / 32, 0, 0};
+    share_tiles = A.p_chunk / 32;
+  } else {
+    item -= p_items;
+    const int blocks = (min(A.max_q * G, kPagedShortRows) + RB - 1) / RB;
+    kvh = item % A.hkv;
+    item /= A.hkv;
+    row0 = item % blocks * RB;
+    item /= blocks;
+    share = item % A.s_shares;
+    const int b = item / A.s_shares;
+    part = A.p_shares + share;
+    S = sequence(A, b);
+    if (S.n * G > kPagedShortRows) { return; }
+    K.table = A.table + (long long)b * A.table_stride;
+    K.prefix = A.p_shares > 0 ? 0 : A.prefix;
+    K.prefix_tiles = (K.prefix + 31) / 32;
+    // own keys that the block's last row sees
+    const int last = (min(S.n * G, row0 + RB) - 1) / G;
+    K.keys = A.causal ? max(S.keys - S.n + last + 1, 0) : S.keys;
+    share_tiles = A.s_chunk / 32;
+  }
   const int rows = S.n * G;
-  const int row0 = rb * RB;
   if (row0 >= rows) { return; }
+  const bool direct = paged_parts(A) == 1;
+  const int tiles = K.prefix_tiles + (K.keys + 31) / 32;
+  const bool last_share = share == (phase ? p_shares : A.s_shares) - 1;
+  K.begin = min(share * share_tiles, tiles);
+  K.end = last_share ? tiles : min(K.begin + share_tiles, tiles);
+  if (!phase && last_share) {
+    mark_parts(A, part + 1, paged_parts(A), S.first, G, kvh, row0, min(rows - row0, RB), kNoKey);
+  }
 
   const int tid = threadIdx.x;
   const int wave = uniform(tid >> 6);
   const int lane = tid & 63;
   const int lr = lane & 15;
   const int g = lane >> 4;
-
-  Walk K;
-  K.table = A.table + (long long)b * A.table_stride;
-  K.prefix = A.prefix;
-  K.prefix_tiles = (A.prefix + 31) / 32;
-  // own keys that the block's last row sees
-  const int last = (min(rows, row0 + RB) - 1) / G;
-  K.keys = A.causal ? max(S.keys - S.n + last + 1, 0) : S.keys;
-  const int tiles = K.prefix_tiles + (K.keys + 31) / 32;
 
   i32x4_t qf[NR][KS];
   int lim[NR];                               // last own key that the row sees
@@ -376,15 +452,16 @@ paged_stream_kernel(const PagedArgs A)
   }
   const int lim0 = A.causal ? S.keys - S.n + row0 / G : S.keys - 1;   // the first row's
 
-  // This wave's i-th tile is wave + W * i; lane 2 (i % 32) + block holds the
+  // This wave's i-th tile is tile0 + W * i; lane 2 (i % 32) + block holds the
   // page of its block of 16 keys, -1 where it has none.
-  const int mine = (tiles - wave + W - 1) / W;
+  const int tile0 = K.begin + wave;
+  const int mine = (K.end - tile0 + W - 1) / W;
   auto pages_of = [&](int group) {
-    const int tile = wave + W * (group * 32 + (lane >> 1));
+    const int tile = tile0 + W * (group * 32 + (lane >> 1));
     const bool pre = tile < K.prefix_tiles;
     const int key = (pre ? tile : tile - K.prefix_tiles) * 32 + (lane & 1) * 16;
     int id = -1;
-    if (key < (pre ? K.prefix : K.keys)) {
+    if (tile < K.end && key < (pre ? K.prefix : K.keys)) {
       id = (pre ? A.prefix_table : K.table)[key >> A.page_log2];
     }
     return (unsigned)id < (unsigned)A.pages ? id : -1;
@@ -400,7 +477,7 @@ paged_stream_kernel(const PagedArgs A)
     int bytes;
   };
   auto block = [&](int i, int blk) {
-    const int tile = wave + W * i;
+    const int tile = tile0 + W * i;
     const bool pre = tile < K.prefix_tiles;
     const int key = (pre ? tile : tile - K.prefix_tiles) * 32 + blk * 16;
     const int id = __builtin_amdgcn_readlane(ids, 2 * (i & 31) + blk);
@@ -467,7 +544,7 @@ paged_stream_kernel(const PagedArgs A)
     load_v(0);
   }
   for (int i = 0; i < mine; ++i) {
-    const int tile = wave + W * i;
+    const int tile = tile0 + W * i;
     const bool pre = tile < K.prefix_tiles;
     const int key0 = (pre ? tile : tile - K.prefix_tiles) * 32;
     const int id0 = __builtin_amdgcn_readlane(ids, 2 * (i & 31));
@@ -570,21 +647,597 @@ paged_stream_kernel(const PagedArgs A)
       sum += f * sl[w][r];
       acc += f * *reinterpret_cast<const f32x4_t*>(so + (w * RB + r) * PITCH + c);
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     const int row = row0 + r;
+    if (!direct) {
+      const Part P = part_of(A, part);
+      const long long at = part_row(A, S.first + row / G, kvh * G + row % G);
+      if (c == 0) { P.ml[at] = make_float2(top, top == -INFINITY ? kNoKey : sum); }
+      if (top == -INFINITY) { continue; }
+      *reinterpret_cast<f32x4_t*>(P.o + at * D + c) = acc;
+      continue;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
     uint16_t* op = A.out + (S.first + row / G) * A.o_tok + (kvh * G + row % G) * D + c;
     *reinterpret_cast<u32x2_t*>(op) = u32x2_t{pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                               pack_bf16x2(acc[2] * inv, acc[3] * inv)};
   }
 }
 
+// paged_tile_kernel: 128 rows of one kv head a workgroup, for sequences (or
+// prefixes of many) whose products outweigh their keys' bytes.  The tile loop is
+// attention_kernel's: scores and output transposed on 32x32x16 products, keys
+// and values of 64-key tiles copied from memory to LDS and read there by all
+// four waves, one barrier a tile, the scores of tile t + 1 beside the
+// exponentials of tile t.  What pages add is the address of a copy: a wave
+// copies 16 keys, which lie in one page, through a buffer resource of its own
+// whose range ends at the last key; so no page ends inside it and keys past the
+// end read as zeros.  The page numbers of the next 16 tiles sit in a register,
+// a lane each, and are read a group of 16 tiles ahead.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x16_t
+mma32(i32x4_t a, i32x4_t b, f32x16_t c)
+{
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                 __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float
+max_halves(float v)
+{
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float
+sum_halves(float v)
+{
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// Swizzle of V's 64-byte blocks: four consecutive keys at one block land on
+// four different bank ranges.
+template <int D>
+__device__ __forceinline__ int
+vswz(int r)
+{
+  return (r * (D / 32) / 4) % (D / 32);
+}
+
+constexpr int kTileRows = 128;
+
+// Block `nb` of the tile kernel's rows of all sequences: the sequence, which
+// has the blocks from first_block(b) = rows before it / 128 + b on (one more
+// than it can need at most), and the block within it.
+__device__ __forceinline__ int
+sequence_of_block(const PagedArgs& A, int G, int nb, int* local)
+{
+  const int lane = threadIdx.x & 63;
+  int count = 0, start = 0;
+  for (int b0 = 0; b0 < A.batch; b0 += 64) {
+    const int b = b0 + lane;
+    int f = INT_MAX;
+    if (b < A.batch) {
+      const int s0 = A.q_start != nullptr ? min(max(A.q_start[b], 0), A.tokens) : b;
+      f = s0 * G / kTileRows + b;
+    }
+    const unsigned long long below = __ballot(f <= nb);
+    if (below == 0) { break; }
+    const int last = 63 - __builtin_clzll(below);
+    count = b0 + last + 1;
+    start = __builtin_amdgcn_readlane(f, last);
+    if (last < 63) { break; }
+  }
+  *local = nb - start;
+  return count - 1;
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void
+paged_tile_kernel(const PagedArgs A)
+{
+  constexpr int BK = 64;                     // keys of a tile
+  constexpr int KCH = D / 8;                 // 16-byte chunks of a key
+  constexpr int NDS = D / 16;                // matrix steps of the scores
+  constexpr int NCB = D / 32;                // blocks of 32 columns of O
+  constexpr int CPW = D / 32;                // 1 KiB copies of a wave's 16 keys
+  __shared__ __attribute__((aligned(16))) uint16_t ks0[BK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t ks1[BK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t vs0[BK * D];
+  __shared__ __attribute__((aligned(16))) uint16_t vs1[BK * D];
+
+  const int G = A.hq / A.hkv;
+  const int p_blocks = (A.tokens * G + kTileRows - 1) / kTileRows;
+  const int p_items = A.p_tile ? A.p_shares * p_blocks * A.hkv : 0;
+  const bool phase = (int)blockIdx.x < p_items;
+  Sequence S;
+  const int32_t* table = nullptr;
+  int prefix = A.prefix, kvh, row0, part, share, shares, chunk;
+  if (phase) {
+    // run by run of one head's keys, cut in 8 ranges, one per die
+    const int b = blockIdx.x;
+    const int item = p_items % 8 == 0 ? (b % 8) * (p_items / 8) + b / 8 : b;
+    row0 = item % p_blocks * kTileRows;
+    share = item / p_blocks % A.p_shares;
+    kvh = item / (p_blocks * A.p_shares);
+    part = share;
+    shares = A.p_shares;
+    chunk = A.p_chunk;
+    S = {0, A.tokens, 0};
+  } else {
+    const int b = blockIdx.x - p_items, items = gridDim.x - p_items;
+    int item = items % 8 == 0 ? (b % 8) * (items / 8) + b / 8 : b;
+    const int blocks = A.tokens * G / kTileRows + A.batch;
+    share = item % A.t_shares;
+    item /= A.t_shares;
+    int local;
+    // the last blocks of a causal sequence see most keys: they go first
+    const int seq = sequence_of_block(A, G, blocks - 1 - item % blocks, &local);
+    kvh = item / blocks;
+    part = A.p_shares + share;
+    shares = A.t_shares;
+    chunk = A.t_chunk;
+    if (seq < 0) { return; }
+    S = sequence(A, uniform(seq));
+    row0 = uniform(local) * kTileRows;
+    if (S.n * G <= kPagedShortRows) { return; }
+    table = A.table + (long long)uniform(seq) * A.table_stride;
+    if (A.p_shares > 0) { prefix = 0; }
+  }
+  const int rows = S.n * G;
+  if (row0 >= rows) { return; }
+  const int parts = paged_parts(A);
+  const bool direct = A.p_shares == 0 && shares == 1;
+  const int nrows = min(rows - row0, kTileRows);
+
+  const int tid = threadIdx.x;
+  const int wave = uniform(tid >> 6);
+  const int lane = tid & 63;
+  const int lq = lane & 31;
+  const int half = lane >> 5;
+  const int row = row0 + wave * 32 + lq;
+  const bool valid = row < rows;
+  const int tok = min(row, rows - 1) / G;
+  const int h = kvh * G + row % G;
+  const float scale = A.scale;
+  const float lazy = kLazy / scale;          // in raw score units
+
+  // own keys: the last that this row, the first row and the last row see
+  const int lim = A.causal ? S.keys - S.n + tok : S.keys - 1;
+  const int lim0 = A.causal ? S.keys - S.n + row0 / G : S.keys - 1;
+  const int keys = A.causal ? max(S.keys - S.n + (row0 + nrows - 1) / G + 1, 0) : S.keys;
+  const int ptiles = (prefix + BK - 1) / BK;
+  const int all = ptiles + (keys + BK - 1) / BK;
+  const int tbeg = min(share * (chunk / BK), all);
+  const int ntiles = share == shares - 1 ? all : min(tbeg + chunk / BK, all);
+  if (!phase) {
+    if (direct) {
+      if (parts > 1) { mark_parts(A, 0, 1, S.first, G, kvh, row0, nrows, kFinal); }
+    } else if (share == shares - 1) {
+      mark_parts(A, part + 1, parts, S.first, G, kvh, row0, nrows, kNoKey);
+    }
+  }
+
+  i32x4_t qf[NDS];
+  const uint16_t* qp = A.q + (S.first + tok) * A.q_tok + h * D;
+#pragma unroll
+  for (int ds = 0; ds < NDS; ++ds) {
+    qf[ds] = valid ? *reinterpret_cast<const i32x4_t*>(qp + ds * 16 + half * 8)
+                   : i32x4_t{0, 0, 0, 0};
+  }
+
+  // ---- pages ---------------------------------------------------------------
+  // Lane 4 i + w: the page of keys [16 w, 16 w + 16) of tile tbeg + 16 group + i,
+  // -1 where it has none; `there` has the lanes that have one.
+  auto number = [&](int group) {             // as the table has it
+    const int t = tbeg + group * 16 + (lane >> 2);
+    const bool pre = t < ptiles;
+    const int key = (pre ? t : t - ptiles) * BK + (lane & 3) * 16;
+    int id = -1;
+    if (t < ntiles && key < (pre ? prefix : keys)) {
+      id = (pre ? A.prefix_table : table)[key >> A.page_log2];
+    }
+    return id;
+  };
+  auto checked = [&](int id) { return (unsigned)id < (unsigned)A.pages ? id : -1; };
+  int ids0 = number(0), ids1 = number(1);
+  ids0 = checked(ids0);
+  ids1 = checked(ids1);
+  unsigned long long there0 = __ballot(ids0 >= 0), there1 = __ballot(ids1 >= 0);
+  int group = 0;                             // of ids0; ids1 the next one's
+  auto page_of = [&](int t) {
+    const int i = t - tbeg;
+    const int at = 4 * (i & 15) + wave;
+    const int a = __builtin_amdgcn_readlane(ids0, at), b = __builtin_amdgcn_readlane(ids1, at);
+    return (i >> 4) == group ? a : b;
+  };
+  auto there_of = [&](int t) {
+    const int i = t - tbeg;
+    return (int)(((i >> 4) == group ? there0 : there1) >> (4 * (i & 15))) & 15;
+  };
+
+  // ---- copies: memory -> LDS -------------------------------------------------
+  i32x4_t koffs = {}, voffs = {};
+#pragma unroll
+  for (int i = 0; i < CPW; ++i) {
+    const int idx = i * 64 + lane;                    // landing chunk in the wave's 16 keys
+    const int r = idx / KCH;
+    koffs[i] = (r * D + (((idx % KCH) ^ (r % KCH)) << 3)) * 2;
+    voffs[i] = (r * D + (((idx % KCH) ^ (4 * vswz<D>(r))) << 3)) * 2;
+  }
+  auto copy = [&](const uint16_t* pool, int t, uint16_t* dst_tile, const i32x4_t& offs) {
+    const bool pre = t < ptiles;
+    const int key = (pre ? t : t - ptiles) * BK + wave * 16;
+    const int id = page_of(t);
+    const int left = min((pre ? prefix : keys) - key, 16);
+    const long long at = max(id, 0) * A.page_stride +
+                         (((long long)kvh << A.page_log2) + (key & ((1 << A.page_log2) - 1))) * D;
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(pool + at, id < 0 ? 0 : left * D * 2);
+    char* dst = reinterpret_cast<char*>(dst_tile) + wave * CPW * 1024;
+#pragma unroll
+    for (int i = 0; i < CPW; ++i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rs, (__attribute__((address_space(3))) void*)(dst + i * 1024), 16, offs[i], 0, 0, 0);
+    }
+  };
+
+  // per-lane fragment offsets (elements)
+  const int koff = lq * D;                             // + swizzled chunk
+  const int vrow = 4 * half + ((lane & 15) >> 2);      // transpose-read key
+  const int vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+
+  f32x16_t o[NCB];
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) { o[cb] = f32x16_t{}; }
+  float m = -INFINITY;      // running max, raw score units
+  float l = 0.0f;           // this half's share of the running sum
+  f32x16_t sc[2];           // scores of the current tile
+  float mb = -INFINITY;     // their max over the row (both halves)
+
+  auto mask = [&](f32x16_t (&s)[2], int t) {
+    const bool pre = t < ptiles;
+    const int j0 = (pre ? t : t - ptiles) * BK;
+    const int there = there_of(t);
+    if (j0 + BK - 1 <= (pre ? prefix - 1 : lim0) && there == 15) { return; }
+    const int last = pre ? prefix - 1 : lim;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      const int kl = (r >> 4) * 32 + 8 * ((r & 15) >> 2) + 4 * half + (r & 3);
+      const bool ok = (j0 + kl <= last) &
+                      (((there >> ((r >> 4) * 2 + ((r & 15) >> 3))) & 1) != 0);
+      s[r >> 4][r & 15] = ok ? s[r >> 4][r & 15] : -INFINITY;
+    }
+  };
+  uint32_t pk[16];
+  float ps;
+  float mc;
+  auto expo = [&](const f32x16_t& s, int r, int slot) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -mc));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], scale, -mc));
+    pk[slot] = pack_bf16x2(p0, p1);
+    ps = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pk[slot]),
+                                         __builtin_bit_cast(bf16x2_t, 0x3f803f80u), ps, false);
+  };
+  auto pv = [&](const uint16_t* vread, int k4, int cb) {
+    const i32x4_t pf = {(int)pk[k4 * 4 + 0], (int)pk[k4 * 4 + 1], (int)pk[k4 * 4 + 2],
+                        (int)pk[k4 * 4 + 3]};
+    const int r0 = k4 * 16 + vrow;
+    const int c = (((cb ^ vswz<D>(r0)) << 5) | vcol);     // r0, r0 + 8 share it
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4_t*)(vread + r0 * D + c));
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4_t*)(vread + (r0 + 8) * D + c));
+    const i32x4_t vf = {__builtin_bit_cast(int, (i16x2_t){lo[0], lo[1]}),
+                        __builtin_bit_cast(int, (i16x2_t){lo[2], lo[3]}),
+                        __builtin_bit_cast(int, (i16x2_t){hi[0], hi[1]}),
+                        __builtin_bit_cast(int, (i16x2_t){hi[2], hi[3]})};
+    o[cb] = mma32(vf, pf, o[cb]);
+  };
+
+  // One iteration over tile t: A scores of tile t + 1 | exponentials of keys
+  // 0..31; B P V of keys 0..31 | exponentials of keys 32..63; C P V of keys
+  // 32..63 | mask and max of tile t + 1's scores.
+  constexpr int EPA = 16 / NDS, EPB = 16 / (2 * NCB), MPC = 32 / (2 * NCB);
+  auto iteration = [&](int t, const uint16_t* kread, uint16_t* kfill, const uint16_t* vread,
+                       uint16_t* vfill) {
+    if (mb > m + lazy) {
+      const float alpha = exp2f((m - mb) * scale);     // 0 while m is -inf
+      l *= alpha;
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { o[cb][r] *= alpha; }
+      }
+      m = mb;
+    }
+    mc = m == -INFINITY ? 0.0f : m * scale;
+    ps = 0.0f;
+    copy(A.k, t + 2, kfill, koffs);
+    copy(A.v, t + 1, vfill, voffs);
+
+    f32x16_t sn[2] = {f32x16_t{}, f32x16_t{}};
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      const int off = koff + (((ds * 2 + half) ^ (lq % KCH)) << 3);
+      const i32x4_t k0 = *reinterpret_cast<const i32x4_t*>(kread + off);
+      const i32x4_t k1 = *reinterpret_cast<const i32x4_t*>(kread + 32 * D + off);
+      sn[0] = mma32(k0, qf[ds], sn[0]);
+#pragma unroll
+      for (int e = 0; e < EPA; e += 2) { expo(sc[0], ds * EPA + e, (ds * EPA + e) >> 1); }
+      sn[1] = mma32(k1, qf[ds], sn[1]);
+    }
+#pragma unroll
+    for (int k4 = 0; k4 < 2; ++k4) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        pv(vread, k4, cb);
+        const int r = (k4 * NCB + cb) * EPB;
+#pragma unroll
+        for (int e = 0; e < EPB; e += 2) { expo(sc[1], r + e, 8 + ((r + e) >> 1)); }
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);                // reads 0, 1
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);              // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, 6 * EPA / 4, 0);    // VALU
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);              // reads +2
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);              // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, 6 * EPA / 4, 0);    // VALU
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NCB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);              // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, 6 * EPB / 4, 0);    // VALU
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);              // reads +2
+      __builtin_amdgcn_sched_group_barrier(0x002, 6 * EPB / 4, 0);    // VALU
+    }
+    // (past the last tile the scores come from stale K and are dropped)
+    if (t + 1 < ntiles) { mask(sn, t + 1); }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k4 = 2; k4 < 4; ++k4) {
+#pragma unroll
+      for (int cb = 0; cb < NCB; ++cb) {
+        pv(vread, k4, cb);
+        const int r = ((k4 - 2) * NCB + cb) * MPC;
+#pragma unroll
+        for (int e = 0; e < MPC; ++e) { mx = fmaxf(mx, sn[(r + e) >> 4][(r + e) & 15]); }
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);                // reads 0, 1
+#pragma unroll
+    for (int i = 0; i < 2 * NCB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);              // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x002, MPC / 2, 0);        // VALU
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);              // reads +2
+    }
+    mb = max_halves(mx);
+    l += ps;
+    // Tiles t + 2 and t + 3 are next: from the end of a group on, its
+    // successor.  The one after that is read here and looked at half a group
+    // later; it is needed from tile 14 of the group on.
+    if (((t + 1 - tbeg) & 7) == 0) {
+      if (((t + 1 - tbeg) & 8) == 0) {
+        ids0 = ids1;
+        there0 = there1;
+        ++group;
+        ids1 = number(group + 1);
+      } else if (group > 0) {
+        ids1 = checked(ids1);
+        there1 = __ballot(ids1 >= 0);
+      }
+    }
+    __syncthreads();
+    sc[0] = sn[0];
+    sc[1] = sn[1];
+  };
+
+  if (tbeg < ntiles) {
+    copy(A.k, tbeg, ks0, koffs);
+    copy(A.k, tbeg + 1, ks1, koffs);
+    copy(A.v, tbeg, vs0, voffs);
+    __syncthreads();
+    sc[0] = f32x16_t{};
+    sc[1] = f32x16_t{};
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) {
+      const int off = koff + (((ds * 2 + half) ^ (lq % KCH)) << 3);
+      sc[0] = mma32(*reinterpret_cast<const i32x4_t*>(ks0 + off), qf[ds], sc[0]);
+      sc[1] = mma32(*reinterpret_cast<const i32x4_t*>(ks0 + 32 * D + off), qf[ds], sc[1]);
+    }
+    mask(sc, tbeg);
+    float mx = sc[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; ++r) { mx = fmaxf(mx, sc[r >> 4][r & 15]); }
+    mb = max_halves(mx);
+    __syncthreads();
+  }
+  for (int t = tbeg; t < ntiles; t += 2) {
+    iteration(t, ks1, ks0, vs0, vs1);
+    if (t + 1 < ntiles) { iteration(t + 1, ks0, ks1, vs1, vs0); }
+  }
+
+  l = sum_halves(l);
+  if (!valid) { return; }
+  if (!direct) {
+    const Part P = part_of(A, part);
+    const long long at = part_row(A, S.first + tok, h);
+    if (half == 0) { P.ml[at] = make_float2(m * scale, m == -INFINITY ? kNoKey : l); }
+    if (m == -INFINITY) { return; }
+    float* op = P.o + at * D;
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        *reinterpret_cast<f32x4_t*>(op + cb * 32 + 8 * g + 4 * half) =
+            f32x4_t{o[cb][4 * g], o[cb][4 * g + 1], o[cb][4 * g + 2], o[cb][4 * g + 3]};
+      }
+    }
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  uint16_t* op = A.out + (S.first + tok) * A.o_tok + h * D;
+#pragma unroll
+  for (int cb = 0; cb < NCB; ++cb) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      *reinterpret_cast<u32x2_t*>(op + cb * 32 + 8 * g + 4 * half) =
+          u32x2_t{pack_bf16x2(o[cb][4 * g] * inv, o[cb][4 * g + 1] * inv),
+                  pack_bf16x2(o[cb][4 * g + 2] * inv, o[cb][4 * g + 3] * inv)};
+    }
+  }
+}
+
+// Whether a token is a row of some sequence.
+__device__ __forceinline__ bool
+in_sequence(const PagedArgs& A, int token)
+{
+  if (A.q_start == nullptr) { return token < A.batch; }
+  int lo = 0, hi = A.batch;                  // the last b with q_start[b] <= token
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (A.q_start[mid] <= token) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  const Sequence S = sequence(A, lo);
+  return token >= S.first && token - S.first < S.n;
+}
+
+// Adds the parts of a row, W waves a row, in the order of the parts:
+// out = sum f_p o_p / sum f_p l_p with f_p = 2^(m_p - max m).
+template <int D, int W>
+__global__ __launch_bounds__(256) void
+paged_combine_kernel(const PagedArgs A)
+{
+  constexpr int C = D / 32;                  // columns a lane
+  constexpr int kAhead = 8;
+  __shared__ float so[4][D];
+  __shared__ float2 sml[4];
+  const int wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int half = lane >> 5;                // parts 2 i + half
+  const int c = (lane & 31) * C;
+  const long long row = (long long)blockIdx.x * (4 / W) + wave / W;
+  const int token = (int)(row / A.hq);
+  const int n = paged_parts(A);
+  bool live = row < (long long)A.tokens * A.hq && in_sequence(A, token);
+  if (live) { live = part_of(A, 0).ml[row].y != kFinal; }
+
+  float m = -INFINITY, l = 0.0f, o[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) { o[e] = 0.0f; }
+  auto add = [&](float m1, float l1, const float* o1) {
+    if (l1 < 0.0f) { return; }
+    const float top = fmaxf(m, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+    l = __builtin_fmaf(l, f0, l1 * f1);
+#pragma unroll
+    for (int e = 0; e < C; ++e) { o[e] = __builtin_fmaf(o1[e], f1, o[e] * f0); }
+    m = top;
+  };
+  if (live) {
+    for (int p0 = (wave % W) * 2 + half; p0 < n; p0 += 2 * W * kAhead) {
+      float2 ml[kAhead];
+      float o1[kAhead][C];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int p = p0 + 2 * W * i;
+        ml[i] = make_float2(-INFINITY, kNoKey);
+        if (p < n) {
+          const Part P = part_of(A, p);
+          ml[i] = P.ml[row];
+          typedef float vec_t __attribute__((ext_vector_type(C)));
+          const vec_t v = *reinterpret_cast<const vec_t*>(P.o + row * D + c);
+#pragma unroll
+          for (int e = 0; e < C; ++e) { o1[i][e] = v[e]; }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) { add(ml[i].x, ml[i].y, o1[i]); }
+    }
+  }
+  // the halves, then the waves
+  {
+    const float m1 = __shfl_xor(m, 32), l1 = __shfl_xor(l, 32);
+    float o1[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) { o1[e] = __shfl_xor(o[e], 32); }
+    add(m1, m1 == -INFINITY ? kNoKey : l1, o1);
+  }
+  if constexpr (W > 1) {
+    if (half == 0) {
+#pragma unroll
+      for (int e = 0; e < C; ++e) { so[wave][c + e] = o[e]; }
+      if (lane == 0) { sml[wave] = make_float2(m, m == -INFINITY ? kNoKey : l); }
+    }
+    __syncthreads();
+    if (wave % W != 0) { return; }
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      float o1[C];
+#pragma unroll
+      for (int e = 0; e < C; ++e) { o1[e] = so[wave + w][c + e]; }
+      add(sml[wave + w].x, sml[wave + w].y, o1);
+    }
+  }
+  if (!live || half != 0) { return; }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  uint16_t* op = A.out + token * A.o_tok + (row - (long long)token * A.hq) * D + c;
+  if constexpr (C == 4) {
+    *reinterpret_cast<u32x2_t*>(op) =
+        u32x2_t{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+  } else if constexpr (C == 2) {
+    *reinterpret_cast<uint32_t*>(op) = pack_bf16x2(o[0] * inv, o[1] * inv);
+  } else {
+    *op = (uint16_t)pack_bf16x2(o[0] * inv, 0.0f);
+  }
+}
+
+template <int D, int NR>
+hipError_t
+launch_stream(const PagedArgs& a, hipStream_t s)
+{
+  const int G = a.hq / a.hkv, RB = 16 * NR;
+  const long long phase =
+      a.p_tile ? 0 : (long long)a.p_shares * a.hkv * ((a.tokens * G + RB - 1) / RB);
+  const int blocks = (std::min(a.max_q * G, kPagedShortRows) + RB - 1) / RB;
+  const long long own = a.shorts ? (long long)a.batch * a.s_shares * blocks * a.hkv : 0;
+  hipLaunchKernelGGL((paged_stream_kernel<D, NR>), dim3((unsigned)(phase + own)), dim3(256), 0, s,
+                     a);
+  return hipGetLastError();
+}
+
 template <int D>
 hipError_t
 launch_paged_d(const PagedArgs& a, hipStream_t s)
 {
-  const int rows = a.max_q * (a.hq / a.hkv);
-  const long long blocks = (long long)a.batch * a.hkv * ((rows + 15) / 16);
-  hipLaunchKernelGGL((paged_stream_kernel<D, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  hipError_t e = hipSuccess;
+  const int G = a.hq / a.hkv;
+  const long long phase =
+      a.p_tile ? (long long)a.p_shares * a.hkv * ((a.tokens * G + kTileRows - 1) / kTileRows) : 0;
+  const long long longs =
+      a.longs ? (long long)a.t_shares * a.hkv * (a.tokens * G / kTileRows + a.batch) : 0;
+  if (phase + longs > 0) {
+    hipLaunchKernelGGL(paged_tile_kernel<D>, dim3((unsigned)(phase + longs)), dim3(256), 0, s, a);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && (a.shorts || (a.p_shares > 0 && !a.p_tile))) {
+    e = a.nr == 1 ? launch_stream<D, 1>(a, s) : launch_stream<D, 2>(a, s);
+  }
+  const int parts = paged_parts(a);
+  if (e != hipSuccess || parts == 1) { return e; }
+  const unsigned rows = (unsigned)a.tokens * a.hq;
+  if (parts > 8 && rows < 4096) {
+    hipLaunchKernelGGL((paged_combine_kernel<D, 4>), dim3(rows), dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((paged_combine_kernel<D, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -613,9 +1266,14 @@ paged_kernels_loadable()
       reinterpret_cast<const void*>(&rope_kernel<8>),
       reinterpret_cast<const void*>(&rope_kernel<2>),
       reinterpret_cast<const void*>(&rope_kernel<1>),
-      reinterpret_cast<const void*>(&paged_stream_kernel<128, 1>),
-      reinterpret_cast<const void*>(&paged_stream_kernel<64, 1>),
-      reinterpret_cast<const void*>(&paged_stream_kernel<32, 1>),
+#define U15H_FN(D)                                                     \
+  reinterpret_cast<const void*>(&paged_stream_kernel<D, 1>),           \
+      reinterpret_cast<const void*>(&paged_stream_kernel<D, 2>),       \
+      reinterpret_cast<const void*>(&paged_tile_kernel<D>),            \
+      reinterpret_cast<const void*>(&paged_combine_kernel<D, 1>),      \
+      reinterpret_cast<const void*>(&paged_combine_kernel<D, 4>),
+      U15H_FN(128) U15H_FN(64) U15H_FN(32)
+#undef U15H_FN
   };
   for (const void* f : fns) {
     hipFuncAttributes a;
