@@ -509,7 +509,7 @@ typedef struct {
  * join through partial results in the context's attention scratch (u15h_sdpa;
  * without it every sequence walks the prefix itself).
  * Limits: hq % kv_heads == 0, hq <= 4096, batch <= 65536, tokens <= 2^22,
- * max_kv and prefix_len < 2^30. */
+ * max_kv and prefix_len < 2^29. */
 u15h_status u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream,
                                  const u15h_paged_kv* kv,
                                  const u15h_paged_batch* batch,

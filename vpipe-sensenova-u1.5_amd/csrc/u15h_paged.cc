@@ -18,7 +18,7 @@ using u15h::RopeArgs;
 constexpr int kMaxHeads = 4096;
 constexpr int kMaxTokens = 1 << 22;
 constexpr int kMaxBatch = 1 << 16;
-constexpr int kMaxKeys = 1 << 30;
+constexpr int kMaxKeys = 1 << 29;
 constexpr long long kMaxStride = 1LL << 40;      // elements between rows or pages
 constexpr double kPi = 3.14159265358979323846;
 
@@ -145,60 +145,90 @@ check_rows(u15h_ctx* ctx, const char* what, const char* name, const void* p, int
   return U15H_OK;
 }
 
-// Shares of `keys` so that `base` workgroups each become about `want`, none
-// under `least` keys; the chunk in keys, a multiple of 128.
-void
-shares_of(long long keys, long long base, long long want, int least, int* shares, int* chunk)
+int
+round_up(long long v, int to)
 {
-  long long n = std::max(1LL, std::min(want / std::max(base, 1LL), keys / least));
-  long long c = ((keys + n - 1) / n + 127) / 128 * 128;
-  c = std::max(c, 128LL);
-  *chunk = (int)c;
-  *shares = (int)std::max(1LL, (keys + c - 1) / c);
+  return (int)((v + to - 1) / to * to);
 }
 
-// How a call is cut (PagedArgs): what the prefix phase and the sequences'
-// workgroups walk.
+// `keys` in at most `n` shares of a multiple of 128.
+void
+cut(long long keys, long long n, int* shares, int* chunk)
+{
+  *chunk = std::max(round_up((keys + n - 1) / n, 128), 128);
+  *shares = (int)std::max((keys + *chunk - 1) / *chunk, 1LL);
+}
+
+// How a call is cut (PagedArgs): what the prefix's workgroups and the
+// sequences' walk.  Lengths are known to their bounds only; own keys are taken
+// as half of max_kv on the mean.
 void
 plan(PagedArgs& a, int cus, void* ws, size_t bytes)
 {
   const int G = a.hq / a.hkv;
-  const long long R1 = (long long)a.max_q * G;
-  a.longs = R1 > u15h::kPagedShortRows;
+  const long long rows1 = (long long)a.max_q * G;       // of a sequence, at most
+  const long long rows = (long long)a.tokens * G;       // of a kv head
+  a.longs = rows1 > u15h::kPagedShortRows;
   a.shorts = G <= u15h::kPagedShortRows;
   a.ws = static_cast<float*>(ws);
-  const long long rows = (long long)a.tokens * G;
-  const int want = 1 * cus;
-  const int pwant = 1 * cus;
-  const int least = 256;
-  bool phase = a.prefix >= 256 && a.batch >= 2 && (long long)a.batch * a.prefix >= 4096 &&
-               rows / a.batch <= 64;
-  a.nr = R1 <= 16 || !a.shorts ? 1 : 2;
-  for (int tries = 0; tries < 2; ++tries, phase = false) {
+  a.nr = rows1 <= 16 || !a.shorts ? 1 : 2;
+  const long long pieces = ws == nullptr ? 1 : 64;      // most shares of anything
+
+  // us: a 64-key tile of one workgroup, the streaming of own keys, a part's
+  // round trip
+  const double tile = a.d == 128 ? 0.94 : a.d == 64 ? 0.63 : 0.52;
+  const double own = (double)a.batch * a.max_kv * 0.5 * a.hkv * a.d * 4 / 5e6;
+  const double part = (double)a.tokens * a.hq * (a.d + 2) * 8 / 4e6;
+
+  // The prefix for all rows at once: where at least 4096 keys would be walked
+  // again and sequences are short.
+  bool phase = ws != nullptr && a.batch >= 2 && a.prefix >= 256 &&
+               (long long)a.batch * a.prefix >= 4096 && rows / a.batch <= 256;
+  for (;; phase = false) {
     a.p_shares = 0;
-    if (phase && ws != nullptr) {
-      a.p_tile = rows > 64;
+    if (phase) {
+      a.p_tile = rows > u15h::kPagedShortRows;
       if (!a.p_tile && rows > 16) { a.nr = 2; }
       const int rb = a.p_tile ? 128 : 16 * a.nr;
-      shares_of(a.prefix, (rows + rb - 1) / rb * a.hkv, pwant, least, &a.p_shares, &a.p_chunk);
+      const long long blocks = (rows + rb - 1) / rb * a.hkv;
+      double best = 1e30;
+      for (int n = 1; n <= pieces; ++n) {
+        int shares, chunk;
+        cut(a.prefix, n, &shares, &chunk);
+        const double items = (double)blocks * shares, walk = chunk / 64.0 * tile;
+        // beside streaming workgroups a tile takes half as long again; two
+        // tile workgroups on a CU take twice as long
+        const double busy = std::max(1.5 * walk, items / cus * walk);
+        const double us = std::max(own, busy + 5.0) + part * shares;
+        if (us < best) {
+          best = us;
+          a.p_shares = shares;
+          a.p_chunk = chunk;
+        }
+      }
     }
-    const long long keys = (a.p_shares > 0 ? 0 : (a.prefix + 63) / 64 * 64) + a.max_kv;
+    // What a sequence walks itself, in shares of 256 keys or more.  One long
+    // sequence: a workgroup a CU fills the memory's rate.  Several: finer, as
+    // their lengths differ.
+    const long long keys =
+        (a.p_shares > 0 ? 0 : round_up(a.prefix, 64)) + (long long)a.max_kv;
     const int rb = 16 * a.nr;
-    const long long sblocks = (std::min<long long>(R1, u15h::kPagedShortRows) + rb - 1) / rb;
-    shares_of(keys, sblocks * a.hkv * a.batch, want, least, &a.s_shares, &a.s_chunk);
-    shares_of(keys, (rows / 128 + a.batch) * a.hkv, want, least, &a.t_shares, &a.t_chunk);
-    if (ws == nullptr) { a.s_shares = a.t_shares = 1; }
+    const long long s_want = (a.batch == 1 ? 1LL : 4LL) * cus;
+    const long long t_want = (a.batch == 1 ? 1LL : 2LL) * cus;
+    const long long s_items = (std::min<long long>(rows1, u15h::kPagedShortRows) + rb - 1) / rb *
+                              a.hkv * a.batch;
+    const long long t_items = (rows / 128 + a.batch) * a.hkv;
+    const long long most = std::max(1LL, std::min(keys / 256, pieces));
+    cut(keys, std::max(1LL, std::min(s_want / s_items, most)), &a.s_shares, &a.s_chunk);
+    cut(keys, std::max(1LL, std::min(t_want / t_items, most)), &a.t_shares, &a.t_chunk);
     while (u15h::paged_ws_bytes(a) > bytes && a.s_shares + a.t_shares > 2) {
-      if (a.s_shares > 1) { --a.s_shares; }
-      if (a.t_shares > 1) { --a.t_shares; }
-      a.s_chunk = (int)(((keys + a.s_shares - 1) / a.s_shares + 127) / 128 * 128);
-      a.t_chunk = (int)(((keys + a.t_shares - 1) / a.t_shares + 127) / 128 * 128);
+      cut(keys, std::max(a.s_shares - 1, 1), &a.s_shares, &a.s_chunk);
+      cut(keys, std::max(a.t_shares - 1, 1), &a.t_shares, &a.t_chunk);
     }
     while (u15h::paged_ws_bytes(a) > bytes && a.p_shares > 1) {
-      --a.p_shares;
-      a.p_chunk = (int)(((a.prefix + a.p_shares - 1) / a.p_shares + 127) / 128 * 128);
+      cut(a.prefix, a.p_shares - 1, &a.p_shares, &a.p_chunk);
     }
-    if (u15h::paged_ws_bytes(a) <= bytes) { break; }
+    if (!phase || u15h::paged_ws_bytes(a) <= bytes) { break; }
   }
 }
 
@@ -423,7 +453,7 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
   a.kv_len = bt->kv_len;
   a.table = bt->table;
   a.prefix_table = bt->prefix_table;
-  a.table_stride = bt->table_stride;
+  a.table_stride = bt->max_kv > 0 ? bt->table_stride : 0;
   a.prefix = bt->prefix_len;
   a.batch = bt->batch;
   a.tokens = bt->tokens;

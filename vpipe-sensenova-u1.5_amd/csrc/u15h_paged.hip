@@ -134,14 +134,109 @@ constexpr int kRopePairs = kRopeMaxHeadDim / 2;
 // workgroups enough.
 constexpr int kRopeGroup = 4;
 
+struct RopeGrid {
+  int group;              // tokens of a workgroup
+  int heads;              // of its blockIdx.y's heads
+  int units;              // of a head
+  int lanes;              // threads of a unit: heads at once
+};
+
+// A thread keeps its unit and steps over the (token, head) pairs, `lanes` of
+// them at a time over the workgroup.  Its first columns are on their way while
+// the angles are formed, later ones while the ones before are turned.
 template <int VEC>
 __global__ __launch_bounds__(256) void
-rope_kernel(const RopeArgs A, int group, int units, uint32_t units_inv)
+rope_kernel(const RopeArgs A, const RopeGrid R)
 {
   __shared__ float2 cs[kRopeGroup * kRopePairs];
   const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * group;
-  const int nt = min(group, A.tokens - t0);
+  const int t0 = blockIdx.x * R.group;
+  const int nt = min(R.group, A.tokens - t0);
+  const int h0 = blockIdx.y * R.heads;
+  const int heads = min(R.heads, A.q.heads + A.k.heads + A.v.heads - h0);
+
+  struct Item {
+    Cols<VEC> a, b;
+  };
+  RopeUnit u;
+  auto fetch = [&](int tok, int head, Item& I) {
+    const int t = t0 + tok;
+    int h = h0 + head;
+    const RopeRows& S = h < A.q.heads ? A.q : h < A.q.heads + A.k.heads ? A.k : A.v;
+    h -= h < A.q.heads ? 0 : h < A.q.heads + A.k.heads ? A.q.heads : A.q.heads + A.k.heads;
+    const uint16_t* x = S.x + t * S.x_tok + h * S.x_head;
+    I.a = load_cols<VEC>(x + u.a);
+    if (u.b >= 0) { I.b = load_cols<VEC>(x + u.b); }
+  };
+  auto finish = [&](int tok, int head, Item& I) {
+    const int t = t0 + tok;
+    int h = h0 + head;
+    bool turned = u.pair >= 0;
+    uint16_t* y;
+    if (A.slot != nullptr) {
+      const int slot = A.slot[t];
+      if ((unsigned)slot >= (unsigned)A.slots) { return; }
+      if (h < A.q.heads) {
+        y = A.q.y + t * A.q.y_tok + h * A.q.y_head;
+      } else {
+        h -= A.q.heads;
+        const bool key = h < A.k.heads;
+        h -= key ? 0 : A.k.heads;
+        turned = turned && key;
+        y = (key ? A.k.y : A.v.y) + (long long)(slot >> A.page_log2) * A.page_stride +
+            (((long long)h << A.page_log2) + (slot & ((1 << A.page_log2) - 1))) * A.d;
+      }
+    } else {
+      y = A.q.y + t * A.q.y_tok + h * A.q.y_head;
+    }
+    const float2* f = cs + tok * A.pairs + (turned ? u.pair : 0);
+    Cols<VEC>& a = I.a;
+    Cols<VEC>& b = I.b;
+    if (u.b >= 0) {
+      if (turned) {
+#pragma unroll
+        for (int e = 0; e < (VEC + 1) / 2; ++e) {
+          const float2 f0 = f[2 * e];
+          const float a0 = bf16_lo(a.w[e]), b0 = bf16_lo(b.w[e]);
+          float a1 = 0.0f, b1 = 0.0f;
+          float2 f1 = make_float2(0.0f, 0.0f);
+          if constexpr (VEC > 1) {
+            f1 = f[2 * e + 1];
+            a1 = bf16_hi(a.w[e]);
+            b1 = bf16_hi(b.w[e]);
+          }
+          a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, a1 * f1.x - b1 * f1.y);
+          b.w[e] = pack_bf16x2(b0 * f0.x + a0 * f0.y, b1 * f1.x + a1 * f1.y);
+        }
+      }
+      store_cols<VEC>(y + u.b, b);
+    } else if (turned) {
+#pragma unroll
+      for (int e = 0; e < VEC / 2; ++e) {
+        const float2 f0 = f[e];
+        const float a0 = bf16_lo(a.w[e]), b0 = bf16_hi(a.w[e]);
+        a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, b0 * f0.x + a0 * f0.y);
+      }
+    }
+    store_cols<VEC>(y + u.a, a);
+  };
+
+  // units past a thread's share of 256 (a head of many single columns) go round
+  // by round; all but those have one round
+  const int lane = R.lanes > 1 ? tid / R.units : 0;
+  const bool idle = lane >= R.lanes;
+  int tok = 0, head = lane;
+  while (head >= heads && tok < nt) {
+    head -= heads;
+    ++tok;
+  }
+  int unit = R.lanes > 1 ? tid - lane * R.units : tid;
+  Item I;
+  bool more = !idle && unit < R.units && tok < nt;
+  if (more) {
+    u = rope_unit<VEC>(A, unit);
+    fetch(tok, head, I);
+  }
 
   for (int i = tid; i < nt * A.pairs; i += 256) {
     const int tok = i / A.pairs, pair = i % A.pairs;
@@ -162,66 +257,29 @@ rope_kernel(const RopeArgs A, int group, int units, uint32_t units_inv)
   }
   __syncthreads();
 
-  const int heads = A.q.heads + A.k.heads + A.v.heads;
-  const int per = units * heads;
-  for (int tok = 0; tok < nt; ++tok) {
-    const int t = t0 + tok;
-    long long at = 0;                    // the slot's place in head 0's page
-    if (A.slot != nullptr) {
-      const int slot = A.slot[t];
-      if ((unsigned)slot >= (unsigned)A.slots) { continue; }
-      at = (long long)(slot >> A.page_log2) * A.page_stride +
-           (long long)(slot & ((1 << A.page_log2) - 1)) * A.d;
+  while (more) {
+    int tok1 = tok, head1 = head + R.lanes;
+    while (head1 >= heads && tok1 < nt) {
+      head1 -= heads;
+      ++tok1;
     }
-    const float2* f = cs + tok * A.pairs;
-    for (int i = tid; i < per; i += 256) {
-      int h = units_inv != 0 ? (int)__umulhi((uint32_t)i, units_inv) : i;
-      const int u = i - h * units;
-      const uint16_t* x;
-      uint16_t* y;
-      bool turned = true;
-      if (h < A.q.heads) {
-        x = A.q.x + t * A.q.x_tok + h * A.q.x_head;
-        y = A.q.y + t * A.q.y_tok + h * A.q.y_head;
-      } else {
-        h -= A.q.heads;
-        turned = h < A.k.heads;
-        const RopeRows& R = turned ? A.k : A.v;
-        h = turned ? h : h - A.k.heads;
-        x = R.x + t * R.x_tok + h * R.x_head;
-        y = R.y + at + ((long long)h << A.page_log2) * A.d;
-      }
-      const RopeUnit U = rope_unit<VEC>(A, u);
-      Cols<VEC> a = load_cols<VEC>(x + U.a);
-      if (U.b >= 0) {
-        Cols<VEC> b = load_cols<VEC>(x + U.b);
-        if (turned && U.pair >= 0) {
-#pragma unroll
-          for (int e = 0; e < (VEC + 1) / 2; ++e) {
-            const float2 f0 = f[U.pair + 2 * e];
-            const float a0 = bf16_lo(a.w[e]), b0 = bf16_lo(b.w[e]);
-            float a1 = 0.0f, b1 = 0.0f;
-            float2 f1 = make_float2(0.0f, 0.0f);
-            if constexpr (VEC > 1) {
-              f1 = f[U.pair + 2 * e + 1];
-              a1 = bf16_hi(a.w[e]);
-              b1 = bf16_hi(b.w[e]);
-            }
-            a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, a1 * f1.x - b1 * f1.y);
-            b.w[e] = pack_bf16x2(b0 * f0.x + a0 * f0.y, b1 * f1.x + a1 * f1.y);
-          }
-        }
-        store_cols<VEC>(y + U.b, b);
-      } else if (turned && U.pair >= 0) {
-#pragma unroll
-        for (int e = 0; e < VEC / 2; ++e) {
-          const float2 f0 = f[U.pair + e];
-          const float a0 = bf16_lo(a.w[e]), b0 = bf16_hi(a.w[e]);
-          a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, b0 * f0.x + a0 * f0.y);
-        }
-      }
-      store_cols<VEC>(y + U.a, a);
+    if (tok1 >= nt && R.lanes == 1 && unit + 256 < R.units) {
+      // the thread's next unit, from the first pair on
+      finish(tok, head, I);
+      unit += 256;
+      u = rope_unit<VEC>(A, unit);
+      tok = 0;
+      head = 0;
+      fetch(tok, head, I);
+      continue;
     }
+    Item J;
+    more = tok1 < nt;
+    if (more) { fetch(tok1, head1, J); }
+    finish(tok, head, I);
+    I = J;
+    tok = tok1;
+    head = head1;
   }
 }
 
@@ -235,12 +293,18 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
     units += a.part[p].width / ((a.neighbours && VEC > 1) ? VEC : 2 * VEC);
   }
   units += columns / VEC;
-  const int group = a.tokens >= 1024 ? kRopeGroup : 1;
-  // i / units as a product's high word: exact while i * units < 2^32, and i <
-  // 4096 heads * 512; one unit a head (2^32, so 0) needs none
-  const uint32_t inv = (uint32_t)(((1ull << 32) + units - 1) / units);
-  hipLaunchKernelGGL(rope_kernel<VEC>, dim3((unsigned)((a.tokens + group - 1) / group)),
-                     dim3(256), 0, s, a, group, units, inv);
+  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  RopeGrid g;
+  g.group = a.tokens >= 1024 ? kRopeGroup : 1;
+  const int groups = (a.tokens + g.group - 1) / g.group;
+  // few tokens: their heads over several workgroups, 128 units each or more
+  int cut = 1;
+  while (groups * cut < 256 && heads * units / (cut * 2) >= 128) { cut *= 2; }
+  g.heads = (heads + cut - 1) / cut;
+  g.units = units;
+  g.lanes = std::max(1, 256 / units);
+  hipLaunchKernelGGL(rope_kernel<VEC>, dim3((unsigned)groups, (heads + g.heads - 1) / g.heads),
+                     dim3(256), 0, s, a, g);
   return hipGetLastError();
 }
 
@@ -249,7 +313,7 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
 // of prefix_table's pages, then a sequence's own.  Keys are walked in tiles of
 // 32; the prefix's last tile and the own keys' first do not share one.
 //
-// paged_stream_kernel: up to 16 * NR rows of one kv head a workgroup, four
+// stream_item: up to 16 * NR rows of one kv head a workgroup, four
 // waves that each take every fourth tile.  Nothing is staged: a wave's tile
 // goes from memory to the registers of the matrix instructions (16x16x32).
 //  - Scores are transposed, S^T = K Q^T.  The key operand is 16 keys x 32
@@ -358,30 +422,33 @@ struct Walk {
 };
 
 // One workgroup: up to RB rows of a kv head over a share of keys.  The first
-// workgroups take the prefix's shares for all rows (where the plan has them on
-// this kernel), the others a sequence each.
+// items are the prefix's shares for all rows (where the plan has them on this
+// kernel), the others a sequence each.  o0 to o3: RB * D floats of LDS a wave.
 template <int D, int NR>
-__global__ __launch_bounds__(256) void
-paged_stream_kernel(const PagedArgs A)
+__device__ __forceinline__ void
+stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float* o3,
+            float (*sm)[16 * NR], float (*sl)[16 * NR])
 {
   constexpr int W = 4;                       // waves
   constexpr int RB = 16 * NR;                // rows
   constexpr int KS = D / 32;                 // matrix steps of a score
   constexpr int DPL = D / 16;                // columns of V a lane
   constexpr int VW = DPL / 2;                // ... in words
-  constexpr int PITCH = D + 4;
-  __shared__ __attribute__((aligned(16))) float so[W * RB * PITCH];
-  __shared__ float sm[W][RB], sl[W][RB];
+
+  auto so = [&](int w) { return w == 0 ? o0 : w == 1 ? o1 : w == 2 ? o2 : o3; };
+  const int tid = threadIdx.x;
+  const int wave = uniform(tid >> 6);
+  const int lane = tid & 63;
+  const int lr = lane & 15;
+  const int g = lane >> 4;
 
   const int G = A.hq / A.hkv;
-  int item = blockIdx.x;
   const int p_shares = A.p_tile ? 0 : A.p_shares;
   const int p_blocks = (A.tokens * G + RB - 1) / RB;
   const int p_items = p_shares * p_blocks * A.hkv;
   const bool phase = item < p_items;
-  Sequence S;
+  int kvh, row0, part, share, share_tiles, seq = 0;
   Walk K;
-  int kvh, row0, part, share, share_tiles;
   if (phase) {
     // the blocks of rows of one share of one head 8 apart: one die's L2
     const int runs = p_shares * A.hkv;
@@ -396,8 +463,8 @@ paged_stream_kernel(const PagedArgs A)
     kvh = run % A.hkv;
     share = run / A.hkv;
     part = share;
-    S = {0, A.tokens, 0};
-    K = {nullptr, A.prefix, 0, (A.prefix + 31) / 32, 0, 0};
+    K.table = nullptr;
+    K.prefix = A.prefix;
     share_tiles = A.p_chunk / 32;
   } else {
     item -= p_items;
@@ -407,20 +474,38 @@ paged_stream_kernel(const PagedArgs A)
     row0 = item % blocks * RB;
     item /= blocks;
     share = item % A.s_shares;
-    const int b = item / A.s_shares;
+    seq = item / A.s_shares;
     part = A.p_shares + share;
-    S = sequence(A, b);
-    if (S.n * G > kPagedShortRows) { return; }
-    K.table = A.table + (long long)b * A.table_stride;
+    K.table = A.table + (long long)seq * A.table_stride;
     K.prefix = A.p_shares > 0 ? 0 : A.prefix;
-    K.prefix_tiles = (K.prefix + 31) / 32;
-    // own keys that the block's last row sees
-    const int last = (min(S.n * G, row0 + RB) - 1) / G;
-    K.keys = A.causal ? max(S.keys - S.n + last + 1, 0) : S.keys;
     share_tiles = A.s_chunk / 32;
   }
+  K.prefix_tiles = (K.prefix + 31) / 32;
+
+  // This wave's i-th tile is tile0 + W * i; lane 2 (i % 32) + block holds the
+  // page of its block of 16 keys, as the table has it (-1 past the table).
+  const int tile0 = share * share_tiles + wave;
+  auto number = [&](int group) {
+    const int tile = tile0 + W * (group * 32 + (lane >> 1));
+    const bool pre = tile < K.prefix_tiles;
+    const int key = (pre ? tile : tile - K.prefix_tiles) * 32 + (lane & 1) * 16;
+    const int at = key >> A.page_log2;
+    int id = -1;
+    if (pre ? key < K.prefix : (!phase && at < A.table_stride)) {
+      id = (pre ? A.prefix_table : K.table)[at];
+    }
+    return id;
+  };
+  // the first numbers need no length and are on their way beside the lengths
+  int ids = number(0);
+
+  Sequence S = {0, A.tokens, 0};
+  if (!phase) { S = sequence(A, seq); }
   const int rows = S.n * G;
-  if (row0 >= rows) { return; }
+  if (row0 >= rows || (!phase && rows > kPagedShortRows)) { return; }
+  // own keys that the block's last row sees
+  const int last = (min(rows, row0 + RB) - 1) / G;
+  K.keys = phase ? 0 : A.causal ? max(S.keys - S.n + last + 1, 0) : S.keys;
   const bool direct = paged_parts(A) == 1;
   const int tiles = K.prefix_tiles + (K.keys + 31) / 32;
   const bool last_share = share == (phase ? p_shares : A.s_shares) - 1;
@@ -429,12 +514,6 @@ paged_stream_kernel(const PagedArgs A)
   if (!phase && last_share) {
     mark_parts(A, part + 1, paged_parts(A), S.first, G, kvh, row0, min(rows - row0, RB), kNoKey);
   }
-
-  const int tid = threadIdx.x;
-  const int wave = uniform(tid >> 6);
-  const int lane = tid & 63;
-  const int lr = lane & 15;
-  const int g = lane >> 4;
 
   i32x4_t qf[NR][KS];
   int lim[NR];                               // last own key that the row sees
@@ -452,21 +531,15 @@ paged_stream_kernel(const PagedArgs A)
   }
   const int lim0 = A.causal ? S.keys - S.n + row0 / G : S.keys - 1;   // the first row's
 
-  // This wave's i-th tile is tile0 + W * i; lane 2 (i % 32) + block holds the
-  // page of its block of 16 keys, -1 where it has none.
-  const int tile0 = K.begin + wave;
+  // a block's page, -1 where it has no keys or its number is not a page
   const int mine = (K.end - tile0 + W - 1) / W;
-  auto pages_of = [&](int group) {
+  auto checked = [&](int id, int group) {
     const int tile = tile0 + W * (group * 32 + (lane >> 1));
     const bool pre = tile < K.prefix_tiles;
     const int key = (pre ? tile : tile - K.prefix_tiles) * 32 + (lane & 1) * 16;
-    int id = -1;
-    if (tile < K.end && key < (pre ? K.prefix : K.keys)) {
-      id = (pre ? A.prefix_table : K.table)[key >> A.page_log2];
-    }
-    return (unsigned)id < (unsigned)A.pages ? id : -1;
+    return key < (pre ? K.prefix : K.keys) && (unsigned)id < (unsigned)A.pages ? id : -1;
   };
-  int ids = pages_of(0);
+  ids = checked(ids, 0);
 
   const int koff = (lr * D + g * 8) * 2;
   const int voff = (4 * g * D + lr * DPL) * 2;
@@ -561,7 +634,7 @@ paged_stream_kernel(const PagedArgs A)
     }
     const bool more = i + 1 < mine;
     const bool refill = ((i + 1) & 31) == 0;
-    if (refill && more) { ids = pages_of((i + 1) >> 5); }
+    if (refill && more) { ids = checked(number((i + 1) >> 5), (i + 1) >> 5); }
     if (more) { load_k(i + 1); }
 
     if (key0 + 31 > (pre ? K.prefix - 1 : lim0) || (id0 | id1) < 0) {
@@ -624,12 +697,15 @@ paged_stream_kernel(const PagedArgs A)
       sm[wave][n * 16 + lr] = m[n];
       sl[wave][n * 16 + lr] = lt;
     }
-    float* to = so + (wave * RB + n * 16 + lr) * PITCH;
+    // row r's 16-byte chunk c at c ^ r: 16 rows' chunk c spread over the banks
+    float* to = so(wave) + (n * 16 + lr) * D;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int c = (4 * g + r) * DPL;
 #pragma unroll
-      for (int j = 0; j < DPL; ++j) { to[c + j] = o[n][j][r]; }
+      for (int j = 0; j < DPL; ++j) {
+        const int c = (4 * g + r) * DPL + j;
+        to[(((c >> 2) ^ lr) & (D / 4 - 1)) * 4 + (c & 3)] = o[n][j][r];
+      }
     }
   }
   __syncthreads();
@@ -645,7 +721,8 @@ paged_stream_kernel(const PagedArgs A)
     for (int w = 0; w < W; ++w) {
       const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - top);
       sum += f * sl[w][r];
-      acc += f * *reinterpret_cast<const f32x4_t*>(so + (w * RB + r) * PITCH + c);
+      acc += f * *reinterpret_cast<const f32x4_t*>(
+                     so(w) + r * D + (((c >> 2) ^ (r & 15)) & (D / 4 - 1)) * 4);
     }
     const int row = row0 + r;
     if (!direct) {
@@ -663,7 +740,7 @@ paged_stream_kernel(const PagedArgs A)
   }
 }
 
-// paged_tile_kernel: 128 rows of one kv head a workgroup, for sequences (or
+// tile_item: 128 rows of one kv head a workgroup, for sequences (or
 // prefixes of many) whose products outweigh their keys' bytes.  The tile loop is
 // attention_kernel's: scores and output transposed on 32x32x16 products, keys
 // and values of 64-key tiles copied from memory to LDS and read there by all
@@ -708,13 +785,40 @@ vswz(int r)
 
 constexpr int kTileRows = 128;
 
-// Block `nb` of the tile kernel's rows of all sequences: the sequence, which
-// has the blocks from first_block(b) = rows before it / 128 + b on (one more
-// than it can need at most), and the block within it.
+// Block `nb` of the long sequences' rows, in blocks of kTileRows: its sequence
+// (-1: there is none) and its place within it.  Up to 64 sequences, those with
+// the most keys come first, each with its last block, which under the causal
+// mask sees the most keys, first: the longest workgroups start early.  (  More sequences
+// are taken as they come, b's blocks from rows before it / 128 + b on, which
+// leaves each one block or two that have no rows.
 __device__ __forceinline__ int
 sequence_of_block(const PagedArgs& A, int G, int nb, int* local)
 {
   const int lane = threadIdx.x & 63;
+  if (A.batch <= 64) {
+    int n = 0, keys = -1;
+    if (lane < A.batch) {
+      int s0 = lane, s1 = lane + 1;
+      if (A.q_start != nullptr) {
+        s0 = min(max(A.q_start[lane], 0), A.tokens);
+        s1 = min(max(A.q_start[lane + 1], s0), A.tokens);
+      }
+      const int rows = min(s1 - s0, A.max_q) * G;
+      n = rows > kPagedShortRows ? (rows + kTileRows - 1) / kTileRows : 0;
+      keys = A.kv_len[lane];
+    }
+    int start = 0;
+    for (int j = 0; j < A.batch; ++j) {
+      const int kj = __builtin_amdgcn_readlane(keys, j);
+      const bool before = kj > keys || (kj == keys && j < lane);
+      start += before ? __builtin_amdgcn_readlane(n, j) : 0;
+    }
+    const unsigned long long mine = __ballot(nb >= start && nb < start + n);
+    if (mine == 0) { return -1; }
+    const int seq = __builtin_ctzll(mine);
+    *local = __builtin_amdgcn_readlane(n, seq) - 1 - (nb - __builtin_amdgcn_readlane(start, seq));
+    return seq;
+  }
   int count = 0, start = 0;
   for (int b0 = 0; b0 < A.batch; b0 += 64) {
     const int b = b0 + lane;
@@ -735,29 +839,25 @@ sequence_of_block(const PagedArgs& A, int G, int nb, int* local)
 }
 
 template <int D>
-__global__ __launch_bounds__(256, 2) void
-paged_tile_kernel(const PagedArgs A)
+__device__ __forceinline__ void
+tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, uint16_t* vs0,
+          uint16_t* vs1)
 {
   constexpr int BK = 64;                     // keys of a tile
   constexpr int KCH = D / 8;                 // 16-byte chunks of a key
   constexpr int NDS = D / 16;                // matrix steps of the scores
   constexpr int NCB = D / 32;                // blocks of 32 columns of O
   constexpr int CPW = D / 32;                // 1 KiB copies of a wave's 16 keys
-  __shared__ __attribute__((aligned(16))) uint16_t ks0[BK * D];
-  __shared__ __attribute__((aligned(16))) uint16_t ks1[BK * D];
-  __shared__ __attribute__((aligned(16))) uint16_t vs0[BK * D];
-  __shared__ __attribute__((aligned(16))) uint16_t vs1[BK * D];
 
   const int G = A.hq / A.hkv;
   const int p_blocks = (A.tokens * G + kTileRows - 1) / kTileRows;
   const int p_items = A.p_tile ? A.p_shares * p_blocks * A.hkv : 0;
-  const bool phase = (int)blockIdx.x < p_items;
+  const bool phase = b < p_items;
   Sequence S;
   const int32_t* table = nullptr;
   int prefix = A.prefix, kvh, row0, part, share, shares, chunk;
   if (phase) {
     // run by run of one head's keys, cut in 8 ranges, one per die
-    const int b = blockIdx.x;
     const int item = p_items % 8 == 0 ? (b % 8) * (p_items / 8) + b / 8 : b;
     row0 = item % p_blocks * kTileRows;
     share = item / p_blocks % A.p_shares;
@@ -767,14 +867,14 @@ paged_tile_kernel(const PagedArgs A)
     chunk = A.p_chunk;
     S = {0, A.tokens, 0};
   } else {
-    const int b = blockIdx.x - p_items, items = gridDim.x - p_items;
+    b -= p_items;
+    items -= p_items;
     int item = items % 8 == 0 ? (b % 8) * (items / 8) + b / 8 : b;
     const int blocks = A.tokens * G / kTileRows + A.batch;
     share = item % A.t_shares;
     item /= A.t_shares;
     int local;
-    // the last blocks of a causal sequence see most keys: they go first
-    const int seq = sequence_of_block(A, G, blocks - 1 - item % blocks, &local);
+    const int seq = sequence_of_block(A, G, item % blocks, &local);
     kvh = item / blocks;
     part = A.p_shares + share;
     shares = A.t_shares;
@@ -1091,22 +1191,52 @@ paged_tile_kernel(const PagedArgs A)
   }
 }
 
+// The kernel: workgroups of tile items first, the longest, then of streaming
+// ones, which fill the CUs as those end (256 sequences behind 32768 keys: 167 us
+// with almost no own keys, 56 with almost no prefix, 182 with both; a streaming
+// workgroup beside every tile one from the start: 212).  TILE or STREAM alone
+// where a call has only those.
+template <int D, int NR, bool TILE, bool STREAM>
+__global__ __launch_bounds__(256, TILE ? 2 : 1) void
+paged_kernel(const PagedArgs A, int tile_items)
+{
+  constexpr int kBuf = TILE ? 64 * D : 32 * NR * D;     // in 2 bytes
+  __shared__ __attribute__((aligned(16))) uint16_t b0[kBuf];
+  __shared__ __attribute__((aligned(16))) uint16_t b1[kBuf];
+  __shared__ __attribute__((aligned(16))) uint16_t b2[kBuf];
+  __shared__ __attribute__((aligned(16))) uint16_t b3[kBuf];
+  if constexpr (TILE) {
+    if (!STREAM || (int)blockIdx.x < tile_items) {
+      tile_item<D>(A, blockIdx.x, tile_items, b0, b1, b2, b3);
+      return;
+    }
+  }
+  if constexpr (STREAM) {
+    __shared__ float sm[4][16 * NR], sl[4][16 * NR];
+    stream_item<D, NR>(A, blockIdx.x - tile_items, reinterpret_cast<float*>(b0),
+                       reinterpret_cast<float*>(b1), reinterpret_cast<float*>(b2),
+                       reinterpret_cast<float*>(b3), sm, sl);
+  }
+}
+
 // Whether a token is a row of some sequence.
 __device__ __forceinline__ bool
 in_sequence(const PagedArgs& A, int token)
 {
   if (A.q_start == nullptr) { return token < A.batch; }
-  int lo = 0, hi = A.batch;                  // the last b with q_start[b] <= token
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (A.q_start[mid] <= token) {
-      lo = mid;
-    } else {
-      hi = mid;
-    }
+  // the last b with q_start[b] <= token, 64 at a time
+  const int lane = threadIdx.x & 63;
+  int b = -1, first = 0;
+  for (int b0 = 0; b0 < A.batch; b0 += 64) {
+    const int s0 = b0 + lane < A.batch ? A.q_start[b0 + lane] : INT_MAX;
+    const unsigned long long below = __ballot(s0 <= token);
+    if (below == 0) { break; }
+    const int last = 63 - __builtin_clzll(below);
+    b = b0 + last;
+    first = max(__builtin_amdgcn_readlane(s0, last), 0);
+    if (last < 63) { break; }
   }
-  const Sequence S = sequence(A, lo);
-  return token >= S.first && token - S.first < S.n;
+  return b >= 0 && token < A.q_start[b + 1] && token - first < A.max_q;
 }
 
 // Adds the parts of a row, W waves a row, in the order of the parts:
@@ -1116,7 +1246,7 @@ __global__ __launch_bounds__(256) void
 paged_combine_kernel(const PagedArgs A)
 {
   constexpr int C = D / 32;                  // columns a lane
-  constexpr int kAhead = 8;
+  constexpr int kAhead = W == 1 ? 8 : 4;
   __shared__ float so[4][D];
   __shared__ float2 sml[4];
   const int wave = uniform(threadIdx.x >> 6);
@@ -1126,8 +1256,7 @@ paged_combine_kernel(const PagedArgs A)
   const long long row = (long long)blockIdx.x * (4 / W) + wave / W;
   const int token = (int)(row / A.hq);
   const int n = paged_parts(A);
-  bool live = row < (long long)A.tokens * A.hq && in_sequence(A, token);
-  if (live) { live = part_of(A, 0).ml[row].y != kFinal; }
+  const bool there = row < (long long)A.tokens * A.hq;
 
   float m = -INFINITY, l = 0.0f, o[C];
 #pragma unroll
@@ -1141,7 +1270,7 @@ paged_combine_kernel(const PagedArgs A)
     for (int e = 0; e < C; ++e) { o[e] = __builtin_fmaf(o1[e], f1, o[e] * f0); }
     m = top;
   };
-  if (live) {
+  if (there) {
     for (int p0 = (wave % W) * 2 + half; p0 < n; p0 += 2 * W * kAhead) {
       float2 ml[kAhead];
       float o1[kAhead][C];
@@ -1162,6 +1291,8 @@ paged_combine_kernel(const PagedArgs A)
       for (int i = 0; i < kAhead; ++i) { add(ml[i].x, ml[i].y, o1[i]); }
     }
   }
+  bool live = there && in_sequence(A, token);
+  if (live && A.longs) { live = part_of(A, 0).ml[row].y != kFinal; }
   // the halves, then the waves
   {
     const float m1 = __shfl_xor(m, 32), l1 = __shfl_xor(l, 32);
@@ -1199,44 +1330,37 @@ paged_combine_kernel(const PagedArgs A)
   }
 }
 
-template <int D, int NR>
-hipError_t
-launch_stream(const PagedArgs& a, hipStream_t s)
-{
-  const int G = a.hq / a.hkv, RB = 16 * NR;
-  const long long phase =
-      a.p_tile ? 0 : (long long)a.p_shares * a.hkv * ((a.tokens * G + RB - 1) / RB);
-  const int blocks = (std::min(a.max_q * G, kPagedShortRows) + RB - 1) / RB;
-  const long long own = a.shorts ? (long long)a.batch * a.s_shares * blocks * a.hkv : 0;
-  hipLaunchKernelGGL((paged_stream_kernel<D, NR>), dim3((unsigned)(phase + own)), dim3(256), 0, s,
-                     a);
-  return hipGetLastError();
-}
-
 template <int D>
 hipError_t
 launch_paged_d(const PagedArgs& a, hipStream_t s)
 {
-  hipError_t e = hipSuccess;
-  const int G = a.hq / a.hkv;
-  const long long phase =
-      a.p_tile ? (long long)a.p_shares * a.hkv * ((a.tokens * G + kTileRows - 1) / kTileRows) : 0;
-  const long long longs =
-      a.longs ? (long long)a.t_shares * a.hkv * (a.tokens * G / kTileRows + a.batch) : 0;
-  if (phase + longs > 0) {
-    hipLaunchKernelGGL(paged_tile_kernel<D>, dim3((unsigned)(phase + longs)), dim3(256), 0, s, a);
-    e = hipGetLastError();
+  const int G = a.hq / a.hkv, RB = 16 * a.nr;
+  const long long rows = (long long)a.tokens * G;
+  const long long tiles =
+      (a.p_tile ? a.p_shares * a.hkv * ((rows + kTileRows - 1) / kTileRows) : 0) +
+      (a.longs ? a.t_shares * a.hkv * (rows / kTileRows + a.batch) : 0);
+  const int blocks = (std::min(a.max_q * G, kPagedShortRows) + RB - 1) / RB;
+  const long long streams = (a.p_tile ? 0 : a.p_shares * a.hkv * ((rows + RB - 1) / RB)) +
+                            (a.shorts ? (long long)a.batch * a.s_shares * blocks * a.hkv : 0);
+#define U15H_RUN(NR, T, S)                                                                       \
+  hipLaunchKernelGGL((paged_kernel<D, NR, T, S>), dim3((unsigned)(tiles + streams)), dim3(256), 0, \
+                     s, a, (int)tiles)
+  if (streams == 0) {
+    U15H_RUN(1, true, false);
+  } else if (tiles == 0) {
+    if (a.nr == 1) { U15H_RUN(1, false, true); } else { U15H_RUN(2, false, true); }
+  } else {
+    if (a.nr == 1) { U15H_RUN(1, true, true); } else { U15H_RUN(2, true, true); }
   }
-  if (e == hipSuccess && (a.shorts || (a.p_shares > 0 && !a.p_tile))) {
-    e = a.nr == 1 ? launch_stream<D, 1>(a, s) : launch_stream<D, 2>(a, s);
-  }
+#undef U15H_RUN
+  const hipError_t e = hipGetLastError();
   const int parts = paged_parts(a);
   if (e != hipSuccess || parts == 1) { return e; }
-  const unsigned rows = (unsigned)a.tokens * a.hq;
-  if (parts > 8 && rows < 4096) {
-    hipLaunchKernelGGL((paged_combine_kernel<D, 4>), dim3(rows), dim3(256), 0, s, a);
+  const unsigned outs = (unsigned)a.tokens * a.hq;
+  if (parts > 8 && outs < 4096) {
+    hipLaunchKernelGGL((paged_combine_kernel<D, 4>), dim3(outs), dim3(256), 0, s, a);
   } else {
-    hipLaunchKernelGGL((paged_combine_kernel<D, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_combine_kernel<D, 1>), dim3((outs + 3) / 4), dim3(256), 0, s, a);
   }
   return hipGetLastError();
 }
@@ -1266,10 +1390,12 @@ paged_kernels_loadable()
       reinterpret_cast<const void*>(&rope_kernel<8>),
       reinterpret_cast<const void*>(&rope_kernel<2>),
       reinterpret_cast<const void*>(&rope_kernel<1>),
-#define U15H_FN(D)                                                     \
-  reinterpret_cast<const void*>(&paged_stream_kernel<D, 1>),           \
-      reinterpret_cast<const void*>(&paged_stream_kernel<D, 2>),       \
-      reinterpret_cast<const void*>(&paged_tile_kernel<D>),            \
+#define U15H_FN(D)                                                   \
+  reinterpret_cast<const void*>(&paged_kernel<D, 1, true, false>),   \
+      reinterpret_cast<const void*>(&paged_kernel<D, 1, false, true>), \
+      reinterpret_cast<const void*>(&paged_kernel<D, 2, false, true>), \
+      reinterpret_cast<const void*>(&paged_kernel<D, 1, true, true>),  \
+      reinterpret_cast<const void*>(&paged_kernel<D, 2, true, true>),  \
       reinterpret_cast<const void*>(&paged_combine_kernel<D, 1>),      \
       reinterpret_cast<const void*>(&paged_combine_kernel<D, 4>),
       U15H_FN(128) U15H_FN(64) U15H_FN(32)
