@@ -207,20 +207,36 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
         }
       }
     }
-    // What a sequence walks itself, in shares of 256 keys or more.  One long
-    // sequence: a workgroup a CU fills the memory's rate.  Several: finer, as
-    // their lengths differ.
-    const long long keys =
-        (a.p_shares > 0 ? 0 : round_up(a.prefix, 64)) + (long long)a.max_kv;
+    // What a sequence walks itself, in shares of 256 keys or more: the walk of
+    // the longest against all workgroups' work, which hides it; a tail of uneven
+    // lengths; and what shares cost.
+    const long long before = a.p_shares > 0 ? 0 : round_up(a.prefix, 64);
+    const long long keys = before + a.max_kv, mean = before + a.max_kv / 2;
     const int rb = 16 * a.nr;
-    const long long s_want = (a.batch == 1 ? 1LL : 4LL) * cus;
-    const long long t_want = (a.batch == 1 ? 1LL : 2LL) * cus;
     const long long s_items = (std::min<long long>(rows1, u15h::kPagedShortRows) + rb - 1) / rb *
                               a.hkv * a.batch;
     const long long t_items = (rows / 128 + a.batch) * a.hkv;
+    const double work = a.longs ? (double)t_items * mean / 64 * tile / cus
+                                : (double)a.batch * mean * a.hkv * a.d * 4 / 5e6;
     const long long most = std::max(1LL, std::min(keys / 256, pieces));
-    cut(keys, std::max(1LL, std::min(s_want / s_items, most)), &a.s_shares, &a.s_chunk);
-    cut(keys, std::max(1LL, std::min(t_want / t_items, most)), &a.t_shares, &a.t_chunk);
+    auto shares_of = [&](double walk, long long most, int* shares, int* chunk) {
+      double best = 1e30;
+      int pick = 1;
+      for (int n = 1; n <= most; ++n) {
+        const double us = std::max(work, walk / n) + 0.3 * walk / n + n * part +
+                          (n > 1 && a.p_shares == 0 ? 4.0 : 0.0);
+        if (us < best) {
+          best = us;
+          pick = n;
+        }
+      }
+      cut(keys, pick, shares, chunk);
+    };
+    // at most one streaming workgroup a CU for a sequence by itself (which
+    // fills the memory's rate), four for several
+    const long long s_most = (a.batch == 1 ? 1LL : 4LL) * cus / s_items;
+    shares_of(keys / 128.0 * 2.0, std::min(most, s_most), &a.s_shares, &a.s_chunk);
+    shares_of(keys / 64.0 * tile, std::min(most, 4LL * cus / t_items), &a.t_shares, &a.t_chunk);
     while (u15h::paged_ws_bytes(a) > bytes && a.s_shares + a.t_shares > 2) {
       cut(keys, std::max(a.s_shares - 1, 1), &a.s_shares, &a.s_chunk);
       cut(keys, std::max(a.t_shares - 1, 1), &a.t_shares, &a.t_chunk);
