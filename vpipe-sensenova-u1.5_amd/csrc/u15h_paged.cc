@@ -175,7 +175,7 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
   const long long pieces = ws == nullptr ? 1 : 64;      // most shares of anything
 
   // us: a 64-key tile of one workgroup, the streaming of own keys, a part's
-  // round trip
+  // round trip (and 0.15 for its place in the sum; 32 parts are one pass)
   const double tile = a.d == 128 ? 0.94 : a.d == 64 ? 0.63 : 0.52;
   const double own = (double)a.batch * a.max_kv * 0.5 * a.hkv * a.d * 4 / 5e6;
   const double part = (double)a.tokens * a.hq * (a.d + 2) * 8 / 4e6;
@@ -192,14 +192,21 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
       const int rb = a.p_tile ? 128 : 16 * a.nr;
       const long long blocks = (rows + rb - 1) / rb * a.hkv;
       double best = 1e30;
-      for (int n = 1; n <= pieces; ++n) {
+      for (int n = 1; n <= std::min(pieces, 30LL); ++n) {
         int shares, chunk;
         cut(a.prefix, n, &shares, &chunk);
-        const double items = (double)blocks * shares, walk = chunk / 64.0 * tile;
-        // beside streaming workgroups a tile takes half as long again; two
-        // tile workgroups on a CU take twice as long
-        const double busy = std::max(1.5 * walk, items / cus * walk);
-        const double us = std::max(own, busy + 5.0) + part * shares;
+        const double items = (double)blocks * shares;
+        double busy;
+        if (a.p_tile) {
+          // beside streaming workgroups a tile takes half as long again; two
+          // tile workgroups on a CU take twice as long
+          const double walk = chunk / 64.0 * tile;
+          busy = std::max(1.5 * walk, std::ceil(items / cus) * walk);
+        } else {
+          const double walk = chunk / 128.0 * 1.2;
+          busy = std::max(walk, items / (2 * cus) * walk);
+        }
+        const double us = std::max(own, busy + 5.0) + (part + 0.15) * shares;
         if (us < best) {
           best = us;
           a.p_shares = shares;
