@@ -201,6 +201,9 @@ set_tiles(GemmBatch& b, Epi epi, int bm, int bn)
 
 // Scratch of split attention calls, per context.
 constexpr size_t kAttnWsBytes = (size_t)32 << 20;
+// Counters behind it (paged attention's shares that have arrived), 0 between
+// calls.
+constexpr size_t kAttnCountBytes = (size_t)u15h::kPagedJoins * sizeof(int);
 
 // Fewest K stages a split share may have.
 constexpr int kMinStagesPerShare = 4;
@@ -873,7 +876,12 @@ u15h_create(int device, u15h_ctx** out)
   ctx->mid_bm = mid == 128 || mid == 192 || mid == 256 ? mid : 0;
   ctx->i8_min_m = std::max(1, env_int("U15H_I8_MIN_M", 1024));
   ctx->attn_split = env_int("U15H_ATTN_SPLIT", -1);
-  if (ctx->attn_split != 0 && hipMalloc(&ctx->attn_ws, kAttnWsBytes) != hipSuccess) {
+  if (ctx->attn_split != 0 &&
+      (hipMalloc(&ctx->attn_ws, kAttnWsBytes + kAttnCountBytes) != hipSuccess ||
+       hipMemset(static_cast<char*>(ctx->attn_ws) + kAttnWsBytes, 0, kAttnCountBytes) !=
+           hipSuccess ||
+       hipStreamSynchronize(nullptr) != hipSuccess)) {
+    if (ctx->attn_ws != nullptr) { (void)hipFree(ctx->attn_ws); }
     ctx->attn_ws = nullptr;
     (void)hipGetLastError();
   }

@@ -387,7 +387,12 @@ struct PagedArgs {
   // unnormalised outputs [part][tokens * hq][d] f32, then the rows' running
   // maxima (base 2) and sums.
   float* ws;
+  // Streaming workgroups only, every sequence by itself: the last of a block's
+  // shares adds them, counted in joins[block], which it leaves at 0; null: a
+  // second kernel does.
+  int* joins;
 };
+constexpr int kPagedJoins = 16384;            // counters behind the scratch
 constexpr int kPagedShortRows = 64;
 __host__ __device__ inline int
 paged_own_parts(const PagedArgs& a)
@@ -419,8 +424,9 @@ int gemm_cus(const u15h_ctx* ctx);
 // capture) and its size (0 where splitting is switched off).
 u15h_status split_workspace(u15h_ctx* ctx, void** ws);
 size_t split_workspace_bytes(const u15h_ctx* ctx);
-// The scratch of attention split over the keys, null where there is none, and
-// the device's compute units.
+// The scratch of attention split over the keys, null where there is none, with
+// kPagedJoins counters (0 between calls) behind its `bytes`; the device's
+// compute units.
 void* attention_scratch(const u15h_ctx* ctx, size_t* bytes);
 int compute_units(const u15h_ctx* ctx);
 

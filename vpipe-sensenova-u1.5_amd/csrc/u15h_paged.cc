@@ -214,9 +214,10 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
         }
       }
     }
-    // What a sequence walks itself, in shares of 256 keys or more: the walk of
-    // the longest against all workgroups' work, which hides it; a tail of uneven
-    // lengths; and what shares cost.
+    // What a sequence walks itself, in shares of 256 keys or more (128 in a
+    // small call): the walk of the longest against all workgroups' work, which
+    // hides it; a tail of uneven lengths; and what shares cost.  128 keys take a
+    // streaming workgroup 1 us, 2 or more once the memory is at its rate.
     const long long before = a.p_shares > 0 ? 0 : round_up(a.prefix, 64);
     const long long keys = before + a.max_kv, mean = before + a.max_kv / 2;
     const int rb = 16 * a.nr;
@@ -225,13 +226,13 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
     const long long t_items = (rows / 128 + a.batch) * a.hkv;
     const double work = a.longs ? (double)t_items * mean / 64 * tile / cus
                                 : (double)a.batch * mean * a.hkv * a.d * 4 / 5e6;
-    const long long most = std::max(1LL, std::min(keys / 256, pieces));
+    const long long most = std::max(1LL, std::min(keys / (work < 10.0 ? 128 : 256), pieces));
     auto shares_of = [&](double walk, long long most, int* shares, int* chunk) {
       double best = 1e30;
       int pick = 1;
       for (int n = 1; n <= most; ++n) {
         const double us = std::max(work, walk / n) + 0.3 * walk / n + n * part +
-                          (n > 1 && a.p_shares == 0 ? 4.0 : 0.0);
+                          (n > 1 && a.p_shares == 0 ? 3.0 : 0.0);
         if (us < best) {
           best = us;
           pick = n;
@@ -242,7 +243,7 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
     // at most one streaming workgroup a CU for a sequence by itself (which
     // fills the memory's rate), four for several
     const long long s_most = (a.batch == 1 ? 1LL : 4LL) * cus / s_items;
-    shares_of(keys / 128.0 * 2.0, std::min(most, s_most), &a.s_shares, &a.s_chunk);
+    shares_of(keys / 128.0 * (work < 10.0 ? 1.0 : 2.0), std::min(most, s_most), &a.s_shares, &a.s_chunk);
     shares_of(keys / 64.0 * tile, std::min(most, 4LL * cus / t_items), &a.t_shares, &a.t_chunk);
     while (u15h::paged_ws_bytes(a) > bytes && a.s_shares + a.t_shares > 2) {
       cut(keys, std::max(a.s_shares - 1, 1), &a.s_shares, &a.s_chunk);
@@ -253,6 +254,14 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
     }
     if (!phase || u15h::paged_ws_bytes(a) <= bytes) { break; }
   }
+  const int rb = 16 * a.nr;
+  const long long joins =
+      (std::min<long long>(rows1, u15h::kPagedShortRows) + rb - 1) / rb * a.hkv * a.batch;
+  const double walked = (double)a.batch * (a.prefix + a.max_kv / 2) * a.hkv * a.d * 4 / 5e6;
+  a.joins = a.p_shares == 0 && !a.longs && a.s_shares > 1 && joins <= u15h::kPagedJoins &&
+                    walked < 30.0
+                ? reinterpret_cast<int*>(static_cast<char*>(ws) + bytes)
+                : nullptr;
 }
 
 }  // namespace

@@ -365,7 +365,7 @@ struct Sequence {
   int first, n, keys;
 };
 __device__ __forceinline__ Sequence
-sequence(const PagedArgs& A, int b)
+sequence_at(const PagedArgs& A, int b)
 {
   int s0 = b, s1 = b + 1;
   if (A.q_start != nullptr) {
@@ -376,7 +376,13 @@ sequence(const PagedArgs& A, int b)
   s1 = min(max(s1, s0), A.tokens);
   const long long room = (long long)A.table_stride << A.page_log2;
   const int most = (int)min((long long)A.max_kv, room);
-  return {uniform(s0), uniform(min(s1 - s0, A.max_q)), uniform(min(max(A.kv_len[b], 0), most))};
+  return {s0, min(s1 - s0, A.max_q), min(max(A.kv_len[b], 0), most)};
+}
+__device__ __forceinline__ Sequence
+sequence(const PagedArgs& A, int b)                    // b the same in all lanes
+{
+  const Sequence S = sequence_at(A, b);
+  return {uniform(S.first), uniform(S.n), uniform(S.keys)};
 }
 
 // The partial results of part p: row r's output, and its maximum and sum (the
@@ -411,6 +417,23 @@ mark_parts(const PagedArgs& A, int from, int to, int first, int G, int kvh, int 
       P.ml[part_row(A, first + row / G, kvh * G + row % G)] = make_float2(-INFINITY, what);
     }
   }
+}
+
+// Values that one workgroup leaves for another of the same launch: written
+// through to the memory and read from there, past the dies' own L2.
+__device__ __forceinline__ void
+give(float* p, float x, float y)
+{
+  const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2
+take(const float* p)
+{
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
 // What a workgroup walks: prefix keys, then own keys, each from a tile's start,
@@ -728,6 +751,15 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
     if (!direct) {
       const Part P = part_of(A, part);
       const long long at = part_row(A, S.first + row / G, kvh * G + row % G);
+      if (A.joins != nullptr) {
+        if (c == 0) {
+          give(reinterpret_cast<float*>(P.ml + at), top, top == -INFINITY ? kNoKey : sum);
+        }
+        if (top == -INFINITY) { continue; }
+        give(P.o + at * D + c, acc[0], acc[1]);
+        give(P.o + at * D + c + 2, acc[2], acc[3]);
+        continue;
+      }
       if (c == 0) { P.ml[at] = make_float2(top, top == -INFINITY ? kNoKey : sum); }
       if (top == -INFINITY) { continue; }
       *reinterpret_cast<f32x4_t*>(P.o + at * D + c) = acc;
@@ -737,6 +769,89 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
     uint16_t* op = A.out + (S.first + row / G) * A.o_tok + (kvh * G + row % G) * D + c;
     *reinterpret_cast<u32x2_t*>(op) = u32x2_t{pack_bf16x2(acc[0] * inv, acc[1] * inv),
                                               pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+  }
+  if (A.joins == nullptr || direct) { return; }
+
+  // The last share of this block to arrive adds them all.  Every wave waits for
+  // its own writes to have reached the memory before the block counts as
+  // arrived.
+  __shared__ int arrived;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    const int blocks = (min(A.max_q * G, kPagedShortRows) + RB - 1) / RB;
+    int* count = A.joins + (seq * blocks + row0 / RB) * A.hkv + kvh;
+    arrived = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+    if (arrived == A.s_shares) {
+      __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  __syncthreads();
+  if (arrived != A.s_shares) { return; }
+  // A row over D / 4 threads, `groups` of those on the parts of one row (p =
+  // group, group + groups, ..), whose sums meet in LDS; always in that order.
+  constexpr int LPR = D / 4, kSlots = 256 / LPR, kAhead = 8;
+  const int live = min(rows - row0, RB);
+  int span = 1;
+  while (span < live && span < kSlots) { span *= 2; }
+  const int groups = kSlots / span;
+  const int slot = tid / LPR, c = tid % LPR * 4;
+  const int grp = slot / span;
+  for (int r = slot % span; r - slot % span < live; r += span) {
+    const int row = row0 + min(r, live - 1);
+    const long long at = part_row(A, S.first + row / G, kvh * G + row % G);
+    float m = -INFINITY, l = 0.0f;
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float m1, float l1, f32x4_t o1) {
+      if (l1 < 0.0f) { return; }
+      const float top = fmaxf(m, m1);
+      const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+      l = __builtin_fmaf(l, f0, l1 * f1);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { acc[e] = __builtin_fmaf(o1[e], f1, acc[e] * f0); }
+      m = top;
+    };
+    for (int p0 = grp; p0 < A.s_shares; p0 += groups * kAhead) {
+      float2 ml[kAhead], lo[kAhead], hi[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int p = p0 + i * groups;
+        ml[i] = make_float2(-INFINITY, kNoKey);
+        lo[i] = hi[i] = make_float2(0.0f, 0.0f);
+        if (p < A.s_shares) {
+          const Part P = part_of(A, p);
+          ml[i] = take(reinterpret_cast<const float*>(P.ml + at));
+          lo[i] = take(P.o + at * D + c);
+          hi[i] = take(P.o + at * D + c + 2);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        add(ml[i].x, ml[i].y, f32x4_t{lo[i].x, lo[i].y, hi[i].x, hi[i].y});
+      }
+    }
+    if (groups > 1) {
+      // RB rows of D a buffer, kSlots <= 2 RB of them in the first two
+      *reinterpret_cast<f32x4_t*>(so(slot / RB) + slot % RB * D + c) = acc;
+      if (c == 0) {
+        o3[2 * slot] = m;
+        o3[2 * slot + 1] = m == -INFINITY ? kNoKey : l;
+      }
+      __syncthreads();
+      if (grp == 0) {
+        for (int q = 1; q < groups; ++q) {
+          const int other = slot + q * span;
+          add(o3[2 * other], o3[2 * other + 1],
+              *reinterpret_cast<const f32x4_t*>(so(other / RB) + other % RB * D + c));
+        }
+      }
+    }
+    if (grp == 0 && r < live) {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      uint16_t* op = A.out + (S.first + row / G) * A.o_tok + (kvh * G + row % G) * D + c;
+      *reinterpret_cast<u32x2_t*>(op) = u32x2_t{pack_bf16x2(acc[0] * inv, acc[1] * inv),
+                                                pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+    }
   }
 }
 
@@ -792,30 +907,25 @@ constexpr int kTileRows = 128;
 // are taken as they come, b's blocks from rows before it / 128 + b on, which
 // leaves each one block or two that have no rows.
 __device__ __forceinline__ int
-sequence_of_block(const PagedArgs& A, int G, int nb, int* local)
+sequence_of_block(const PagedArgs& A, int G, int nb, int* local, Sequence* S)
 {
   const int lane = threadIdx.x & 63;
   if (A.batch <= 64) {
-    int n = 0, keys = -1;
-    if (lane < A.batch) {
-      int s0 = lane, s1 = lane + 1;
-      if (A.q_start != nullptr) {
-        s0 = min(max(A.q_start[lane], 0), A.tokens);
-        s1 = min(max(A.q_start[lane + 1], s0), A.tokens);
-      }
-      const int rows = min(s1 - s0, A.max_q) * G;
-      n = rows > kPagedShortRows ? (rows + kTileRows - 1) / kTileRows : 0;
-      keys = A.kv_len[lane];
-    }
+    Sequence mine = {0, 0, -1};
+    if (lane < A.batch) { mine = sequence_at(A, lane); }
+    const int rows = mine.n * G, keys = mine.keys;
+    const int n = rows > kPagedShortRows ? (rows + kTileRows - 1) / kTileRows : 0;
     int start = 0;
     for (int j = 0; j < A.batch; ++j) {
       const int kj = __builtin_amdgcn_readlane(keys, j);
       const bool before = kj > keys || (kj == keys && j < lane);
       start += before ? __builtin_amdgcn_readlane(n, j) : 0;
     }
-    const unsigned long long mine = __ballot(nb >= start && nb < start + n);
-    if (mine == 0) { return -1; }
-    const int seq = __builtin_ctzll(mine);
+    const unsigned long long here = __ballot(nb >= start && nb < start + n);
+    if (here == 0) { return -1; }
+    const int seq = __builtin_ctzll(here);
+    *S = {__builtin_amdgcn_readlane(mine.first, seq), __builtin_amdgcn_readlane(mine.n, seq),
+          __builtin_amdgcn_readlane(keys, seq)};
     *local = __builtin_amdgcn_readlane(n, seq) - 1 - (nb - __builtin_amdgcn_readlane(start, seq));
     return seq;
   }
@@ -835,6 +945,7 @@ sequence_of_block(const PagedArgs& A, int G, int nb, int* local)
     if (last < 63) { break; }
   }
   *local = nb - start;
+  if (count > 0) { *S = sequence(A, count - 1); }
   return count - 1;
 }
 
@@ -874,13 +985,12 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
     share = item % A.t_shares;
     item /= A.t_shares;
     int local;
-    const int seq = sequence_of_block(A, G, item % blocks, &local);
+    const int seq = sequence_of_block(A, G, item % blocks, &local, &S);
     kvh = item / blocks;
     part = A.p_shares + share;
     shares = A.t_shares;
     chunk = A.t_chunk;
     if (seq < 0) { return; }
-    S = sequence(A, uniform(seq));
     row0 = uniform(local) * kTileRows;
     if (S.n * G <= kPagedShortRows) { return; }
     table = A.table + (long long)uniform(seq) * A.table_stride;
@@ -1355,7 +1465,7 @@ launch_paged_d(const PagedArgs& a, hipStream_t s)
 #undef U15H_RUN
   const hipError_t e = hipGetLastError();
   const int parts = paged_parts(a);
-  if (e != hipSuccess || parts == 1) { return e; }
+  if (e != hipSuccess || parts == 1 || a.joins != nullptr) { return e; }
   const unsigned outs = (unsigned)a.tokens * a.hq;
   if (parts > 8 && outs < 4096) {
     hipLaunchKernelGGL((paged_combine_kernel<D, 4>), dim3(outs), dim3(256), 0, s, a);
