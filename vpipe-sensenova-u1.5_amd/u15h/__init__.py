@@ -59,6 +59,7 @@ class _MotProjI8(ctypes.Structure):
 # pointer's alignment
 _PROJ_FP8 = [struct.Struct("@" + "PPPPPi0P" * n) for n in range(1, MAX_PROJ + 1)]
 _BF16, _F8, _F32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32
+_I32 = torch.int32
 
 
 class _LayerIO(ctypes.Structure):
@@ -565,7 +566,8 @@ class PagedKV:
                 raise ValueError(f"{name}'s pages must be contiguous")
         if k.shape != v.shape or k.stride(0) != v.stride(0) or k.get_device() != v.get_device():
             raise ValueError("k and v must have one shape, distance between pages and device")
-        pages, heads, page, d = self.shape = tuple(k.shape)
+        pages, heads, page, d = k.shape
+        self.heads, self.page, self.head_dim = heads, page, d
         self.k, self.v, self.device = k, v, k.get_device()
         whole = heads * page * d
         stride = k.stride(0) if pages > 1 else whole
@@ -1356,48 +1358,59 @@ class Ops:
 
     # ---- attention -------------------------------------------------------
     # ---- many requests at once ----------------------------------------------
+    # (one pass over a tensor's properties each: these calls' checks are as long
+    # as their launches)
     def _rows(self, t, name):
-        """(address, distance of tokens, heads, head_dim) of [tokens][heads]
-        [head_dim] bf16 on this context's device whose heads are contiguous."""
-        if t.dtype is not _BF16 or t.dim() != 3 or t.get_device() != self.device:
-            raise ValueError(f"{name} must be [tokens][heads][head_dim] bf16 on "
-                             f"cuda:{self.device}")
-        _, h, d = t.shape
-        st, sh, sd = t.stride()
-        if (sd != 1 and d > 1) or (sh != d and h > 1):
-            raise ValueError(f"{name}'s heads must be contiguous")
-        return t.data_ptr(), st if t.shape[0] > 1 else h * d, h, d
+        """(address, distance of tokens, tokens, heads, head_dim) of [tokens]
+        [heads][head_dim] bf16 on this context's device whose heads are
+        contiguous."""
+        if t.dtype is _BF16 and t.get_device() == self.device:
+            s = t.stride()
+            if len(s) == 3:
+                n, h, d = t.shape
+                if (s[2] == 1 or d == 1) and (s[1] == d or h == 1):
+                    return t.data_ptr(), s[0] if n > 1 else h * d, n, h, d
+                raise ValueError(f"{name}'s heads must be contiguous")
+        raise ValueError(f"{name} must be [tokens][heads][head_dim] bf16 on cuda:{self.device}")
+
+    def _index(self, t, n, name):
+        """The address of n int32 on this context's device."""
+        if t.dtype is _I32 and t.get_device() == self.device and t.is_contiguous() \
+                and t.shape == (n,):
+            return t.data_ptr()
+        raise ValueError(f"{name} must be [{n}] int32, contiguous, on cuda:{self.device}")
 
     def _turn(self, rope, pos, tokens):
         """The addresses of a rotation and of its positions."""
         if rope.device != self.device:
             raise ValueError(f"the rotation is on cuda:{rope.device}, this context on "
                              f"cuda:{self.device}")
-        if pos.dim() == 1 and rope.axes == 1:
-            good = pos.shape[0] == tokens
-        else:
-            good = pos.dim() == 2 and pos.shape[0] >= rope.axes and pos.shape[1] == tokens
-        if not good:
-            raise ValueError(f"pos must be [{rope.axes}][{tokens}]")
-        return rope._at, _table(pos, self.device, "pos")
+        if pos.dtype is _I32 and pos.get_device() == self.device and pos.is_contiguous():
+            s = pos.shape
+            if (len(s) == 2 and s[1] == tokens and s[0] >= rope.axes) or \
+                    (rope.axes == 1 and s == (tokens,)):
+                return rope._at, pos.data_ptr()
+        raise ValueError(f"pos must be [{rope.axes}][{tokens}] int32, contiguous, on "
+                         f"cuda:{self.device}")
 
     def rope(self, x, pos, rope, y, inverse=False, stream=None):
         """y = x [tokens][heads][head_dim] turned by its tokens' positions
         [axes][tokens] (int32), or turned back; any strides between tokens and
         heads; y may be x."""
-        for t, name in ((x, "x"), (y, "y")):
-            if t.dtype is not _BF16 or t.dim() != 3 or t.get_device() != self.device:
-                raise ValueError(f"{name} must be [tokens][heads][head_dim] bf16 on "
-                                 f"cuda:{self.device}")
-            if t.stride(2) != 1 and t.shape[2] > 1:
-                raise ValueError(f"{name}'s columns must be contiguous")
-        if x.shape != y.shape:
-            raise ValueError(f"y: shape {tuple(y.shape)}, expected {tuple(x.shape)}")
-        tokens, heads, d = x.shape
+        dev = self.device
+        if x.dtype is not _BF16 or y.dtype is not _BF16 or x.get_device() != dev or \
+                y.get_device() != dev:
+            raise ValueError(f"x and y must be bf16 on cuda:{dev}")
+        shape, xs, ys = x.shape, x.stride(), y.stride()
+        if len(xs) != 3 or y.shape != shape:
+            raise ValueError("x and y must both be [tokens][heads][head_dim]")
+        tokens, heads, d = shape
+        if (xs[2] != 1 or ys[2] != 1) and d > 1:
+            raise ValueError("the columns of x and y must be contiguous")
         rp, pp = self._turn(rope, pos, tokens)
         st = self._lib.u15h_rope(self._ctx, self._stream_here(stream), rp, pp, x.data_ptr(),
-                                 x.stride(0), x.stride(1), y.data_ptr(), y.stride(0),
-                                 y.stride(1), tokens, heads, d, inverse)
+                                 xs[0], xs[1], y.data_ptr(), ys[0], ys[1], tokens, heads, d,
+                                 inverse)
         if st:
             self._check(st, "u15h_rope")
 
@@ -1410,13 +1423,10 @@ class Ops:
         if kv.device != self.device:
             raise ValueError(f"the cache is on cuda:{kv.device}, this context on "
                              f"cuda:{self.device}")
-        kp, ks, h, d = self._rows(k, "k")
-        vp, vs, _, _ = self._rows(v, "v")
-        tokens = k.shape[0]
-        if k.shape != v.shape or h != kv.shape[1] or d != kv.shape[3]:
-            raise ValueError(f"k and v must be [tokens][{kv.shape[1]}][{kv.shape[3]}]")
-        if slot.dim() != 1 or slot.shape[0] != tokens:
-            raise ValueError(f"slot must be [{tokens}]")
+        kp, ks, tokens, h, d = self._rows(k, "k")
+        vp, vs, n, vh, vd = self._rows(v, "v")
+        if h != kv.heads or d != kv.head_dim or vh != h or vd != d or n != tokens:
+            raise ValueError(f"k and v must be [tokens][{kv.heads}][{kv.head_dim}]")
         rp = pp = qp = op = None
         qs = os_ = hq = 0
         if rope is not None:
@@ -1424,15 +1434,16 @@ class Ops:
                 raise ValueError("a rotation needs positions")
             rp, pp = self._turn(rope, pos, tokens)
         if q is not None:
-            if q_out is None or q.shape != q_out.shape or q.shape[0] != tokens or \
-                    q.shape[2] != d:
-                raise ValueError(f"q and q_out must be [{tokens}][heads][{d}], both given")
-            qp, qs, hq, _ = self._rows(q, "q")
-            op, os_, _, _ = self._rows(q_out, "q_out")
+            if q_out is None:
+                raise ValueError("q without q_out")
+            qp, qs, n, hq, qd = self._rows(q, "q")
+            op, os_, on, oh, od = self._rows(q_out, "q_out")
+            if n != tokens or on != tokens or oh != hq or qd != d or od != d:
+                raise ValueError(f"q and q_out must be [{tokens}][heads][{d}]")
         elif q_out is not None:
             raise ValueError("q_out without q")
         st = self._lib.u15h_paged_append(
-            self._ctx, self._stream_here(stream), kv._at, _table(slot, self.device, "slot"), rp,
+            self._ctx, self._stream_here(stream), kv._at, self._index(slot, tokens, "slot"), rp,
             pp, kp, ks, vp, vs, qp, qs, op, os_, hq, tokens)
         if st:
             self._check(st, "u15h_paged_append")
@@ -1444,16 +1455,16 @@ class Ops:
         if kv.device != self.device or batch.device != self.device:
             raise ValueError(f"cache on cuda:{kv.device}, batch on cuda:{batch.device}, this "
                              f"context on cuda:{self.device}")
-        qp, qs, h, d = self._rows(q, "q")
-        op, os_, _, _ = self._rows(out, "out")
-        if q.shape != out.shape or d != kv.shape[3]:
-            raise ValueError(f"q and out must be [tokens][heads][{kv.shape[3]}]")
+        qp, qs, n, h, d = self._rows(q, "q")
+        op, os_, on, oh, od = self._rows(out, "out")
+        if d != kv.head_dim or on != n or oh != h or od != d:
+            raise ValueError(f"q and out must be [tokens][heads][{kv.head_dim}]")
         b = batch._b
-        room = batch.width * kv.shape[2]
+        room = batch.width * kv.page
         most = room if batch.max_kv is None else batch.max_kv
-        if most > room or batch.prefix_len > batch.prefix_pages * kv.shape[2]:
+        if most > room or batch.prefix_len > batch.prefix_pages * kv.page:
             raise ValueError("the tables have fewer pages than max_kv or prefix_len keys")
-        b.tokens, b.max_kv = q.shape[0], most
+        b.tokens, b.max_kv = n, most
         st = self._lib.u15h_paged_attention(
             self._ctx, self._stream_here(stream), kv._at, batch._at, qp, qs, op, os_, h, scale,
             causal)
