@@ -31,8 +31,9 @@
  * without synchronising.  A context is not thread-safe: use one per host
  * thread, or serialise.  A context owns scratch memory that its GEMM and
  * attention calls write and read on the device (the split-K partial sums,
- * the partial outputs of attention split over the keys, the int8 route's
- * codes and scales, the dequant expansion), so ALL calls on one context
+ * the partial outputs of attention split over the keys and their counters,
+ * the int8 route's codes and scales, the dequant expansion), so ALL calls on
+ * one context
  * must be ordered on ONE stream (or otherwise ordered by the caller, e.g.
  * with events): two calls on one context queued on unordered streams race
  * on that scratch.  Use one context per stream for concurrent work.
@@ -442,7 +443,7 @@ u15h_status u15h_rope(u15h_ctx* ctx, u15h_stream stream,
  * allocation, and a page of a whole context is a contiguous cache.
  * Limits: page a power of two in [16, 2^20], head_dim 32, 64 or 128,
  * page_stride >= kv_heads * page * head_dim and a multiple of 8,
- * pages * page < 2^31; pointers 16-byte aligned. */
+ * pages * page < 2^31, pages * page_stride <= 2^40; pointers 16-byte aligned. */
 typedef struct {
   u15h_bf16* k;
   u15h_bf16* v;
@@ -501,15 +502,19 @@ typedef struct {
  * every sequence; u15h_attention_token_major for many requests.  q, out
  * [tokens][hq * head_dim] bf16, rows *_stride elements apart (multiples of 8);
  * query head h reads kv head h / (hq / kv_heads); scale 0 stands for
- * 1 / sqrt(head_dim); causal 0: every query sees all keys.  A query that sees
- * no key gets zeros; rows of no sequence are left as they are.  out may not
- * overlap q.
+ * 1 / sqrt(head_dim), any other is from 1e-12 to 1e12; causal 0: every query
+ * sees all keys.  A query that sees no key gets zeros; rows of no sequence are
+ * left as they are.  out may not overlap q.
+ * Slots from kv_len on (and past prefix_len) are not read, whatever they hold.
+ * Among the keys below kv_len that the causal mask hides from a query, the
+ * values have to be finite: weights of 0 times an infinity or NaN are NaN.
  * The prefix is walked once for the whole batch where that is less work: its
  * keys meet all sequences' queries as one matrix, and the sequences' own keys
  * join through partial results in the context's attention scratch (u15h_sdpa;
  * without it every sequence walks the prefix itself).
  * Limits: hq % kv_heads == 0, hq <= 4096, batch <= 65536, tokens <= 2^22,
- * max_kv and prefix_len < 2^29. */
+ * max_kv and prefix_len < 2^29, tokens * hq < 2^31, 5 * batch * kv_heads +
+ * tokens * hq / 128 <= 2^23. */
 u15h_status u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream,
                                  const u15h_paged_kv* kv,
                                  const u15h_paged_batch* batch,

@@ -69,14 +69,21 @@ launch_rope(const RopeArgs& a, hipStream_t)
 hipError_t
 launch_paged_attention(const PagedArgs& a, hipStream_t)
 {
-  if (paged_ws_bytes(a) > g_bytes || (paged_parts(a) > 1 && a.ws == nullptr)) {
+  // the scratch holds the parts, chunks cover what they cut, and a call that
+  // joins in its own workgroups has no parts of another kind
+  const long long keys = (a.p_shares > 0 ? 0 : a.prefix) + (long long)a.max_kv;
+  if (paged_ws_bytes(a) > g_bytes || (paged_parts(a) > 1 && a.ws == nullptr) ||
+      (a.p_shares > 0 && (long long)a.p_shares * a.p_chunk < a.prefix) ||
+      (long long)a.s_shares * a.s_chunk < keys || (long long)a.t_shares * a.t_chunk < keys ||
+      a.s_chunk % 128 != 0 || a.t_chunk % 128 != 0 || a.p_chunk % 128 != 0 ||
+      (a.joins != nullptr && (a.p_shares > 0 || a.longs || a.s_shares < 2))) {
     return hipErrorInvalidValue;
   }
   std::ostringstream s;
   s << "attn parts=" << paged_parts(a) << " p=" << a.p_shares << "x" << a.p_chunk << " "
     << (a.p_shares == 0 ? "none" : a.p_tile ? "tile" : "stream") << " s=" << a.shorts << ":"
     << a.s_shares << "x" << a.s_chunk << " t=" << a.longs << ":" << a.t_shares << "x" << a.t_chunk
-    << " nr=" << a.nr << " max_q=" << a.max_q << " scale=" << a.scale << " stride="
+    << " nr=" << a.nr << " joins=" << (a.joins != nullptr) << " max_q=" << a.max_q << " scale=" << a.scale << " stride="
     << a.table_stride;
   g_out += s.str();
   return hipSuccess;

@@ -98,3 +98,38 @@ def attend(q, kp, vp, prefix_table, prefix_len, tables, lens, counts, causal, sc
         out.append(o.transpose(0, 1))
         bound.append(tol.transpose(0, 1))
     return torch.cat(out), torch.cat(bound)
+
+
+# Batches for every way in which a call is cut: (own keys, queries, prefix, heads,
+# more of Case, the plan that tests/paged_host.cc prints for 256 compute units).
+PLANS = {
+    "whole": ([77, 5], [1, 1], 50, (32, 8, 128), {}, r"parts=1 .*none s=1:1x.* t=0:.* nr=1"),
+    "joined": ([1800], [1], 0, (8, 2, 128), {}, r"none s=1:(?!1x).* t=0.* nr=1 .*joins=1"),
+    "joined_rows": ([1800, 40], [9, 3], 0, (10, 2, 64), {}, r"none s=1:(?!1x).* t=0.* nr=2 .*joins=1"),
+    "joined_narrow": ([700], [2], 100, (6, 1, 32), {}, r"none s=1:(?!1x).* nr=1 .*joins=1"),
+    "second_kernel": ([3000, 2500], [1, 1], 0, (8, 8, 128), dict(max_kv=50000, wide=3125),
+                      r"none s=1:(?!1x).* t=0.*joins=0"),
+    "prefix_streamed": ([30, 1, 500], [1, 1, 1], 2000, (6, 2, 128), {}, r"stream s=1:.* nr=1"),
+    "prefix_streamed_wide": ([30, 1, 500, 7] * 2, [1] * 8, 600, (8, 2, 64), {},
+                             r"stream s=1:.* nr=2"),
+    "prefix_tiled": ([30, 1, 200, 7] * 6, [1] * 24, 700, (8, 2, 128), {}, r"tile s=1:.* t=0:"),
+    "prefix_many_parts": ([30, 1, 90, 7] * 5, [1] * 20, 6000, (4, 1, 64), {}, r"parts=[1-9]\d .*tile"),
+    "prefix_drafts": ([30, 8, 200, 7] * 2, [5, 8, 3, 7] * 2, 900, (8, 2, 64), {},
+                      r"tile s=1:.* t=0:.* nr=2"),
+    "prefix_beside_long": ([150, 33, 60, 200, 20], [100, 3, 60, 1, 20], 900, (8, 2, 128), {},
+                           r"tile s=1:.* t=1:"),
+    "long_whole": ([300, 301], [300, 17], 40, (8, 2, 128), {}, r"parts=1 .*none .* t=1:1x"),
+    "long_split": ([3000], [100], 70, (8, 2, 128), {}, r"none .* t=1:(?!1x)"),
+    "long_beside_split": ([700, 3000, 90, 400], [680, 1, 1, 2], 0, (32, 1, 64),
+                          dict(max_kv=4096, wide=256), r"none s=1:(?!1x)"),
+    "seventy": ([40, 3] * 35, [20, 1] * 35, 30, (8, 2, 32), {}, r"none .* t=1:"),
+    "head_group_of_80": ([90, 300], [1, 3], 33, (80, 1, 64), {}, r"s=0:.* t=1:"),
+}
+
+
+def plan_call(name):
+    """The line that asks tests/paged_host.cc for a case's plan."""
+    lens, counts, prefix, (hq, hkv, d), more, _ = PLANS[name]
+    most = more.get("max_kv", max(-(-n // 16) for n in lens) * 16)
+    return (f"attn batch={len(lens)} tokens={sum(counts) + 2} max_q={max(counts)} max_kv={most} "
+            f"prefix_len={prefix} hq={hq} heads={hkv} d={d} table_stride=9999")

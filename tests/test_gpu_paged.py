@@ -246,6 +246,12 @@ class Case:
                                max_kv=max_kv, prefix_table=self.prefix_table.cuda(),
                                prefix_len=self.prefix)
 
+    def widen(self, pages):
+        """The table with room for as many pages."""
+        more = torch.full((len(self.lens), pages), -1, dtype=I32)
+        more[:, :self.table.shape[1]] = self.table
+        self.table = more
+
     def run(self, ops, causal, scale=0.0, batch=None, pad_q=0, pad_out=0, stream=None):
         """out [rows + pad][hq][d], guarded by rows of a wider matrix."""
         n, hq, d = self.q.shape
@@ -293,6 +299,172 @@ def test_attention(ops, hq, hkv, d, name, prefix, page, causal):
     lens, counts = BATCHES[name]
     c = Case(lens, counts, prefix, hq, hkv, d, page, seed=prefix + hq)
     check(c.run(ops, causal), c.want(causal))
+
+
+def planned(name, **more):
+    lens, counts, prefix, (hq, hkv, d), kw, _ = ref.PLANS[name]
+    c = Case(lens, counts, prefix, hq, hkv, d, 16, seed=len(name), **more)
+    if "wide" in kw:
+        c.widen(kw["wide"])
+    return c, dict(max_kv=kw.get("max_kv"))
+
+
+@pytest.mark.parametrize("name", list(ref.PLANS))
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_every_plan(ops, name, causal):
+    """Every way in which a call is cut over workgroups, joined and added; twice,
+    so that what one call leaves in the scratch does not reach the next."""
+    c, kw = planned(name)
+    want = c.want(causal)
+    first = c.run(ops, causal, batch=c.batch(**kw))
+    check(first, want)
+    other, okw = planned("joined" if name != "joined" else "prefix_beside_long")
+    other.run(ops, causal, batch=other.batch(**okw))
+    assert torch.equal(bits(c.run(ops, causal, batch=c.batch(**kw))), bits(first))
+
+
+@pytest.mark.parametrize("name", list(ref.PLANS))
+def test_attention_bad_pages_every_plan(ops, name):
+    """Holes in the prefix's and the sequences' pages."""
+    c, kw = planned(name)
+    if c.prefix > 16:
+        c.prefix_table[1::3] = -1
+    c.table[:, 0::4] = c.kp.shape[0]
+    check(c.run(ops, True, batch=c.batch(**kw)), c.want(True))
+
+
+def test_attention_without_scratch(monkeypatch):
+    """A context without the split's scratch: every sequence by itself."""
+    monkeypatch.setenv("U15H_ATTN_SPLIT", "0")
+    o = u15h.Ops(0)
+    for name in ("joined", "prefix_tiled", "prefix_beside_long", "long_split",
+                 "long_beside_split"):
+        c, kw = planned(name)
+        check(c.run(o, True, batch=c.batch(**kw)), c.want(True))
+    torch.cuda.synchronize()
+    o.close()
+
+
+@pytest.mark.parametrize("names", [("joined", "prefix_tiled"), ("prefix_beside_long", "joined_rows"),
+                                   ("long_beside_split", "prefix_streamed")])
+def test_attention_captured(ops, names):
+    """Two graphs over one context's scratch, replayed in turn with eager calls
+    between, while lengths, starts and pages change under them."""
+    made = []
+    for name in names:
+        c, kw = planned(name)
+        kv = u15h.PagedKV(c.kp.cuda(), c.vp.cuda())
+        kv_len, q_start = torch.tensor(c.lens, dtype=I32).cuda(), c.q_start.cuda()
+        table = c.table.cuda()
+        b = u15h.PagedBatch(kv_len, table, q_start=q_start, max_q=max(c.counts),
+                            max_kv=kw["max_kv"], prefix_table=c.prefix_table.cuda(),
+                            prefix_len=c.prefix)
+        q = c.q.cuda()
+        out = torch.full_like(q, 5.0)
+        ops.paged_attention(kv, b, q, out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.paged_attention(kv, b, q, out)
+        made.append((c, kv, b, q, out, kv_len, q_start, table, g))
+    for step in range(4):
+        for c, kv, b, q, out, kv_len, q_start, table, g in made:
+            lens = [max(0, n - 7 * step) for n in c.lens]
+            counts = [max(0, n - step) for n in c.counts]
+            start = [0]
+            for n in counts:
+                start.append(start[-1] + n)
+            order = torch.roll(torch.arange(len(lens)), step).tolist()
+            tables = c.table[order]
+            lens = [lens[i] for i in order]
+            kv_len.copy_(torch.tensor(lens, dtype=I32))
+            q_start.copy_(torch.tensor(start, dtype=I32))
+            table.copy_(tables)
+            out.fill_(5.0)
+            g.replay()
+            got = out.clone()
+            out.fill_(5.0)
+            ops.paged_attention(kv, b, q, out)
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out), bits(got)), step
+            check(got[:start[-1]].cpu(),
+                  ref.attend(c.q[:start[-1]], c.kp, c.vp, c.prefix_table, c.prefix, tables, lens,
+                             counts, True))
+            assert bool((got[start[-1]:] == 5.0).all())
+
+
+def test_calls_on_another_stream(ops):
+    """All three on a stream that is not the current one, in its order."""
+    other = torch.cuda.Stream()
+    hq, hkv, d, T = 8, 2, 128, 70
+    rope, host, _ = rotation([(0, d, 0)])
+    qkv = bf16(3, T, hq + 2 * hkv, d).cuda()
+    pos = torch.arange(T, dtype=I32)[None].cuda()
+    slot = torch.arange(T, dtype=I32).cuda()
+    pool = torch.zeros(2, 5, hkv, 16, d, dtype=BF16, device="cuda")
+    kv = u15h.PagedKV(pool[0], pool[1])
+    q, out, y = (torch.zeros(T, hq, d, dtype=BF16, device="cuda") for _ in range(3))
+    b = u15h.PagedBatch(torch.tensor([T], dtype=I32).cuda(), torch.arange(5, dtype=I32)[None].cuda(),
+                        q_start=torch.tensor([0, T], dtype=I32).cuda(), max_q=T)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(20_000_000)
+        ops.paged_append(kv, qkv[:, hq:hq + hkv], qkv[:, hq + hkv:], slot, pos, rope, q=qkv[:, :hq],
+                         q_out=q, stream=other)
+        ops.paged_attention(kv, b, q, out, stream=other)
+        ops.rope(out, pos, rope, y, inverse=True, stream=other)
+    assert bool((y == 0).all())                      # not in the current stream's way
+    other.synchronize()
+    check(out.cpu(), ref.attend(q.cpu(), pool[0].cpu(), pool[1].cpu(), [], 0,
+                                [list(range(5))], [T], [T], True))
+    want, off = ref.turn(out.cpu(), pos.cpu(), host, inverse=True)
+    assert bool(((y.cpu().to(F64) - want).abs() <= off).all())
+
+
+def test_python_refusals(ops):
+    """What the Python forms refuse before the library is asked."""
+    c = Case([20], [1], 0, 8, 2, 64, 16)
+    kv, b = u15h.PagedKV(c.kp.cuda(), c.vp.cuda()), c.batch()
+    q = c.q[:1].cuda()
+    out = torch.empty_like(q)
+    rope, _, _ = rotation([(0, 64, 0)])
+    pos, slot = torch.zeros(1, 1, dtype=I32).cuda(), torch.zeros(1, dtype=I32).cuda()
+    k = torch.zeros(1, 2, 64, dtype=BF16, device="cuda")
+    wide = torch.zeros(1, 8, 128, dtype=BF16, device="cuda")
+    bad = [lambda: ops.paged_attention(kv, b, q.float(), out),
+           lambda: ops.paged_attention(kv, b, q.cpu(), out),
+           lambda: ops.paged_attention(kv, b, q[0], out),
+           lambda: ops.paged_attention(kv, b, q, out[:, :4]),
+           lambda: ops.paged_attention(kv, b, q[:, :7], out[:, :7]),
+           lambda: ops.paged_attention(kv, b, wide[..., ::2], out),
+           lambda: ops.paged_attention(kv, b, wide, wide.clone()),
+           lambda: ops.paged_attention(kv, b, q, out, scale=-1.0),
+           lambda: ops.rope(q, pos[0, :0], rope, out),
+           lambda: ops.rope(q, pos.long(), rope, out),
+           lambda: ops.rope(q, pos, rope, out[:, :2]),
+           lambda: ops.rope(q[..., :32], pos, rope, out[..., :32]),
+           lambda: ops.paged_append(kv, k, k[:, :1], slot),
+           lambda: ops.paged_append(kv, k, k, slot, rope=rope),
+           lambda: ops.paged_append(kv, k, k, slot.long()),
+           lambda: ops.paged_append(kv, k, k, slot, pos, rope, q=q),
+           lambda: ops.paged_append(kv, k, k, slot, q_out=out),
+           lambda: ops.paged_append(kv, k, k, slot, q=q, q_out=out),
+           lambda: u15h.PagedKV(c.kp.cuda(), c.vp.cuda()[1:]),
+           lambda: u15h.PagedKV(c.kp.cuda()[:, :, ::2], c.vp.cuda()[:, :, ::2]),
+           lambda: u15h.PagedKV(c.kp, c.vp),
+           lambda: u15h.PagedBatch(torch.zeros(2, dtype=I32).cuda(), c.table.cuda()),
+           lambda: u15h.PagedBatch(torch.zeros(1).cuda(), c.table.cuda()),
+           lambda: u15h.PagedBatch(torch.zeros(1, dtype=I32).cuda(), c.table.cuda(), max_q=2),
+           lambda: c.batch(max_kv=1000) and ops.paged_attention(kv, c.batch(max_kv=1000), q, out),
+           lambda: u15h.Rope([]),
+           lambda: u15h.Rope([(torch.zeros(4, device="cuda"), 0, 0)]),
+           lambda: u15h.Rope([(torch.zeros(4, dtype=F64, device="cuda"), 0, 3)])]
+    for i, f in enumerate(bad):
+        with pytest.raises((ValueError, TypeError, u15h.U15hError)):
+            f()
+            pytest.fail(f"refusal {i}")
+    ops.paged_attention(kv, b, q, out)
+    ops.paged_append(kv, k, k, slot)
 
 
 @pytest.mark.parametrize("batch,prefix", [(40, 700), (100, 64), (17, 2000), (3, 1000)])

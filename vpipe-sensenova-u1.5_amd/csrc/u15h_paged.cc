@@ -20,6 +20,8 @@ constexpr int kMaxTokens = 1 << 22;
 constexpr int kMaxBatch = 1 << 16;
 constexpr int kMaxKeys = 1 << 29;
 constexpr long long kMaxStride = 1LL << 40;      // elements between rows or pages
+constexpr long long kMaxGroups = 1LL << 23;      // workgroups of a launch: 2^31 threads
+constexpr float kLeastScale = 1e-12f, kMostScale = 1e12f;
 constexpr double kPi = 3.14159265358979323846;
 
 u15h_status
@@ -117,9 +119,10 @@ check_cache(u15h_ctx* ctx, const char* what, const u15h_paged_kv* kv, long long*
   }
   const long long whole = (long long)kv->kv_heads * kv->page * kv->head_dim;
   *page_stride = kv->page_stride == 0 ? whole : kv->page_stride;
-  if (*page_stride < whole || *page_stride % 8 != 0 || *page_stride > kMaxStride) {
-    return refuse(ctx, "%s: page_stride %lld (at least %lld, a multiple of 8)", what,
-                  (long long)kv->page_stride, whole);
+  if (*page_stride < whole || *page_stride % 8 != 0 ||
+      *page_stride > kMaxStride / std::max(kv->pages, 1)) {
+    return refuse(ctx, "%s: page_stride %lld (at least %lld, a multiple of 8; at most 2^40 "
+                  "elements over all pages)", what, (long long)kv->page_stride, whole);
   }
   if (kv->pages > 0 && (kv->k == nullptr || kv->v == nullptr)) {
     return refuse(ctx, "%s: null cache", what);
@@ -445,8 +448,9 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
                   what, bt->batch, bt->tokens, bt->max_q, bt->max_kv, bt->prefix_len,
                   bt->table_stride);
   }
-  if (!(scale >= 0.0f) || !(scale < INFINITY)) {
-    return refuse(ctx, "%s: scale %g (0 for 1/sqrt(head_dim), or positive)", what, (double)scale);
+  if (scale != 0.0f && !(scale >= kLeastScale && scale <= kMostScale)) {
+    return refuse(ctx, "%s: scale %g (0 for 1/sqrt(head_dim), or %g to %g)", what, (double)scale,
+                  (double)kLeastScale, (double)kMostScale);
   }
   if (bt->batch == 0 || bt->tokens == 0 || bt->max_q == 0) { return done(ctx); }
   if (bt->q_start == nullptr && bt->tokens < bt->batch) {
@@ -459,10 +463,12 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
   for (const int32_t* p : {bt->q_start, bt->kv_len, bt->table, bt->prefix_table}) {
     if (!aligned(p, 4)) { return refuse(ctx, "%s: tables must be 4-byte aligned", what); }
   }
-  // rows are counted in 32 bits, and so are the workgroups of 16 of them
-  const long long rows = (long long)std::min(bt->max_q, bt->tokens) * (hq / kv->kv_heads);
-  if ((long long)bt->tokens * hq >= (1LL << 31) ||
-      bt->batch * ((rows + 15) / 16) * kv->kv_heads >= (1LL << 31)) {
+  // rows are counted in 32 bits; each sequence has up to 4 streaming workgroups
+  // and a tile workgroup more than its rows fill
+  const long long groups =
+      ((long long)bt->batch * 5 + (long long)bt->tokens * (hq / kv->kv_heads) / 128) *
+      kv->kv_heads;
+  if ((long long)bt->tokens * hq >= (1LL << 31) || groups > kMaxGroups) {
     return refuse(ctx, "%s: %d sequences, %d rows of %d heads: too many", what, bt->batch,
                   bt->tokens, hq);
   }

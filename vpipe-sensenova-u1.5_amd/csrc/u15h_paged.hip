@@ -136,14 +136,15 @@ constexpr int kRopeGroup = 4;
 
 struct RopeGrid {
   int group;              // tokens of a workgroup
-  int heads;              // of its blockIdx.y's heads
-  int units;              // of a head
+  int heads;              // of its blockIdx.y's heads, of q, then k, then v
+  int units;              // of a head, 256 of them to a blockIdx.z
   int lanes;              // threads of a unit: heads at once
 };
 
-// A thread keeps its unit and steps over the (token, head) pairs, `lanes` of
-// them at a time over the workgroup.  Its first columns are on their way while
-// the angles are formed, later ones while the ones before are turned.
+// A thread keeps its unit and steps over the (token, head) pairs of q, then k,
+// then v, `lanes` of them at a time over the workgroup; addresses go by steps.
+// A pair's columns are on their way while the pair before is turned, the first
+// ones while the angles are formed.
 template <int VEC>
 __global__ __launch_bounds__(256) void
 rope_kernel(const RopeArgs A, const RopeGrid R)
@@ -153,133 +154,116 @@ rope_kernel(const RopeArgs A, const RopeGrid R)
   const int t0 = blockIdx.x * R.group;
   const int nt = min(R.group, A.tokens - t0);
   const int h0 = blockIdx.y * R.heads;
-  const int heads = min(R.heads, A.q.heads + A.k.heads + A.v.heads - h0);
+  const int unit0 = blockIdx.z * 256, units = min(R.units - unit0, 256);
+  const int lane = (unsigned)tid / (unsigned)units;
+  const RopeUnit u = rope_unit<VEC>(A, unit0 + tid - lane * units);
+
+  bool formed = false;
+  auto angles = [&] {
+    for (int i = tid; i < nt * A.pairs; i += 256) {
+      const int tok = (unsigned)i / (unsigned)A.pairs, pair = i - tok * A.pairs;
+      double turns = 0.0;
+#pragma unroll
+      for (int p = 0; p < U15H_MAX_ROPE_PARTS; ++p) {
+        if (p < A.nparts && pair >= A.part[p].pair) {
+          const RopePart& P = A.part[p];
+          if (pair - P.pair < P.width / 2) {
+            turns = (double)P.pos[t0 + tok] * (P.freq[pair - P.pair] * 0.15915494309189535);
+          }
+        }
+      }
+      turns -= __builtin_rint(turns);
+      float s, c;
+      sincospif(2.0f * (float)turns, &s, &c);
+      cs[i] = make_float2(c * A.scale, s * A.scale * A.sign);
+    }
+    __syncthreads();
+    formed = true;
+  };
 
   struct Item {
     Cols<VEC> a, b;
   };
-  RopeUnit u;
-  auto fetch = [&](int tok, int head, Item& I) {
-    const int t = t0 + tok;
-    int h = h0 + head;
-    const RopeRows& S = h < A.q.heads ? A.q : h < A.q.heads + A.k.heads ? A.k : A.v;
-    h -= h < A.q.heads ? 0 : h < A.q.heads + A.k.heads ? A.q.heads : A.q.heads + A.k.heads;
-    const uint16_t* x = S.x + t * S.x_tok + h * S.x_head;
-    I.a = load_cols<VEC>(x + u.a);
-    if (u.b >= 0) { I.b = load_cols<VEC>(x + u.b); }
-  };
-  auto finish = [&](int tok, int head, Item& I) {
-    const int t = t0 + tok;
-    int h = h0 + head;
-    bool turned = u.pair >= 0;
-    uint16_t* y;
-    if (A.slot != nullptr) {
-      const int slot = A.slot[t];
-      if ((unsigned)slot >= (unsigned)A.slots) { return; }
-      if (h < A.q.heads) {
-        y = A.q.y + t * A.q.y_tok + h * A.q.y_head;
-      } else {
-        h -= A.q.heads;
-        const bool key = h < A.k.heads;
-        h -= key ? 0 : A.k.heads;
-        turned = turned && key;
-        y = (key ? A.k.y : A.v.y) + (long long)(slot >> A.page_log2) * A.page_stride +
-            (((long long)h << A.page_log2) + (slot & ((1 << A.page_log2) - 1))) * A.d;
+  // The heads [lo, lo + n) of S, whose first is the workgroups' head `first`;
+  // kind 0: to strided rows, 1: to the cache.
+  auto walk = [&](const RopeRows& S, int first, bool cache, bool turn) {
+    const int lo = max(h0 - first, 0), n = min(h0 + R.heads - first, S.heads) - lo;
+    if (n <= 0) { return; }
+    const bool turned = turn && u.pair >= 0;
+    // one step: `lanes` pairs on, which is dq tokens and dr heads, and where
+    // that passes the last head one token more and n heads less
+    const int dq = R.lanes / n, dr = R.lanes - dq * n;
+    const long long step = dq * S.x_tok + dr * S.x_head, wrap = S.x_tok - n * S.x_head;
+    const long long ystep = dq * S.y_tok + dr * S.y_head, ywrap = S.y_tok - n * S.y_head;
+    int tok = lane / n, head = lane - tok * n;
+    if (lane >= R.lanes) { tok = nt; }
+    const uint16_t* x = S.x + (t0 + tok) * S.x_tok + (lo + head) * S.x_head;
+    uint16_t* y = S.y + (t0 + tok) * S.y_tok + (lo + head) * S.y_head;
+    auto fetch = [&](Item& I) {
+      I.a = load_cols<VEC>(x + u.a);
+      if (u.b >= 0) { I.b = load_cols<VEC>(x + u.b); }
+    };
+    Item I;
+    if (tok < nt) { fetch(I); }
+    if (!formed) { angles(); }
+    while (tok < nt) {
+      const int tok0 = tok, head0 = head;
+      uint16_t* y0 = y;
+      tok += dq;
+      head += dr;
+      x += step;
+      y += ystep;
+      if (head >= n) {
+        head -= n;
+        ++tok;
+        x += wrap;
+        y += ywrap;
       }
-    } else {
-      y = A.q.y + t * A.q.y_tok + h * A.q.y_head;
-    }
-    const float2* f = cs + tok * A.pairs + (turned ? u.pair : 0);
-    Cols<VEC>& a = I.a;
-    Cols<VEC>& b = I.b;
-    if (u.b >= 0) {
-      if (turned) {
+      Cols<VEC> a = I.a, b = I.b;
+      if (tok < nt) { fetch(I); }
+
+      if (A.slot != nullptr) {
+        const int slot = A.slot[t0 + tok0];
+        if ((unsigned)slot >= (unsigned)A.slots) { continue; }
+        if (cache) {
+          y0 = S.y + (slot >> A.page_log2) * A.page_stride +
+               (((long long)(lo + head0) << A.page_log2) + (slot & ((1 << A.page_log2) - 1))) * A.d;
+        }
+      }
+      const float2* f = cs + tok0 * A.pairs + (turned ? u.pair : 0);
+      if (u.b >= 0) {
+        if (turned) {
 #pragma unroll
-        for (int e = 0; e < (VEC + 1) / 2; ++e) {
-          const float2 f0 = f[2 * e];
-          const float a0 = bf16_lo(a.w[e]), b0 = bf16_lo(b.w[e]);
-          float a1 = 0.0f, b1 = 0.0f;
-          float2 f1 = make_float2(0.0f, 0.0f);
-          if constexpr (VEC > 1) {
-            f1 = f[2 * e + 1];
-            a1 = bf16_hi(a.w[e]);
-            b1 = bf16_hi(b.w[e]);
+          for (int e = 0; e < (VEC + 1) / 2; ++e) {
+            const float2 f0 = f[2 * e];
+            const float a0 = bf16_lo(a.w[e]), b0 = bf16_lo(b.w[e]);
+            float a1 = 0.0f, b1 = 0.0f;
+            float2 f1 = make_float2(0.0f, 0.0f);
+            if constexpr (VEC > 1) {
+              f1 = f[2 * e + 1];
+              a1 = bf16_hi(a.w[e]);
+              b1 = bf16_hi(b.w[e]);
+            }
+            a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, a1 * f1.x - b1 * f1.y);
+            b.w[e] = pack_bf16x2(b0 * f0.x + a0 * f0.y, b1 * f1.x + a1 * f1.y);
           }
-          a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, a1 * f1.x - b1 * f1.y);
-          b.w[e] = pack_bf16x2(b0 * f0.x + a0 * f0.y, b1 * f1.x + a1 * f1.y);
+        }
+        store_cols<VEC>(y0 + u.b, b);
+      } else if (turned) {
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          const float2 f0 = f[e];
+          const float a0 = bf16_lo(a.w[e]), b0 = bf16_hi(a.w[e]);
+          a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, b0 * f0.x + a0 * f0.y);
         }
       }
-      store_cols<VEC>(y + u.b, b);
-    } else if (turned) {
-#pragma unroll
-      for (int e = 0; e < VEC / 2; ++e) {
-        const float2 f0 = f[e];
-        const float a0 = bf16_lo(a.w[e]), b0 = bf16_hi(a.w[e]);
-        a.w[e] = pack_bf16x2(a0 * f0.x - b0 * f0.y, b0 * f0.x + a0 * f0.y);
-      }
+      store_cols<VEC>(y0 + u.a, a);
     }
-    store_cols<VEC>(y + u.a, a);
   };
-
-  // units past a thread's share of 256 (a head of many single columns) go round
-  // by round; all but those have one round
-  const int lane = R.lanes > 1 ? tid / R.units : 0;
-  const bool idle = lane >= R.lanes;
-  int tok = 0, head = lane;
-  while (head >= heads && tok < nt) {
-    head -= heads;
-    ++tok;
-  }
-  int unit = R.lanes > 1 ? tid - lane * R.units : tid;
-  Item I;
-  bool more = !idle && unit < R.units && tok < nt;
-  if (more) {
-    u = rope_unit<VEC>(A, unit);
-    fetch(tok, head, I);
-  }
-
-  for (int i = tid; i < nt * A.pairs; i += 256) {
-    const int tok = i / A.pairs, pair = i % A.pairs;
-    double turns = 0.0;
-#pragma unroll
-    for (int p = 0; p < U15H_MAX_ROPE_PARTS; ++p) {
-      if (p < A.nparts && pair >= A.part[p].pair) {
-        const RopePart& P = A.part[p];
-        if (pair - P.pair < P.width / 2) {
-          turns = (double)P.pos[t0 + tok] * (P.freq[pair - P.pair] * 0.15915494309189535);
-        }
-      }
-    }
-    turns -= __builtin_rint(turns);
-    float s, c;
-    sincospif(2.0f * (float)turns, &s, &c);
-    cs[i] = make_float2(c * A.scale, s * A.scale * A.sign);
-  }
-  __syncthreads();
-
-  while (more) {
-    int tok1 = tok, head1 = head + R.lanes;
-    while (head1 >= heads && tok1 < nt) {
-      head1 -= heads;
-      ++tok1;
-    }
-    if (tok1 >= nt && R.lanes == 1 && unit + 256 < R.units) {
-      // the thread's next unit, from the first pair on
-      finish(tok, head, I);
-      unit += 256;
-      u = rope_unit<VEC>(A, unit);
-      tok = 0;
-      head = 0;
-      fetch(tok, head, I);
-      continue;
-    }
-    Item J;
-    more = tok1 < nt;
-    if (more) { fetch(tok1, head1, J); }
-    finish(tok, head, I);
-    I = J;
-    tok = tok1;
-    head = head1;
+  walk(A.q, 0, false, true);
+  if (A.slot != nullptr) {
+    walk(A.k, A.q.heads, true, true);
+    walk(A.v, A.q.heads + A.k.heads, true, false);
   }
 }
 
@@ -297,13 +281,17 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
   RopeGrid g;
   g.group = a.tokens >= 1024 ? kRopeGroup : 1;
   const int groups = (a.tokens + g.group - 1) / g.group;
-  // few tokens: their heads over several workgroups, 128 units each or more
+  // Few tokens: their heads over several workgroups, 128 units each or more;
+  // of an append as many as the cache has, so that one walks q, k or v alone (64
+  // tokens of 32 + 8 + 8 heads: 5.2 -> 4.1 us).
   int cut = 1;
   while (groups * cut < 256 && heads * units / (cut * 2) >= 128) { cut *= 2; }
   g.heads = (heads + cut - 1) / cut;
+  if (a.slot != nullptr && groups < 512) { g.heads = a.k.heads; }
   g.units = units;
   g.lanes = std::max(1, 256 / units);
-  hipLaunchKernelGGL(rope_kernel<VEC>, dim3((unsigned)groups, (heads + g.heads - 1) / g.heads),
+  hipLaunchKernelGGL(rope_kernel<VEC>, dim3((unsigned)groups, (heads + g.heads - 1) / g.heads,
+                                            (units + 255) / 256),
                      dim3(256), 0, s, a, g);
   return hipGetLastError();
 }
