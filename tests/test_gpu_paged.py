@@ -140,7 +140,8 @@ def test_rope_gradient(ops):
 # ---- appending ----------------------------------------------------------------
 
 @pytest.mark.parametrize("tokens,hq,hkv,d,page", [(1, 32, 8, 128, 16), (67, 6, 2, 64, 32),
-                                                  (1030, 4, 4, 32, 256), (40, 0, 1, 128, 16)])
+                                                  (1030, 4, 4, 32, 256), (40, 0, 1, 128, 16),
+                                                  (300, 66, 1, 64, 16)])
 @pytest.mark.parametrize("parts", ["whole", "axes", "odd", None])
 def test_append(ops, tokens, hq, hkv, d, page, parts):
     """Keys, values and queries from columns of one matrix into slots in any

@@ -55,8 +55,11 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 // drops out exactly, so a position of 2^31 costs no precision: what is left is
 // in [-1/2, 1/2] and goes through sincospif in 32 bits.
 //
-// Memory-bound: 4 bytes an element; the angles are 1/16 of the work at 32
-// heads of 64 pairs.
+// Bound by memory, 4 bytes an element.  4224 tokens of 32 heads of 128 turned as
+// a whole, 69 MB: 14.4 us with inputs in the caches, 15.7 from memory, as a copy
+// of as many bytes; in the model's three parts, whose runs of 32 and 64 bytes
+// make more requests, 14.7 and 18.6.  Stepping addresses by addition in place of
+// products took a tenth off, a third of neighbouring pairs' 24.5 us.
 
 // Access unit u of a head: the first column of its one or two runs of VEC
 // columns (b -1: one run), and its first pair (-1: columns passed on).
@@ -131,7 +134,7 @@ store_cols(uint16_t* p, const Cols<VEC>& c)
 
 constexpr int kRopePairs = kRopeMaxHeadDim / 2;
 // Tokens of a workgroup: as many as give every thread an angle, once there are
-// workgroups enough.
+// workgroups enough.  (1, 2, 8: 21.5, 16.0, 18.4 us against 15.7.)
 constexpr int kRopeGroup = 4;
 
 struct RopeGrid {
@@ -184,8 +187,8 @@ rope_kernel(const RopeArgs A, const RopeGrid R)
   struct Item {
     Cols<VEC> a, b;
   };
-  // The heads [lo, lo + n) of S, whose first is the workgroups' head `first`;
-  // kind 0: to strided rows, 1: to the cache.
+  // The heads [lo, lo + n) of S, whose first is the workgroups' head `first`, to
+  // strided rows or to the cache's slots.
   auto walk = [&](const RopeRows& S, int first, bool cache, bool turn) {
     const int lo = max(h0 - first, 0), n = min(h0 + R.heads - first, S.heads) - lo;
     if (n <= 0) { return; }
@@ -283,11 +286,15 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
   const int groups = (a.tokens + g.group - 1) / g.group;
   // Few tokens: their heads over several workgroups, 128 units each or more;
   // of an append as many as the cache has, so that one walks q, k or v alone (64
-  // tokens of 32 + 8 + 8 heads: 5.2 -> 4.1 us).
+  // tokens of 32 + 8 + 8 heads: 5.2 -> 4.1 us), or twice, thrice .. as many where
+  // that makes thousands of workgroups.
   int cut = 1;
   while (groups * cut < 256 && heads * units / (cut * 2) >= 128) { cut *= 2; }
   g.heads = (heads + cut - 1) / cut;
-  if (a.slot != nullptr && groups < 512) { g.heads = a.k.heads; }
+  if (a.slot != nullptr && groups < 512) {
+    const long long all = (long long)groups * (heads / a.k.heads);
+    g.heads = a.k.heads * (int)((all + 4095) / 4096);
+  }
   g.units = units;
   g.lanes = std::max(1, 256 / units);
   hipLaunchKernelGGL(rope_kernel<VEC>, dim3((unsigned)groups, (heads + g.heads - 1) / g.heads,
@@ -316,6 +323,11 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
 // The running maximum is raised only when a score passes it by more than kLazy
 // (base 2): probabilities stay <= 2^kLazy and the quotient is the same.
 // The sum counts the probabilities as rounded to bf16 for the product.
+//
+// Bound by the keys' bytes: the products of 16 rows take a quarter of a tile's
+// time at the memory's rate.  131072 keys of 8 heads of 128 (537 MB) take 91 us,
+// 5.9 TB/s, one workgroup a CU; a workgroup alone takes 1.2 us per 128 keys and
+// 4.5 before and after.  Eight waves, or a second tile in registers, are level.
 
 constexpr float kLazy = 8.0f;
 
@@ -760,9 +772,11 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
   }
   if (A.joins == nullptr || direct) { return; }
 
-  // The last share of this block to arrive adds them all.  Every wave waits for
-  // its own writes to have reached the memory before the block counts as
-  // arrived.
+  // The last share of this block to arrive adds them all, which a second launch
+  // does 1 to 2 us slower where the shares are small (1800 keys of one request
+  // 11.4 -> 9.5 us) and 1 us faster where they are large (131072 keys).  Every
+  // wave waits for its own writes to have reached the memory before the block
+  // counts as arrived.
   __shared__ int arrived;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -853,6 +867,12 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
 // whose range ends at the last key; so no page ends inside it and keys past the
 // end read as zeros.  The page numbers of the next 16 tiles sit in a register,
 // a lane each, and are read a group of 16 tiles ahead.
+//
+// Bound by the matrix unit under the power cap: two workgroups of a CU take 1.8
+// us a tile of 64 keys (d = 128).  4096 queries of 32 heads over 4096 keys: 260
+// us, 1.06 PFLOP/s, as over the contiguous cache.  A round of workgroups starts
+// and ends in 13 us more: four images of 1024 queries over 333 + 1024 keys, two
+// rounds, 99 us, 0.92 PFLOP/s.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
@@ -1338,7 +1358,9 @@ in_sequence(const PagedArgs& A, int token)
 }
 
 // Adds the parts of a row, W waves a row, in the order of the parts:
-// out = sum f_p o_p / sum f_p l_p with f_p = 2^(m_p - max m).
+// out = sum f_p o_p / sum f_p l_p with f_p = 2^(m_p - max m).  All of a lane's
+// loads go out before the row is looked up.  Bound by latency and the parts'
+// bytes: 2048 rows of 7 parts 4.9 us, 8192 rows of 9 (38 MB) 12.4.
 template <int D, int W>
 __global__ __launch_bounds__(256) void
 paged_combine_kernel(const PagedArgs A)
