@@ -16,6 +16,7 @@
 
 struct u15h_ctx {
   std::string error;
+  bool cleared = false;
 };
 
 namespace {
@@ -23,8 +24,16 @@ namespace {
 std::string g_out;
 int g_cus = 256;
 size_t g_bytes = 0;
+bool g_capturing = false;
 
 }  // namespace
+
+hipError_t
+hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus* status)
+{
+  *status = g_capturing ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
+  return hipSuccess;
+}
 
 namespace u15h {
 
@@ -44,6 +53,15 @@ attention_scratch(const u15h_ctx*, size_t* bytes)
 }
 
 int compute_units(const u15h_ctx*) { return g_cus; }
+
+bool* joins_cleared(u15h_ctx* ctx) { return &ctx->cleared; }
+
+hipError_t
+launch_clear_joins(int* joins, hipStream_t)
+{
+  g_out += joins == reinterpret_cast<int*>(4096 + g_bytes) ? "clear " : "clear elsewhere ";
+  return hipSuccess;
+}
 
 u15h_status
 set_error(u15h_ctx* ctx, u15h_status st, const char* msg)
@@ -117,6 +135,7 @@ main(int argc, char** argv)
     };
     g_out.clear();
     ctx.error.clear();
+    g_capturing = n("capturing", 0) != 0;
     u15h_status st = U15H_OK;
     const int d = n("d", 128), heads = n("heads", 8);
     u15h_rope_spec r = {};

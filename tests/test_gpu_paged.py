@@ -394,6 +394,31 @@ def test_attention_captured(ops, names):
             assert bool((got[start[-1]:] == 5.0).all())
 
 
+def test_attention_first_call_captured():
+    """A context whose first joined call is captured and runs after an eager one."""
+    o = u15h.Ops(0)
+    junk = torch.full((64 << 20,), 7, dtype=torch.uint8, device="cuda")     # what memory held
+    c, kw = planned("joined")
+    kv, b = u15h.PagedKV(c.kp.cuda(), c.vp.cuda()), c.batch(**kw)
+    q = c.q.cuda()
+    out, eager = torch.zeros_like(q), torch.zeros_like(q)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o.paged_attention(kv, b, q, out)
+    o.paged_attention(kv, b, q, eager)
+    for _ in range(3):
+        out.fill_(0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bits(out), bits(eager))
+        o.paged_attention(kv, b, q, eager)
+    check(eager[:c.rows].cpu(), c.want(True))
+    torch.cuda.synchronize()
+    del g, junk
+    o.close()
+
+
 def test_calls_on_another_stream(ops):
     """All three on a stream that is not the current one, in its order."""
     other = torch.cuda.Stream()

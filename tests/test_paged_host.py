@@ -146,6 +146,14 @@ def test_every_batch_has_a_plan(host, cus, scratch):
     assert kinds == ({"none", "stream", "tile"} if scratch else {"none"})
 
 
+def test_counters_are_cleared_before_they_count(host):
+    """By the first call that counts; a captured one leaves that to the next."""
+    join, other = "attn batch=1 heads=2 hq=8 max_kv=1800", "attn batch=3"
+    got = [launch.split(" parts")[0] for launch, _ in host(
+        [other, join + " capturing=1", join + " capturing=1", join, join, join + " capturing=1"])]
+    assert got == ["attn", "clear attn", "clear attn", "clear attn", "attn", "attn"]
+
+
 # ---- frequencies ------------------------------------------------------------------
 
 def test_rope_freqs():

@@ -60,6 +60,7 @@ struct u15h_ctx {
   // no call splits) and env U15H_ATTN_SPLIT: -1 the planner's key shares,
   // 0 none, n >= 2 that many.
   void* attn_ws = nullptr;
+  bool joins_cleared = false;       // the counters behind attn_ws are 0
   int attn_split = -1;
   bool i8_on = false;
   int i8_min_m = 1024;
@@ -202,7 +203,7 @@ set_tiles(GemmBatch& b, Epi epi, int bm, int bn)
 // Scratch of split attention calls, per context.
 constexpr size_t kAttnWsBytes = (size_t)32 << 20;
 // Counters behind it (paged attention's shares that have arrived), 0 between
-// calls.
+// calls once a kernel has cleared them.
 constexpr size_t kAttnCountBytes = (size_t)u15h::kPagedJoins * sizeof(int);
 
 // Fewest K stages a split share may have.
@@ -783,6 +784,12 @@ u15h::attention_scratch(const u15h_ctx* ctx, size_t* bytes)
   return ctx->attn_ws;
 }
 
+bool*
+u15h::joins_cleared(u15h_ctx* ctx)
+{
+  return &ctx->joins_cleared;
+}
+
 int
 u15h::compute_units(const u15h_ctx* ctx)
 {
@@ -877,11 +884,7 @@ u15h_create(int device, u15h_ctx** out)
   ctx->i8_min_m = std::max(1, env_int("U15H_I8_MIN_M", 1024));
   ctx->attn_split = env_int("U15H_ATTN_SPLIT", -1);
   if (ctx->attn_split != 0 &&
-      (hipMalloc(&ctx->attn_ws, kAttnWsBytes + kAttnCountBytes) != hipSuccess ||
-       hipMemset(static_cast<char*>(ctx->attn_ws) + kAttnWsBytes, 0, kAttnCountBytes) !=
-           hipSuccess ||
-       hipStreamSynchronize(nullptr) != hipSuccess)) {
-    if (ctx->attn_ws != nullptr) { (void)hipFree(ctx->attn_ws); }
+      hipMalloc(&ctx->attn_ws, kAttnWsBytes + kAttnCountBytes) != hipSuccess) {
     ctx->attn_ws = nullptr;
     (void)hipGetLastError();
   }

@@ -412,6 +412,8 @@ paged_ws_bytes(const PagedArgs& a)
   return n > 1 ? (size_t)n * a.tokens * a.hq * (a.d + 2) * 4 : 0;
 }
 hipError_t launch_paged_attention(const PagedArgs& a, hipStream_t s);
+// Sets kPagedJoins counters to 0.
+hipError_t launch_clear_joins(int* joins, hipStream_t s);
 bool paged_kernels_loadable();
 
 // What entry points outside u15h_api.cc need of the context: the device made
@@ -425,9 +427,10 @@ int gemm_cus(const u15h_ctx* ctx);
 u15h_status split_workspace(u15h_ctx* ctx, void** ws);
 size_t split_workspace_bytes(const u15h_ctx* ctx);
 // The scratch of attention split over the keys, null where there is none, with
-// kPagedJoins counters (0 between calls) behind its `bytes`; the device's
-// compute units.
+// kPagedJoins counters behind its `bytes`; whether those are 0, as they are
+// between calls once a call has cleared them; the device's compute units.
 void* attention_scratch(const u15h_ctx* ctx, size_t* bytes);
+bool* joins_cleared(u15h_ctx* ctx);
 int compute_units(const u15h_ctx* ctx);
 
 // Forces every kernel's code object to load; false if any cannot.

@@ -503,8 +503,17 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
   void* ws = u15h::attention_scratch(ctx, &bytes);
   plan(a, u15h::compute_units(ctx), ws, bytes);
   if ((st = u15h::begin_call(ctx)) != U15H_OK) { return st; }
-  return u15h::end_call(
-      ctx, u15h::launch_paged_attention(a, reinterpret_cast<hipStream_t>(stream)), what);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a.joins != nullptr && !*u15h::joins_cleared(ctx)) {
+    // The context's first call that counts.  A captured clear runs when its graph
+    // does, so it says nothing about the next call's counters.
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(s, &capture);
+    if (e == hipSuccess) { e = u15h::launch_clear_joins(a.joins, s); }
+    if (e != hipSuccess) { return u15h::end_call(ctx, e, what); }
+    *u15h::joins_cleared(ctx) = capture == hipStreamCaptureStatusNone;
+  }
+  return u15h::end_call(ctx, u15h::launch_paged_attention(a, s), what);
 }
 
 }  // extern "C"

@@ -1450,6 +1450,12 @@ paged_combine_kernel(const PagedArgs A)
   }
 }
 
+__global__ __launch_bounds__(256) void
+clear_joins_kernel(int* joins)
+{
+  joins[blockIdx.x * 256 + threadIdx.x] = 0;
+}
+
 template <int D>
 hipError_t
 launch_paged_d(const PagedArgs& a, hipStream_t s)
@@ -1503,10 +1509,19 @@ launch_paged_attention(const PagedArgs& a, hipStream_t s)
   return launch_paged_d<32>(a, s);
 }
 
+hipError_t
+launch_clear_joins(int* joins, hipStream_t s)
+{
+  static_assert(kPagedJoins % 256 == 0, "a thread a counter");
+  hipLaunchKernelGGL(clear_joins_kernel, dim3(kPagedJoins / 256), dim3(256), 0, s, joins);
+  return hipGetLastError();
+}
+
 bool
 paged_kernels_loadable()
 {
   const void* fns[] = {
+      reinterpret_cast<const void*>(&clear_joins_kernel),
       reinterpret_cast<const void*>(&rope_kernel<8>),
       reinterpret_cast<const void*>(&rope_kernel<2>),
       reinterpret_cast<const void*>(&rope_kernel<1>),
