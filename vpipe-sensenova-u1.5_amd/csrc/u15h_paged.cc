@@ -164,7 +164,17 @@ cut(long long keys, long long n, int* shares, int* chunk)
 
 // How a call is cut (PagedArgs): what the prefix's workgroups and the
 // sequences' walk.  Lengths are known to their bounds only; own keys are taken
-// as half of max_kv on the mean.
+// as half of max_kv on the mean.  Measured in a graph, 32 query heads over 8 of
+// 128 unless said, us:
+//  - the prefix once for all / by every sequence: 4 queries behind 8192 keys 13.2
+//    / 19.7, 128 behind 500 25 / 35, 20 of 8 queries behind 4000 30 / 44; below
+//    4096 keys walked again, 8 behind 256 11.1 / 8.0, 2 behind 600 11.0 / 11.1;
+//  - its rows on tiles / streaming: 256 rows behind 4224 keys 36 / 45, 640 rows
+//    (heads of 64) behind 8192 18 / 28; 64 rows and fewer stream;
+//  - a sequence of 100 queries whose 400 rows walk 3000 keys in shares / whole 39
+//    / 47 (five of them), of 300 over 5000 keys 48 / 101;
+//  - parts added by the last share / by a second kernel: 1800 keys of one request
+//    9.5 / 11.4, three of 20000 to 40000 81 / 79.
 void
 plan(PagedArgs& a, int cus, void* ws, size_t bytes)
 {
@@ -246,7 +256,8 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
     // at most one streaming workgroup a CU for a sequence by itself (which
     // fills the memory's rate), four for several
     const long long s_most = (a.batch == 1 ? 1LL : 4LL) * cus / s_items;
-    shares_of(keys / 128.0 * (work < 10.0 ? 1.0 : 2.0), std::min(most, s_most), &a.s_shares, &a.s_chunk);
+    shares_of(keys / 128.0 * (work < 10.0 ? 1.0 : 2.0), std::min(most, s_most), &a.s_shares,
+              &a.s_chunk);
     shares_of(keys / 64.0 * tile, std::min(most, 4LL * cus / t_items), &a.t_shares, &a.t_chunk);
     while (u15h::paged_ws_bytes(a) > bytes && a.s_shares + a.t_shares > 2) {
       cut(keys, std::max(a.s_shares - 1, 1), &a.s_shares, &a.s_chunk);
@@ -257,6 +268,7 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
     }
     if (!phase || u15h::paged_ws_bytes(a) <= bytes) { break; }
   }
+  // Small calls of sequences by themselves are added by their own workgroups.
   const int rb = 16 * a.nr;
   const long long joins =
       (std::min<long long>(rows1, u15h::kPagedShortRows) + rb - 1) / rb * a.hkv * a.batch;
