@@ -334,6 +334,29 @@ def test_attention_bad_pages_every_plan(ops, name):
     check(c.run(ops, True, batch=c.batch(**kw)), c.want(True))
 
 
+@pytest.mark.parametrize("name", list(ref.PLANS))
+def test_attention_nan(ops, name):
+    """A NaN in a query reaches its own row and head, one in a key that a query
+    sees all heads of that key's, one in a key that the mask hides nothing."""
+    c, kw = planned(name)
+    G = c.q.shape[1] // c.kp.shape[1]
+    want = c.want(True)
+    clean = c.run(ops, True, batch=c.batch(**kw))
+    row = c.rows - 1
+    c.q[row, 1, 5] = math.nan
+    nan = torch.zeros(c.rows, c.q.shape[1], dtype=torch.bool)
+    nan[row, 1] = c.prefix > 0 or c.lens[-1] > 0
+    # the last key of the sequence with most queries: the last of those sees it
+    b = max(range(len(c.lens)), key=lambda i: c.counts[i])
+    n = c.lens[b]
+    c.kp[int(c.table[b, (n - 1) // 16]), 0, (n - 1) % 16, 3] = math.nan
+    nan[int(c.q_start[b + 1]) - 1, :G] = True
+    out = c.run(ops, True, batch=c.batch(**kw))
+    assert torch.equal(torch.isnan(out).any(-1), nan) and torch.equal(torch.isnan(out).all(-1), nan)
+    assert torch.equal(bits(out[~nan]), bits(clean[~nan]))
+    check(clean, want)
+
+
 def test_attention_without_scratch(monkeypatch):
     """A context without the split's scratch: every sequence by itself."""
     monkeypatch.setenv("U15H_ATTN_SPLIT", "0")

@@ -389,6 +389,13 @@ sequence(const PagedArgs& A, int b)                    // b the same in all lane
 // sum kNoKey where the part saw no key of it, kFinal in part 0 where the row's
 // output is written already).
 constexpr float kNoKey = -1.0f, kFinal = -2.0f;
+// The sum to leave of a maximum and a sum.  (Scores that are all NaN leave the
+// maximum as it was and a sum that is not 0: they are passed on.)
+__device__ __forceinline__ float
+sum_of(float m, float l)
+{
+  return m == -INFINITY && l == 0.0f ? kNoKey : l;
+}
 struct Part {
   float* o;
   float2* ml;
@@ -753,15 +760,15 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
       const long long at = part_row(A, S.first + row / G, kvh * G + row % G);
       if (A.joins != nullptr) {
         if (c == 0) {
-          give(reinterpret_cast<float*>(P.ml + at), top, top == -INFINITY ? kNoKey : sum);
+          give(reinterpret_cast<float*>(P.ml + at), top, sum_of(top, sum));
         }
-        if (top == -INFINITY) { continue; }
+        if (sum_of(top, sum) == kNoKey) { continue; }
         give(P.o + at * D + c, acc[0], acc[1]);
         give(P.o + at * D + c + 2, acc[2], acc[3]);
         continue;
       }
-      if (c == 0) { P.ml[at] = make_float2(top, top == -INFINITY ? kNoKey : sum); }
-      if (top == -INFINITY) { continue; }
+      if (c == 0) { P.ml[at] = make_float2(top, sum_of(top, sum)); }
+      if (sum_of(top, sum) == kNoKey) { continue; }
       *reinterpret_cast<f32x4_t*>(P.o + at * D + c) = acc;
       continue;
     }
@@ -837,7 +844,7 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
       *reinterpret_cast<f32x4_t*>(so(slot / RB) + slot % RB * D + c) = acc;
       if (c == 0) {
         o3[2 * slot] = m;
-        o3[2 * slot + 1] = m == -INFINITY ? kNoKey : l;
+        o3[2 * slot + 1] = sum_of(m, l);
       }
       __syncthreads();
       if (grp == 0) {
@@ -1283,8 +1290,8 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
   if (!direct) {
     const Part P = part_of(A, part);
     const long long at = part_row(A, S.first + tok, h);
-    if (half == 0) { P.ml[at] = make_float2(m * scale, m == -INFINITY ? kNoKey : l); }
-    if (m == -INFINITY) { return; }
+    if (half == 0) { P.ml[at] = make_float2(m * scale, sum_of(m, l)); }
+    if (sum_of(m, l) == kNoKey) { return; }
     float* op = P.o + at * D;
 #pragma unroll
     for (int cb = 0; cb < NCB; ++cb) {
@@ -1419,13 +1426,13 @@ paged_combine_kernel(const PagedArgs A)
     float o1[C];
 #pragma unroll
     for (int e = 0; e < C; ++e) { o1[e] = __shfl_xor(o[e], 32); }
-    add(m1, m1 == -INFINITY ? kNoKey : l1, o1);
+    add(m1, sum_of(m1, l1), o1);
   }
   if constexpr (W > 1) {
     if (half == 0) {
 #pragma unroll
       for (int e = 0; e < C; ++e) { so[wave][c + e] = o[e]; }
-      if (lane == 0) { sml[wave] = make_float2(m, m == -INFINITY ? kNoKey : l); }
+      if (lane == 0) { sml[wave] = make_float2(m, sum_of(m, l)); }
     }
     __syncthreads();
     if (wave % W != 0) { return; }
