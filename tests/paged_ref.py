@@ -123,6 +123,10 @@ PLANS = {
     "long_beside_split": ([700, 3000, 90, 400], [680, 1, 1, 2], 0, (32, 1, 64),
                           dict(max_kv=4096, wide=256), r"none s=1:(?!1x)"),
     "seventy": ([40, 3] * 35, [20, 1] * 35, 30, (8, 2, 32), {}, r"none .* t=1:"),
+    "seventy_behind_a_prefix": ([40, 3] * 35, [20, 1] * 35, 300, (8, 2, 32), {},
+                                r"tile s=1:.* t=1:"),
+    "head_group_of_80_behind_a_prefix": ([30, 9, 77, 1, 5, 60], [1, 2, 1, 1, 1, 1], 900,
+                                         (80, 1, 64), {}, r"tile s=0:.* t=1:"),
     "head_group_of_80": ([90, 300], [1, 3], 33, (80, 1, 64), {}, r"s=0:.* t=1:"),
 }
 

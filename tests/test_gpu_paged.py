@@ -597,6 +597,72 @@ def test_attention_page_stride_and_offsets(ops):
     check(out.cpu(), c.want(True))
 
 
+# ---- the largest calls ----------------------------------------------------------
+
+@pytest.mark.parametrize("tokens,heads,d,turned", [(1 << 22, 1, 16, 16), (3, 4096, 32, 32),
+                                                   (5, 4096, 512, 30), (1500, 300, 512, 500),
+                                                   (1, 1, 512, 2)])
+def test_rope_largest(ops, tokens, heads, d, turned):
+    rope, host, _ = rotation([(0, turned, 1)])                  # theta 1e4
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    x = torch.randn(tokens, heads, d, device="cuda", generator=g).to(BF16)
+    y = torch.full_like(x, math.nan)
+    pos = torch.arange(tokens, dtype=I32, device="cuda")[None].repeat(2, 1)
+    ops.rope(x, pos, rope, y)
+    parts = [(f.cuda(), s, a) for f, s, a in host]
+    step = max(1, (1 << 22) // (heads * d))
+    for t in range(0, tokens, step):
+        want, off = ref.turn(x[t:t + step], pos[:, t:t + step], parts)
+        assert bool(((y[t:t + step].to(F64) - want).abs() <= off).all()), t
+
+
+def test_append_4096_heads(ops):
+    """As the rotation by itself, values bit for bit."""
+    hq, hkv, d, T = 4096, 64, 32, 40
+    rope, _, _ = rotation([(0, d, 0)])
+    q, k, v = bf16(1, T, hq, d).cuda(), bf16(2, T, hkv, d).cuda(), bf16(3, T, hkv, d).cuda()
+    pool = torch.zeros(2, 4, hkv, 16, d, dtype=BF16, device="cuda")
+    pos = torch.arange(T, dtype=I32, device="cuda")[None]
+    out, yq, yk = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(k)
+    ops.paged_append(u15h.PagedKV(pool[0], pool[1]), k, v, pos[0].contiguous(), pos, rope, q=q,
+                     q_out=out)
+    ops.rope(q, pos, rope, yq)
+    ops.rope(k, pos, rope, yk)
+    slots = pool.transpose(2, 3).flatten(1, 2)[:, :T]
+    assert torch.equal(bits(out), bits(yq)) and torch.equal(bits(slots[0]), bits(yk))
+    assert torch.equal(bits(slots[1]), bits(v))
+
+
+@pytest.mark.parametrize("prefix", [0, 60])
+def test_attention_20000_sequences(ops, prefix):
+    """More sequences than are looked at together; the reference on the GPU in 64
+    bits, within the weights' and the output's rounding of values below 6."""
+    b, hq, hkv, d, most = 20000, 8, 2, 32, 40
+    g = torch.Generator(device="cuda").manual_seed(prefix)
+    lens = torch.randint(0, most, (b,), device="cuda", generator=g).to(I32)
+    table = torch.randint(0, 500, (b, 3), device="cuda", generator=g).to(I32)
+    kp, vp = (torch.randn(500, hkv, 16, d, device="cuda", generator=g).to(BF16)
+              for _ in range(2))
+    q = torch.randn(b, hq, d, device="cuda", generator=g).to(BF16)
+    out = torch.full_like(q, math.nan)
+    pt = torch.arange(40, 44, device="cuda", dtype=I32)
+    ops.paged_attention(u15h.PagedKV(kp, vp),
+                        u15h.PagedBatch(lens, table, max_kv=most, prefix_table=pt,
+                                        prefix_len=prefix), q, out)
+    both = []
+    for pool in (kp, vp):
+        own = pool[table.long()].transpose(2, 3).flatten(1, 2)[:, :most]
+        first = pool[pt.long()].transpose(1, 2).flatten(0, 1)[:prefix].expand(b, -1, -1, -1)
+        both.append(torch.cat([first, own], 1).to(F64).repeat_interleave(hq // hkv, 2))
+    s = (q.to(F64)[:, None] * both[0]).sum(-1) / math.sqrt(d)
+    hidden = torch.arange(prefix + most, device="cuda")[None] >= prefix + lens[:, None]
+    s = s.masked_fill(hidden[..., None], -math.inf)
+    w = torch.softmax(s, 1).nan_to_num(0.0)
+    want = (w[..., None] * both[1]).sum(1)
+    assert float(both[1].abs().max()) < 6
+    assert float((out.to(F64) - want).abs().max()) <= 2.1 * 2.0 ** -8 * 6
+
+
 # ---- a step -------------------------------------------------------------------
 
 def test_step_with_the_layer_s_operators(ops):
