@@ -169,6 +169,8 @@ cut(long long keys, long long n, int* shares, int* chunk)
 //  - the prefix once for all / by every sequence: 4 queries behind 8192 keys 13.2
 //    / 19.7, 128 behind 500 25 / 35, 20 of 8 queries behind 4000 30 / 44; below
 //    4096 keys walked again, 8 behind 256 11.1 / 8.0, 2 behind 600 11.0 / 11.1;
+//  - shares of it that make 256 tile workgroups / 512: 128 queries behind 16384
+//    keys 58 / 75, 200 behind 8192 65 / 77, 256 behind 32768 189 / 194 (384: 181);
 //  - its rows on tiles / streaming: 256 rows behind 4224 keys 36 / 45, 640 rows
 //    (heads of 64) behind 8192 18 / 28; 64 rows and fewer stream;
 //  - a sequence of 100 queries whose 400 rows walk 3000 keys in shares / whole 39
@@ -209,17 +211,21 @@ plan(PagedArgs& a, int cus, void* ws, size_t bytes)
         int shares, chunk;
         cut(a.prefix, n, &shares, &chunk);
         const double items = (double)blocks * shares;
-        double busy;
+        double us;
         if (a.p_tile) {
-          // beside streaming workgroups a tile takes half as long again; two
-          // tile workgroups on a CU take twice as long
+          // A tile workgroup to a CU: the sequences' workgroups run beside it, and
+          // a tile takes half as long again.  Two to a CU: those wait, and a pair
+          // of tiles takes twice as long.
           const double walk = chunk / 64.0 * tile;
-          busy = std::max(1.5 * walk, std::ceil(items / cus) * walk);
+          const double beside = std::max(own, 1.5 * walk + 5.0);
+          const double after = std::max(items / cus, 2.0) * walk + own + 5.0;
+          const double full = std::min(std::max((items - cus) / cus, 0.0), 1.0);
+          us = (1.0 - full) * beside + full * after + (items > cus ? 4.0 : 0.0);
         } else {
           const double walk = chunk / 128.0 * 1.2;
-          busy = std::max(walk, items / (2 * cus) * walk);
+          us = std::max(own, std::max(walk, items / (2 * cus) * walk) + 5.0);
         }
-        const double us = std::max(own, busy + 5.0) + (part + 0.15) * shares;
+        us += (part + 0.15) * shares;
         if (us < best) {
           best = us;
           a.p_shares = shares;
