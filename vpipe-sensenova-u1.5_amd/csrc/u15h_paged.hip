@@ -1367,7 +1367,7 @@ in_sequence(const PagedArgs& A, int token)
 // Adds the parts of a row, W waves a row, in the order of the parts:
 // out = sum f_p o_p / sum f_p l_p with f_p = 2^(m_p - max m).  All of a lane's
 // loads go out before the row is looked up.  Bound by latency and the parts'
-// bytes: 2048 rows of 7 parts 4.9 us, 8192 rows of 9 (38 MB) 12.4.
+// bytes: 2048 rows of 7 parts 4.9 us, 8192 rows of 7 (30 MB) 12.4.
 template <int D, int W>
 __global__ __launch_bounds__(256) void
 paged_combine_kernel(const PagedArgs A)
