@@ -385,7 +385,7 @@ struct PagedArgs {
   int nr;                       // 16-row blocks of a streaming workgroup: 1, 2
   // With more than one part (p_shares + the larger of the others): their
   // unnormalised outputs [part][tokens * hq][d] f32, then the rows' running
-  // maxima (base 2) and sums.
+  // maxima (of the unscaled scores) and sums.
   float* ws;
   // Streaming workgroups only, every sequence by itself: the last of a block's
   // shares adds them, counted in joins[block], which it leaves at 0; null: a

@@ -320,9 +320,14 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
 //  - The first operand wants 8 keys of one column a lane.  A lane loads 8 keys
 //    x D / 16 consecutive columns (whole rows over 16 lanes) and transposes
 //    them among its own registers, one v_perm a pair of keys and column.
-// The running maximum is raised only when a score passes it by more than kLazy
-// (base 2): probabilities stay <= 2^kLazy and the quotient is the same.
-// The sum counts the probabilities as rounded to bf16 for the product.
+// The running maximum, in the scores' own units, is raised only when a score
+// passes it by more than kLazy / scale: probabilities stay <= 2^(2 kLazy) and the
+// quotient is the same.  Where the scaled maximum is large the difference comes
+// before the product (kFused).
+// Probabilities are rounded to bf16, the type in which the matrix unit multiplies
+// them by V at its full rate, and the sum counts them as rounded, so that a row's
+// weights add up to 1: an output moves by at most 2^-8 of the spread of its values,
+// as its own rounding moves it by 2^-8 of itself.
 //
 // Bound by the keys' bytes: the products of 16 rows take a quarter of a tile's
 // time at the memory's rate.  131072 keys of 8 heads of 128 (537 MB) take 91 us,
@@ -330,6 +335,13 @@ launch_rope_vec(const RopeArgs& a, hipStream_t s)
 // 4.5 before and after.  Eight waves, or a second tile in registers, are level.
 
 constexpr float kLazy = 8.0f;
+// Exponents are one fma, score * scale - (max * scale), whose last product is
+// rounded: to 2^10 that is at most 2^-14 of a weight, but it grows with the product
+// and past 2^31 exceeds the exponential's range, 2^127 and 0 in place of 1.  So above
+// 2^10 they are (score - max) * scale, 0 at the maximum whatever the scale: such a
+// row takes the maximum's branch at every tile, and other rows pay nothing (269 us
+// for 4096 queries over 4096 keys, as without it; a test of its own: 276).
+constexpr float kFused = 1024.0f;
 
 __device__ __forceinline__ f32x4_t
 mma16(i32x4_t a, i32x4_t b, f32x4_t c)
@@ -385,9 +397,9 @@ sequence(const PagedArgs& A, int b)                    // b the same in all lane
   return {uniform(S.first), uniform(S.n), uniform(S.keys)};
 }
 
-// The partial results of part p: row r's output, and its maximum and sum (the
-// sum kNoKey where the part saw no key of it, kFinal in part 0 where the row's
-// output is written already).
+// The partial results of part p: row r's output, and its maximum (of the unscaled
+// scores) and sum (the sum kNoKey where the part saw no key of it, kFinal in part 0
+// where the row's output is written already).
 constexpr float kNoKey = -1.0f, kFinal = -2.0f;
 // The sum to leave of a maximum and a sum.  (Scores that are all NaN leave the
 // maximum as it was and a sum that is not 0: they are passed on.)
@@ -633,14 +645,17 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
 
   f32x4_t o[NR][DPL];
   float m[NR], l[NR];
+  float mc[NR];                              // what the exponents have subtracted
+  float edge[NR];                            // scores past it raise the maximum
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
-    m[n] = -INFINITY;
-    l[n] = 0.0f;
+    m[n] = edge[n] = -INFINITY;
+    l[n] = mc[n] = 0.0f;
 #pragma unroll
     for (int j = 0; j < DPL; ++j) { o[n][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}; }
   }
   const float scale = A.scale;
+  const float lazy = kLazy / scale;
 
   if (mine > 0) {
     load_k(0);
@@ -684,20 +699,30 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
     for (int n = 0; n < NR; ++n) {
       float mx = fmaxf(fmaxf(fmaxf(sc[n][0][0], sc[n][0][1]), fmaxf(sc[n][0][2], sc[n][0][3])),
                        fmaxf(fmaxf(sc[n][1][0], sc[n][1][1]), fmaxf(sc[n][1][2], sc[n][1][3])));
-      mx *= scale;
-      if (__any(mx > m[n] + kLazy)) {
+      if (__any(mx > edge[n])) {
         mx = fmaxf(max_groups(mx), m[n]);
-        const float alpha = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[n] - mx);
+        const float alpha =
+            m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mx) * scale);
         m[n] = mx;
         l[n] *= alpha;
 #pragma unroll
         for (int j = 0; j < DPL; ++j) { o[n][j] *= alpha; }
+        if (mx != -INFINITY) {
+          mc[n] = mx * scale;
+          edge[n] = mx + lazy;
+          if (fabsf(mc[n]) > kFused) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { sc[n][e >> 2][e & 3] -= mx; }
+            mc[n] = 0.0f;
+            edge[n] = -INFINITY;
+          }
+        }
       }
-      const float mc = m[n] == -INFINITY ? 0.0f : m[n];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n][p >> 1][(2 * p) & 3], scale, -mc));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[n][p >> 1][(2 * p + 1) & 3], scale, -mc));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[n][p >> 1][(2 * p) & 3], scale, -mc[n]));
+        const float p1 =
+            __builtin_amdgcn_exp2f(fmaf(sc[n][p >> 1][(2 * p + 1) & 3], scale, -mc[n]));
         const uint32_t pk = pack_bf16x2(p0, p1);
         pf[n][p] = (int)pk;
         l[n] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pk),
@@ -749,7 +774,8 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - top);
+      const float f =
+          sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm[w][r] - top) * scale);
       sum += f * sl[w][r];
       acc += f * *reinterpret_cast<const f32x4_t*>(
                      so(w) + r * D + (((c >> 2) ^ (r & 15)) & (D / 4 - 1)) * 4);
@@ -814,7 +840,8 @@ stream_item(const PagedArgs& A, int item, float* o0, float* o1, float* o2, float
     auto add = [&](float m1, float l1, f32x4_t o1) {
       if (l1 < 0.0f) { return; }
       const float top = fmaxf(m, m1);
-      const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+      const float f0 = __builtin_amdgcn_exp2f((m - top) * scale);
+      const float f1 = __builtin_amdgcn_exp2f((m1 - top) * scale);
       l = __builtin_fmaf(l, f0, l1 * f1);
 #pragma unroll
       for (int e = 0; e < 4; ++e) { acc[e] = __builtin_fmaf(o1[e], f1, acc[e] * f0); }
@@ -1117,9 +1144,10 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
 #pragma unroll
   for (int cb = 0; cb < NCB; ++cb) { o[cb] = f32x16_t{}; }
   float m = -INFINITY;      // running max, raw score units
+  float mc = 0.0f;          // what the exponents have subtracted
+  float edge = -INFINITY;   // scores past it raise the maximum
   float l = 0.0f;           // this half's share of the running sum
   f32x16_t sc[2];           // scores of the current tile
-  float mb = -INFINITY;     // their max over the row (both halves)
 
   auto mask = [&](f32x16_t (&s)[2], int t) {
     const bool pre = t < ptiles;
@@ -1137,7 +1165,6 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
   };
   uint32_t pk[16];
   float ps;
-  float mc;
   auto expo = [&](const f32x16_t& s, int r, int slot) {
     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], scale, -mc));
     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], scale, -mc));
@@ -1161,13 +1188,13 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
     o[cb] = mma32(vf, pf, o[cb]);
   };
 
-  // One iteration over tile t: A scores of tile t + 1 | exponentials of keys
-  // 0..31; B P V of keys 0..31 | exponentials of keys 32..63; C P V of keys
-  // 32..63 | mask and max of tile t + 1's scores.
-  constexpr int EPA = 16 / NDS, EPB = 16 / (2 * NCB), MPC = 32 / (2 * NCB);
-  auto iteration = [&](int t, const uint16_t* kread, uint16_t* kfill, const uint16_t* vread,
-                       uint16_t* vfill) {
-    if (mb > m + lazy) {
+  // Raises the maximum to mb, that of the scores `s` of the tile that is next, where
+  // they pass it by enough.  It stands before an iteration's barrier: scores that
+  // change at the start of the next would be copied there (170 -> 177 us for 4096
+  // queries over 4096 keys, d = 64), and after the barrier all wait for the test.
+  auto raise = [&](float mb, f32x16_t (&s)[2]) {
+    if (mb > edge) {
+      mb = fmaxf(mb, m);
       const float alpha = exp2f((m - mb) * scale);     // 0 while m is -inf
       l *= alpha;
 #pragma unroll
@@ -1176,8 +1203,23 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
         for (int r = 0; r < 16; ++r) { o[cb][r] *= alpha; }
       }
       m = mb;
+      mc = m * scale;
+      edge = m + lazy;
+      if (fabsf(mc) > kFused) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) { s[r >> 4][r & 15] -= m; }
+        mc = 0.0f;
+        edge = -INFINITY;
+      }
     }
-    mc = m == -INFINITY ? 0.0f : m * scale;
+  };
+
+  // One iteration over tile t: A scores of tile t + 1 | exponentials of keys
+  // 0..31; B P V of keys 0..31 | exponentials of keys 32..63; C P V of keys
+  // 32..63 | mask and max of tile t + 1's scores.
+  constexpr int EPA = 16 / NDS, EPB = 16 / (2 * NCB), MPC = 32 / (2 * NCB);
+  auto iteration = [&](int t, const uint16_t* kread, uint16_t* kfill, const uint16_t* vread,
+                       uint16_t* vfill) {
     ps = 0.0f;
     copy(A.k, t + 2, kfill, koffs);
     copy(A.v, t + 1, vfill, voffs);
@@ -1239,7 +1281,7 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
       __builtin_amdgcn_sched_group_barrier(0x002, MPC / 2, 0);        // VALU
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);              // reads +2
     }
-    mb = max_halves(mx);
+    mx = max_halves(mx);
     l += ps;
     // Tiles t + 2 and t + 3 are next: from the end of a group on, its
     // successor.  The one after that is read here and looked at half a group
@@ -1255,6 +1297,7 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
         there1 = __ballot(ids1 >= 0);
       }
     }
+    if (t + 1 < ntiles) { raise(mx, sn); }
     __syncthreads();
     sc[0] = sn[0];
     sc[1] = sn[1];
@@ -1277,12 +1320,14 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
     float mx = sc[0][0];
 #pragma unroll
     for (int r = 1; r < 32; ++r) { mx = fmaxf(mx, sc[r >> 4][r & 15]); }
-    mb = max_halves(mx);
+    raise(max_halves(mx), sc);
     __syncthreads();
   }
-  for (int t = tbeg; t < ntiles; t += 2) {
+  for (int t = tbeg; t < ntiles;) {
     iteration(t, ks1, ks0, vs0, vs1);
-    if (t + 1 < ntiles) { iteration(t + 1, ks0, ks1, vs1, vs0); }
+    if (++t >= ntiles) { break; }
+    iteration(t, ks0, ks1, vs1, vs0);
+    ++t;
   }
 
   l = sum_halves(l);
@@ -1290,7 +1335,7 @@ tile_item(const PagedArgs& A, int b, int items, uint16_t* ks0, uint16_t* ks1, ui
   if (!direct) {
     const Part P = part_of(A, part);
     const long long at = part_row(A, S.first + tok, h);
-    if (half == 0) { P.ml[at] = make_float2(m * scale, sum_of(m, l)); }
+    if (half == 0) { P.ml[at] = make_float2(m, sum_of(m, l)); }
     if (sum_of(m, l) == kNoKey) { return; }
     float* op = P.o + at * D;
 #pragma unroll
@@ -1365,7 +1410,7 @@ in_sequence(const PagedArgs& A, int token)
 }
 
 // Adds the parts of a row, W waves a row, in the order of the parts:
-// out = sum f_p o_p / sum f_p l_p with f_p = 2^(m_p - max m).  All of a lane's
+// out = sum f_p o_p / sum f_p l_p with f_p = 2^((m_p - max m) scale).  All of a lane's
 // loads go out before the row is looked up.  Bound by latency and the parts'
 // bytes: 2048 rows of 7 parts 4.9 us, 8192 rows of 7 (30 MB) 12.4.
 template <int D, int W>
@@ -1391,7 +1436,8 @@ paged_combine_kernel(const PagedArgs A)
   auto add = [&](float m1, float l1, const float* o1) {
     if (l1 < 0.0f) { return; }
     const float top = fmaxf(m, m1);
-    const float f0 = __builtin_amdgcn_exp2f(m - top), f1 = __builtin_amdgcn_exp2f(m1 - top);
+    const float f0 = __builtin_amdgcn_exp2f((m - top) * A.scale);
+    const float f1 = __builtin_amdgcn_exp2f((m1 - top) * A.scale);
     l = __builtin_fmaf(l, f0, l1 * f1);
 #pragma unroll
     for (int e = 0; e < C; ++e) { o[e] = __builtin_fmaf(o1[e], f1, o[e] * f0); }
