@@ -527,6 +527,23 @@ def _table(t, device, name):
     return t.data_ptr()
 
 
+def _meet(a, b, n, pitch_a, width_a, pitch_b, width_b):
+    """Whether rows of two matrices share an element: n rows each of `width`
+    elements, `pitch` apart, from the byte addresses a and b.  (Pitches below the
+    width are the library's to refuse.)"""
+    if b < a:
+        a, b, pitch_a, width_a, pitch_b, width_b = b, a, pitch_b, width_b, pitch_a, width_a
+    apart = (b - a) // 2
+    if apart >= (n - 1) * pitch_a + width_a or n == 0 or pitch_a < width_a or pitch_b < width_b:
+        return False
+    if pitch_a != pitch_b and n > 1:
+        return any(at % pitch_a < width_a or at % pitch_a + width_b > pitch_a
+                   for at in range(apart, min(apart + n * pitch_b, (n - 1) * pitch_a + width_a),
+                                   pitch_b))
+    row, at = divmod(apart, pitch_a)
+    return at < width_a or (row + 1 < n and at + width_b > pitch_a)
+
+
 class Rope:
     """A rotation (u15h_rope_spec), kept from call to call: `parts` is one to
     three (freq, start, axis), freq a device f64 tensor as rope_freqs makes it,
@@ -1356,7 +1373,6 @@ class Ops:
                                 dst.numel())
         self._check(st, "u15h_add")
 
-    # ---- attention -------------------------------------------------------
     # ---- many requests at once ----------------------------------------------
     # (one pass over a tensor's properties each: these calls' checks are as long
     # as their launches)
@@ -1396,7 +1412,7 @@ class Ops:
     def rope(self, x, pos, rope, y, inverse=False, stream=None):
         """y = x [tokens][heads][head_dim] turned by its tokens' positions
         [axes][tokens] (int32), or turned back; any strides between tokens and
-        heads; y may be x."""
+        heads; y may be x, and otherwise may not overlap it."""
         dev = self.device
         if x.dtype is not _BF16 or y.dtype is not _BF16 or x.get_device() != dev or \
                 y.get_device() != dev:
@@ -1408,8 +1424,12 @@ class Ops:
         if (xs[2] != 1 or ys[2] != 1) and d > 1:
             raise ValueError("the columns of x and y must be contiguous")
         rp, pp = self._turn(rope, pos, tokens)
-        st = self._lib.u15h_rope(self._ctx, self._stream_here(stream), rp, pp, x.data_ptr(),
-                                 xs[0], xs[1], y.data_ptr(), ys[0], ys[1], tokens, heads, d,
+        xp, yp = x.data_ptr(), y.data_ptr()
+        if xp != yp and abs(yp - xp) < 2 * tokens * (xs[0] + ys[0]) and xs[1] == d == ys[1] and \
+                _meet(xp, yp, tokens, xs[0], heads * d, ys[0], heads * d):
+            raise ValueError("y may be x, but not overlap it otherwise")
+        st = self._lib.u15h_rope(self._ctx, self._stream_here(stream), rp, pp, xp,
+                                 xs[0], xs[1], yp, ys[0], ys[1], tokens, heads, d,
                                  inverse)
         if st:
             self._check(st, "u15h_rope")
@@ -1419,7 +1439,8 @@ class Ops:
         """k [tokens][kv_heads][head_dim], turned, and v into the cache's slots
         (int32 [tokens], page * page size + place; tokens whose slot is no
         place are passed over), and q_out = q [tokens][heads][head_dim]
-        turned.  Rows may be columns of a wider matrix; q_out may be q."""
+        turned.  Rows may be columns of a wider matrix; q_out may be q, and
+        otherwise may not overlap q, k or v."""
         if kv.device != self.device:
             raise ValueError(f"the cache is on cuda:{kv.device}, this context on "
                              f"cuda:{self.device}")
@@ -1440,6 +1461,11 @@ class Ops:
             op, os_, on, oh, od = self._rows(q_out, "q_out")
             if n != tokens or on != tokens or oh != hq or qd != d or od != d:
                 raise ValueError(f"q and q_out must be [{tokens}][heads][{d}]")
+            wide, own, near = hq * d, h * d, 2 * n * (qs + os_ + ks + vs)
+            if (op != qp and abs(op - qp) < near and _meet(qp, op, n, qs, wide, os_, wide)) or \
+                    (abs(op - kp) < near and _meet(kp, op, n, ks, own, os_, wide)) or \
+                    (abs(op - vp) < near and _meet(vp, op, n, vs, own, os_, wide)):
+                raise ValueError("q_out may be q, but not overlap q, k or v otherwise")
         elif q_out is not None:
             raise ValueError("q_out without q")
         st = self._lib.u15h_paged_append(
@@ -1451,7 +1477,8 @@ class Ops:
     def paged_attention(self, kv, batch, q, out, scale=0.0, causal=True, stream=None):
         """out = softmax(q . k * scale) . v for every sequence of the batch over
         the shared prefix and its own keys; q, out [tokens][heads][head_dim]
-        (rows may be columns of a wider matrix); scale 0: 1/sqrt(head_dim)."""
+        (rows may be columns of a wider matrix); scale 0: 1/sqrt(head_dim).
+        out may not overlap q, whose rows other workgroups still read."""
         if kv.device != self.device or batch.device != self.device:
             raise ValueError(f"cache on cuda:{kv.device}, batch on cuda:{batch.device}, this "
                              f"context on cuda:{self.device}")
@@ -1459,6 +1486,8 @@ class Ops:
         op, os_, on, oh, od = self._rows(out, "out")
         if d != kv.head_dim or on != n or oh != h or od != d:
             raise ValueError(f"q and out must be [tokens][heads][{kv.head_dim}]")
+        if abs(op - qp) < 2 * n * (qs + os_) and _meet(qp, op, n, qs, h * d, os_, h * d):
+            raise ValueError("out may not overlap q")
         b = batch._b
         room = batch.width * kv.page
         most = room if batch.max_kv is None else batch.max_kv
@@ -1471,6 +1500,7 @@ class Ops:
         if st:
             self._check(st, "u15h_paged_attention")
 
+    # ---- attention -------------------------------------------------------
     def sdpa(self, q, k, v, out, hkv, tk, causal=False, q_offset=0,
              stream=None):
         """MetalOps::sdpa / sdpa_steel: q, out [hq][tq][d]; k, v caches
