@@ -1425,8 +1425,8 @@ class Ops:
             raise ValueError("the columns of x and y must be contiguous")
         rp, pp = self._turn(rope, pos, tokens)
         xp, yp = x.data_ptr(), y.data_ptr()
-        if xp != yp and abs(yp - xp) < 2 * tokens * (xs[0] + ys[0]) and xs[1] == d == ys[1] and \
-                _meet(xp, yp, tokens, xs[0], heads * d, ys[0], heads * d):
+        if xp != yp and yp < xp + 2 * tokens * xs[0] and xp < yp + 2 * tokens * ys[0] and \
+                xs[1] == d == ys[1] and _meet(xp, yp, tokens, xs[0], heads * d, ys[0], heads * d):
             raise ValueError("y may be x, but not overlap it otherwise")
         st = self._lib.u15h_rope(self._ctx, self._stream_here(stream), rp, pp, xp,
                                  xs[0], xs[1], yp, ys[0], ys[1], tokens, heads, d,
@@ -1461,10 +1461,14 @@ class Ops:
             op, os_, on, oh, od = self._rows(q_out, "q_out")
             if n != tokens or on != tokens or oh != hq or qd != d or od != d:
                 raise ValueError(f"q and q_out must be [{tokens}][heads][{d}]")
-            wide, own, near = hq * d, h * d, 2 * n * (qs + os_ + ks + vs)
-            if (op != qp and abs(op - qp) < near and _meet(qp, op, n, qs, wide, os_, wide)) or \
-                    (abs(op - kp) < near and _meet(kp, op, n, ks, own, os_, wide)) or \
-                    (abs(op - vp) < near and _meet(vp, op, n, vs, own, os_, wide)):
+            n2 = 2 * n
+            end = op + n2 * os_
+            if (qp < end and op < qp + n2 * qs and op != qp and
+                _meet(qp, op, n, qs, hq * d, os_, hq * d)) or \
+                    (kp < end and op < kp + n2 * ks and
+                     _meet(kp, op, n, ks, h * d, os_, hq * d)) or \
+                    (vp < end and op < vp + n2 * vs and
+                     _meet(vp, op, n, vs, h * d, os_, hq * d)):
                 raise ValueError("q_out may be q, but not overlap q, k or v otherwise")
         elif q_out is not None:
             raise ValueError("q_out without q")
@@ -1486,7 +1490,8 @@ class Ops:
         op, os_, on, oh, od = self._rows(out, "out")
         if d != kv.head_dim or on != n or oh != h or od != d:
             raise ValueError(f"q and out must be [tokens][heads][{kv.head_dim}]")
-        if abs(op - qp) < 2 * n * (qs + os_) and _meet(qp, op, n, qs, h * d, os_, h * d):
+        if op < qp + 2 * n * qs and qp < op + 2 * n * os_ and \
+                _meet(qp, op, n, qs, h * d, os_, h * d):
             raise ValueError("out may not overlap q")
         b = batch._b
         room = batch.width * kv.page
