@@ -888,16 +888,6 @@ u15h_create(int device, u15h_ctx** out)
     ctx->attn_ws = nullptr;
     (void)hipGetLastError();
   }
-  // env U15H_ATTN_FILL: the byte that the scratch and its counters start as, in
-  // place of whatever the memory holds: no call may rely on that.
-  const int fill = env_int("U15H_ATTN_FILL", -1);
-  if (ctx->attn_ws != nullptr && fill >= 0 &&
-      (hipMemset(ctx->attn_ws, fill, kAttnWsBytes + kAttnCountBytes) != hipSuccess ||
-       hipDeviceSynchronize() != hipSuccess)) {
-    u15h_destroy(ctx);
-    if (prev >= 0 && prev != device) { (void)hipSetDevice(prev); }
-    return U15H_ELAUNCH;
-  }
   if (prev >= 0 && prev != device) { (void)hipSetDevice(prev); }
   *out = ctx;
   return U15H_OK;
