@@ -164,8 +164,12 @@ cut(long long keys, long long n, int* shares, int* chunk)
 
 // How a call is cut (PagedArgs): what the prefix's workgroups and the
 // sequences' walk.  Lengths are known to their bounds only; own keys are taken
-// as half of max_kv on the mean.  Measured in a graph, 32 query heads over 8 of
-// 128 unless said, us:
+// as half of max_kv on the mean, and a share's keys are fixed here.  So a bound
+// far above the lengths leaves few shares with keys: one request of 4000 keys
+// takes 10.9 us where max_kv is 4000, 13.7 at 16384 and 42 at 131072, four of them
+// 18, 25 and 78, 32 of 1 to 4000 keys 51, 113 and 113.  The figures below have
+// max_kv at the longest sequence.  In a graph, 32 query heads over 8 of 128 unless
+// said, us:
 //  - the prefix once for all / by every sequence: 4 queries behind 8192 keys 13.2
 //    / 19.7, 128 behind 500 25 / 35, 20 of 8 queries behind 4000 30 / 44; below
 //    4096 keys walked again, 8 behind 256 11.1 / 8.0, 2 behind 600 11.0 / 11.1;
@@ -481,8 +485,9 @@ u15h_paged_attention(u15h_ctx* ctx, u15h_stream stream, const u15h_paged_kv* kv,
   for (const int32_t* p : {bt->q_start, bt->kv_len, bt->table, bt->prefix_table}) {
     if (!aligned(p, 4)) { return refuse(ctx, "%s: tables must be 4-byte aligned", what); }
   }
-  // rows are counted in 32 bits; each sequence has up to 4 streaming workgroups
-  // and a tile workgroup more than its rows fill
+  // rows are counted in 32 bits; a sequence counts as 5 workgroups a kv head (at
+  // most 2 streaming ones and a tile one that its rows do not fill are launched;
+  // shares are planned only while they are few), its rows as whole tiles
   const long long groups =
       ((long long)bt->batch * 5 + (long long)bt->tokens * (hq / kv->kv_heads) / 128) *
       kv->kv_heads;

@@ -599,8 +599,9 @@ class PagedBatch:
     [batch] and table [batch][pages of a sequence] int32; q_start [batch + 1],
     or None for one query each; the shared prefix's pages and length.  max_q
     and max_kv bound the queries and own keys of a sequence (max_kv: the
-    table's width where not given).  The tensors may be rewritten in place
-    between calls or replays."""
+    table's width where not given; near the longest sequence is fastest, as
+    keys are split by it).  The tensors may be rewritten in place between calls
+    or replays."""
 
     def __init__(self, kv_len, table, q_start=None, max_q=1, max_kv=None, prefix_table=None,
                  prefix_len=0):
@@ -1411,8 +1412,8 @@ class Ops:
 
     def rope(self, x, pos, rope, y, inverse=False, stream=None):
         """y = x [tokens][heads][head_dim] turned by its tokens' positions
-        [axes][tokens] (int32), or turned back; any strides between tokens and
-        heads; y may be x, and otherwise may not overlap it."""
+        [axes][tokens] (int32), or by their negatives (the gradient); any
+        strides between tokens and heads; y may be x, and otherwise may not overlap it."""
         dev = self.device
         if x.dtype is not _BF16 or y.dtype is not _BF16 or x.get_device() != dev or \
                 y.get_device() != dev:
