@@ -342,8 +342,9 @@ constexpr float kLazy = 8.0f;
 // rounded: to 2^10 that is at most 2^-14 of a weight, but it grows with the product
 // and past 2^31 exceeds the exponential's range, 2^127 and 0 in place of 1.  So above
 // 2^10 they are (score - max) * scale, 0 at the maximum whatever the scale: such a
-// row takes the maximum's branch at every tile, and other rows pay nothing (269 us
-// for 4096 queries over 4096 keys, as without it; a test of its own: 276).
+// row takes the maximum's branch at every tile (2 to 3% of a call whose rows are all
+// such), and other rows pay nothing (269 us for 4096 queries over 4096 keys, as
+// without it; a test of its own: 276).
 constexpr float kFused = 1024.0f;
 
 __device__ __forceinline__ f32x4_t
